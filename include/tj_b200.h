@@ -198,6 +198,94 @@ TJ_API int tj_b200_ipc_open(const tj_ipc_handle* handle, uint64_t offset, int32_
  * have synchronised every stream that still writes through it. */
 TJ_API int tj_b200_ipc_close(void* dptr, uint64_t offset, int32_t device);
 
+/* ---------------------------------------------------------------------------------------------
+ * Serving operators: rotary positions, a paged cache of keys and values, attention over it.
+ * No counterpart in the reference (its programs have no state between calls).  They launch one
+ * kernel each on `stream` (a cudaStream_t of the current device), allocate nothing and wait for
+ * nothing.  Extents and strides are in elements.  Host-side faults return TJ_ERR_INVALID before
+ * anything is launched.  What only the device can see (a slot, position, page or length out of
+ * range) is skipped there and recorded in status words, read by tj_b200_serving_status. */
+enum { TJ_F32 = 0, TJ_F16 = 1, TJ_BF16 = 2, TJ_I8 = 3, TJ_E4M3 = 4 };
+
+/* A pool of `pages` pages of `page_size` slots; slot s is place s % page_size of page
+ * s / page_size.  k and v share their strides, element 1 apart along the head dim.  dtype f16 or
+ * bf16 (no scales), or i8 or e4m3 with one f32 scale for each (slot, head): value = code * scale. */
+typedef struct tj_kv_cache {
+  void* k;
+  void* v;
+  float* k_scale;
+  float* v_scale;
+  int64_t pages, page_size, heads, dim;
+  int64_t page_stride, slot_stride, head_stride;
+  int64_t scale_page, scale_slot, scale_head;
+  int64_t dtype;
+} tj_kv_cache;
+
+/* Rows [tokens, heads, dim] of queries, keys and values.  rot: how many leading elements of q's and
+ * k's rows are turned (0: none), by the angles whose cosines and sines are table[position][0 .. rot/2)
+ * and [rot/2 .. rot).  interleaved: pairs (2i, 2i + 1), else (i, i + rot/2).  inverse: the other way. */
+typedef struct tj_rows {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* q_out;
+  void* k_out;
+  const int32_t* slots;     /* [tokens] cache slots; negative: the token is not written */
+  const int32_t* positions; /* [tokens] */
+  const float* table;       /* [table_rows, rot] */
+  int64_t tokens, q_heads, kv_heads, dim, rot, table_rows;
+  int64_t q_token, q_head, k_token, k_head, v_token, v_head, qo_token, qo_head, ko_token, ko_head;
+  int64_t dtype, interleaved, inverse;
+  tj_kv_cache cache;
+} tj_rows;
+
+/* q (and k, unless NULL) turned into q_out (k_out), which may be q (k) itself. */
+TJ_API int tj_b200_rotary(const tj_rows* args, void* stream);
+
+/* k and v into the cache's slots, quantised if the cache is; with rot > 0 the keys are turned first,
+ * and q (unless NULL) is turned into q_out. */
+TJ_API int tj_b200_cache_write(const tj_rows* args, void* stream);
+
+/* Slots' keys and values as dense rows [count, heads, dim] of `dtype`; a negative slot reads as 0. */
+TJ_API int tj_b200_cache_read(const tj_kv_cache* cache, const int32_t* slots, int64_t count, void* k_out, void* v_out,
+                              int32_t dtype, void* stream);
+
+/* Attention of new tokens over the cache.  Sequence b's new tokens are rows q_starts[b] .. q_starts[b+1]
+ * of q (q_starts NULL: one token each, row b); they stand at the end of its kv_lens[b] keys, which lie
+ * in pages page_table[b * table_row + i].  causal: a token sees the keys up to its own position;
+ * window > 0: the last `window` of those.  A row that sees nothing is 0 (lse: -inf).
+ * counters: int32, zero before the first call and left zero by every call; workspace: anything.
+ * Calls that share them must not overlap.  max_new: no sequence has more new tokens. */
+typedef struct tj_paged_attention {
+  const void* q;  /* [tokens, q_heads, dim], the 16-bit type `dtype` */
+  void* out;      /* the same */
+  float* lse;     /* [tokens, q_heads] or NULL: log of the sum of exponentials */
+  const int32_t* page_table;
+  const int32_t* kv_lens;
+  const int32_t* q_starts;
+  void* workspace;
+  int32_t* counters;
+  int64_t tokens, batch, q_heads, max_new;
+  int64_t table_row, table_width;
+  int64_t q_token, q_head, out_token, out_head;
+  int64_t dtype, causal, window;
+  double scale;
+  int64_t workspace_bytes, counters_count;
+  tj_kv_cache cache;
+} tj_paged_attention;
+
+TJ_API int tj_b200_paged_attention(const tj_paged_attention* args, void* stream);
+
+/* What a call with these arguments needs (its workspace and counters fields are not read). */
+TJ_API int tj_b200_paged_attention_workspace(const tj_paged_attention* args, int64_t* workspace_bytes,
+                                             int64_t* counters_count);
+
+/* Waits for `stream`, reads the serving operators' status words of the current device and clears
+ * them: TJ_OK and *code = 0, or TJ_ERR_DEVICE_STATUS with *code (1 wait timeout, 2 index out of range)
+ * and *where = operator * 16 + site (operators 0 rotary, 1 write, 2 read, 3 attention; sites 1 slot,
+ * 2 position, 3 page, 4 length, 5 and up a wait). */
+TJ_API int tj_b200_serving_status(int32_t* code, int32_t* where, void* stream);
+
 /* Message of the last failure on this thread ("" if none). */
 TJ_API const char* tj_b200_last_error(void);
 

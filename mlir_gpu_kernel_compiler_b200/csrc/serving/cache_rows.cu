@@ -1,0 +1,547 @@
+// Rotary positions, and the paged cache's writes and reads: everything a decoder does to the
+// rows (token, head) of its queries, keys and values besides attending.
+//
+// Mathematics.  A row's first `rot` elements are rot / 2 pairs, (2i, 2i + 1) or (i, i + rot / 2);
+// each is turned by the angle of the token's position and the pair's frequency, whose cosine and
+// sine the table holds in f32:  a' = a c - b s,  b' = b c + a s  (inverse: s -> -s, which is also
+// the gradient).  A quantised cache keeps, of each row, x = code * scale with scale = max|x| / 127
+// (i8, code = x / scale to the nearest even integer) or max|x| / 448 (e4m3, code rounded to
+// nearest even).  Products and the sum are rounded one by one (no FMA) and quotients are IEEE
+// divisions, so the codes are the same for every layout of the work and equal those of the same
+// formulas evaluated elementwise in f32.
+//
+// One kernel does them all, because they read the same rows: with rotary positions and a cache
+// write in one launch the rotated keys never travel through memory, and single-token steps, whose
+// cost is the launch, pay for one.
+//
+// Layout.  A row is cut into slots of two 8-element units; a lane holds one slot, so a rotary
+// pair (half layout: units u and u + rot / 16) is in one lane's registers, max|x| is a shuffle
+// over the row's lanes, and every access is 16 bytes.  A lane keeps its slot's cosines and sines
+// in registers over the heads of its token: the table is read once per token, not once per row.
+// A warp takes 32 / lanes rows at a time, `batch` of them before it stores.
+#include "serving_common.cuh"
+
+static __device__ __align__(16) int tj_serving_words[4];
+
+namespace tjs {
+
+struct RowsParams {
+  tj_rows a;
+  int* status;
+  int lanes_log2;  // lanes of a row
+  int slots;       // slots of a row: ceil(dim / 16)
+  int iters;       // warp iterations over a token's rows
+  int segs;        // warps that share a token
+  int op;
+};
+
+// a plain (coherent) load that stays out of L1: rows are read once, and may be written in place
+TJ_DEV uint4 ld16_row(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p)
+               : "memory");
+  return v;
+}
+TJ_DEV void load8(const float* p, float* f) {
+  tj_unpack(ld16_row(p), f, p);
+  tj_unpack(ld16_row(p + 4), f + 4, p);
+}
+template <class T> TJ_DEV void load8(const T* p, float* f) { tj_unpack(ld16_row(p), f, p); }
+TJ_DEV void store8(float* p, const float* f) {
+  tj_store_vec(p, f);
+  tj_store_vec(p + 4, f + 4);
+}
+template <class T> TJ_DEV void store8(T* p, const float* f) { tj_store_vec(p, f); }
+
+TJ_DEV uint32_t e4m3x4(const float* f) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+TJ_DEV uint32_t i8x4(const float* f) {
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w |= static_cast<uint32_t>(max(-127, min(127, __float2int_rn(f[i]))) & 0xff) << (8 * i);
+  return w;
+}
+
+// ROT: 0 none; 1 half layout, whole units; 2 interleaved, whole units; 3 either, any even rot
+// (pairs that cross units: partners and table entries one by one).
+template <class T, int ROT>
+__global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ RowsParams p) {
+  const tj_rows& a = p.a;
+  const int lane = threadIdx.x & 31;
+  const long wid = static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const long token = wid / p.segs;
+  const int seg = static_cast<int>(wid - token * p.segs);
+  if (token >= a.tokens) return;
+  const int dim = static_cast<int>(a.dim), rot = static_cast<int>(a.rot), half = rot >> 1;
+  const int lpr = 1 << p.lanes_log2, sub = lane >> p.lanes_log2, per = 32 >> p.lanes_log2, s = lane & (lpr - 1);
+  const bool on = s < p.slots;
+
+  // the slot's two units (ua < 0 or ub < 0: none)
+  int ua = 2 * s, ub = 2 * s + 1;
+  if (ROT == 1) {
+    const int pairs = rot >> 4;
+    if (s < pairs) {
+      ua = s;
+      ub = s + pairs;
+    } else {
+      ua = 2 * pairs + 2 * (s - pairs);
+      ub = ua + 1;
+    }
+  }
+  const bool has_b = on && ub * 8 < dim;
+
+  float cs[8] = {}, sn[8] = {};
+  const float* trow = nullptr;
+  bool lost = false;  // a position outside the table: the row becomes NaN
+  if (ROT) {
+    const int pos = a.positions[token];
+    lost = pos < 0 || pos >= a.table_rows;
+    if (lost) {
+      if (lane == 0) tj_report(p.status, TJ_STATUS_BOUNDS, p.op * 16 + SITE_POSITION);
+    }
+    trow = a.table + (lost ? 0 : static_cast<long>(pos) * rot);
+    const float sign = a.inverse ? -1.0f : 1.0f;
+    if (ROT == 1 && on && ua * 8 < half) {
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        tj_unpack(tj_ld16(trow + ua * 8 + i), cs + i, (const float*)nullptr);
+        tj_unpack(tj_ld16(trow + half + ua * 8 + i), sn + i, (const float*)nullptr);
+      }
+    }
+    if (ROT == 2 && on) {  // unit u holds pairs 4u .. 4u + 3
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int u = i ? ub : ua;
+        if (u * 8 < rot) {
+          tj_unpack(tj_ld16(trow + u * 4), cs + 4 * i, (const float*)nullptr);
+          tj_unpack(tj_ld16(trow + half + u * 4), sn + 4 * i, (const float*)nullptr);
+        }
+      }
+    }
+    if (ROT != 3) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        sn[i] *= sign;
+        if (lost) cs[i] = sn[i] = __int_as_float(0x7fffffff);
+      }
+    }
+  }
+  long crow = -1, srow = 0;
+  if (a.slots) {
+    const int slot = a.slots[token];
+    const long cap = a.cache.pages * a.cache.page_size;
+    if (slot >= 0 && slot < cap) {
+      const int page = slot / static_cast<int>(a.cache.page_size), at = slot - page * static_cast<int>(a.cache.page_size);
+      crow = page * a.cache.page_stride + at * a.cache.slot_stride;
+      srow = page * a.cache.scale_page + at * a.cache.scale_slot;
+    } else if (slot >= cap && lane == 0) {
+      tj_report(p.status, TJ_STATUS_BOUNDS, p.op * 16 + SITE_SLOT);
+    }
+  }
+
+  const int nq = a.q ? static_cast<int>(a.q_heads) : 0, nk = a.k ? static_cast<int>(a.kv_heads) : 0,
+            nv = a.v ? static_cast<int>(a.kv_heads) : 0;
+  const int rows = nq + nk + nv;
+  const int i0 = static_cast<int>(static_cast<long>(seg) * p.iters / p.segs),
+            i1 = static_cast<int>(static_cast<long>(seg + 1) * p.iters / p.segs);
+  constexpr int BATCH = 4;
+  for (int it = i0; it < i1; it += BATCH) {
+    float x[BATCH][16];
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      const int r = (it + j) * per + sub;
+      if (it + j < i1 && r < rows && on) {
+        const T* src = r < nq          ? static_cast<const T*>(a.q) + token * a.q_token + r * a.q_head
+                       : r < nq + nk ? static_cast<const T*>(a.k) + token * a.k_token + (r - nq) * a.k_head
+                                     : static_cast<const T*>(a.v) + token * a.v_token + (r - nq - nk) * a.v_head;
+        load8(src + ua * 8, x[j]);
+        if (has_b) {
+          load8(src + ub * 8, x[j] + 8);
+        } else {
+#pragma unroll
+          for (int i = 8; i < 16; ++i) x[j][i] = 0.0f;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[j][i] = 0.0f;
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      const int r = (it + j) * per + sub;
+      const bool mine = it + j < i1 && r < rows && on;
+      if (ROT == 1 && mine && r < nq + nk && ua * 8 < half) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float u = x[j][i], v = x[j][i + 8];
+          x[j][i] = __fsub_rn(__fmul_rn(u, cs[i]), __fmul_rn(v, sn[i]));
+          x[j][i + 8] = __fadd_rn(__fmul_rn(v, cs[i]), __fmul_rn(u, sn[i]));
+        }
+      }
+      if (ROT == 2 && mine && r < nq + nk) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          if ((i < 4 ? ua : ub) * 8 < rot) {
+            const float u = x[j][2 * i], v = x[j][2 * i + 1];
+            x[j][2 * i] = __fsub_rn(__fmul_rn(u, cs[i]), __fmul_rn(v, sn[i]));
+            x[j][2 * i + 1] = __fadd_rn(__fmul_rn(v, cs[i]), __fmul_rn(u, sn[i]));
+          }
+        }
+      }
+      if (ROT == 3) {
+        if (mine && r < nq + nk) {
+          const T* src = r < nq ? static_cast<const T*>(a.q) + token * a.q_token + r * a.q_head
+                                : static_cast<const T*>(a.k) + token * a.k_token + (r - nq) * a.k_head;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const int e = (i < 8 ? ua : ub) * 8 + (i & 7);
+            if (e >= rot || (i >= 8 && !has_b)) continue;
+            const bool second = a.interleaved ? (e & 1) : e >= half;
+            const int pair = a.interleaved ? e >> 1 : (second ? e - half : e);
+            const int other = a.interleaved ? e ^ 1 : (second ? e - half : e + half);
+            float c = trow[pair], sv = trow[half + pair] * (a.inverse ? -1.0f : 1.0f);
+            if (lost) c = sv = __int_as_float(0x7fffffff);
+            // re-read: the partner may be in another lane, and x[j] is overwritten in place
+            const float mate = tj_f32(src[other]), own = tj_f32(src[e]);
+            x[j][i] = second ? __fadd_rn(__fmul_rn(own, c), __fmul_rn(mate, sv))
+                             : __fsub_rn(__fmul_rn(own, c), __fmul_rn(mate, sv));
+          }
+        }
+        __syncwarp();  // every lane has read the row before any lane stores over it (outputs in place)
+      }
+      const bool to_cache = a.slots && r >= nq;
+      if (!to_cache) {
+        if (mine) {
+          T* dst = r < nq ? static_cast<T*>(a.q_out) + token * a.qo_token + r * a.qo_head
+                          : static_cast<T*>(a.k_out) + token * a.ko_token + (r - nq) * a.ko_head;
+          store8(dst + ua * 8, x[j]);
+          if (has_b) store8(dst + ub * 8, x[j] + 8);
+        }
+      }
+      if (!a.slots) continue;
+      const bool key = r < nq + nk;
+      const int h = key ? r - nq : r - nq - nk;
+      void* base = key ? a.cache.k : a.cache.v;
+      const long off = crow + h * a.cache.head_stride;
+      const bool put = mine && to_cache && crow >= 0;
+      if (a.cache.dtype == TJ_BF16 || a.cache.dtype == TJ_F16) {
+        if (put) {
+          if (a.cache.dtype == TJ_BF16) {
+            store8(static_cast<__nv_bfloat16*>(base) + off + ua * 8, x[j]);
+            if (has_b) store8(static_cast<__nv_bfloat16*>(base) + off + ub * 8, x[j] + 8);
+          } else {
+            store8(static_cast<__half*>(base) + off + ua * 8, x[j]);
+            if (has_b) store8(static_cast<__half*>(base) + off + ub * 8, x[j] + 8);
+          }
+        }
+      } else {
+        // max|x| over the row's lanes, as bits: an infinity or a NaN orders above every number
+        uint32_t top = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[j][i]) & 0x7fffffffu);
+        for (int o = lpr >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const bool i8 = a.cache.dtype == TJ_I8;
+        float scale = __fdiv_rn(__uint_as_float(top), i8 ? 127.0f : 448.0f);
+        if (put) {
+          // a row with an infinity or a NaN is held as NaN (scale) times zero codes
+          const bool bad = top >= 0x7f800000u;
+          if (bad) scale = __int_as_float(0x7fffffff);
+          const bool zero = bad || scale == 0.0f;
+          float y[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) y[i] = zero ? 0.0f : __fdiv_rn(x[j][i], scale);
+          uint8_t* dst = static_cast<uint8_t*>(base) + off;
+          uint2 w0, w1;
+          if (i8) {
+            w0 = make_uint2(i8x4(y), i8x4(y + 4));
+            w1 = make_uint2(i8x4(y + 8), i8x4(y + 12));
+          } else {
+            w0 = make_uint2(e4m3x4(y), e4m3x4(y + 4));
+            w1 = make_uint2(e4m3x4(y + 8), e4m3x4(y + 12));
+          }
+          *reinterpret_cast<uint2*>(dst + ua * 8) = w0;
+          if (has_b) *reinterpret_cast<uint2*>(dst + ub * 8) = w1;
+          if (s == 0) (key ? a.cache.k_scale : a.cache.v_scale)[srow + h * a.cache.scale_head] = scale;
+        }
+      }
+    }
+  }
+}
+
+struct ReadParams {
+  tj_kv_cache c;
+  const int* slots;
+  void* out[2];
+  long rows;  // n * heads
+  int* status;
+  int lanes_log2, slots_per_row, batch;
+};
+
+// Rows (slot, head) of the keys and of the values back as T: value = code * scale in f32, rounded
+// once.  CD: the cache's dtype.  A slot of -1 reads as zeros.
+template <class T, int CD>
+__global__ void __launch_bounds__(128) read_kernel(const __grid_constant__ ReadParams p) {
+  const int lane = threadIdx.x & 31;
+  const int lpr = 1 << p.lanes_log2, sub = lane >> p.lanes_log2, per = 32 >> p.lanes_log2, s = lane & (lpr - 1);
+  const int dim = static_cast<int>(p.c.dim), heads = static_cast<int>(p.c.heads);
+  const bool on = s < p.slots_per_row, has_b = s * 16 + 8 < dim;
+  const bool val = blockIdx.y;
+  const char* base = static_cast<const char*>(val ? p.c.v : p.c.k);
+  const float* scales = val ? p.c.v_scale : p.c.k_scale;
+  T* out = static_cast<T*>(p.out[val]);
+  constexpr int BATCH = 4, ES = CD == TJ_I8 || CD == TJ_E4M3 ? 1 : 2;
+  const bool wide = ES == 2 || (dim % 16 == 0 && (p.c.page_stride | p.c.slot_stride | p.c.head_stride) % 16 == 0);
+  const long first = (static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 5)) * p.batch * per + sub;
+  uint4 raw[BATCH][2];
+  float scale[BATCH];
+#pragma unroll
+  for (int j = 0; j < BATCH; ++j) {
+    const long r = first + static_cast<long>(j) * per;
+    raw[j][0] = raw[j][1] = make_uint4(0, 0, 0, 0);
+    scale[j] = 1.0f;
+    if (j >= p.batch || r >= p.rows) continue;
+    const long n = r / heads;
+    const int h = static_cast<int>(r - n * heads), slot = p.slots[n];
+    if (slot < 0) continue;
+    if (slot >= p.c.pages * p.c.page_size) {
+      if (s == 0) tj_report(p.status, TJ_STATUS_BOUNDS, OP_CACHE_READ * 16 + SITE_SLOT);
+      continue;
+    }
+    const int page = slot / static_cast<int>(p.c.page_size), at = slot - page * static_cast<int>(p.c.page_size);
+    const char* src = base + (page * p.c.page_stride + at * p.c.slot_stride + h * p.c.head_stride + s * 16) * ES;
+    if (on) {
+      if (ES == 2) {
+        raw[j][0] = tj_ld16_stream(src);
+        if (has_b) raw[j][1] = tj_ld16_stream(src + 16);
+      } else if (wide) {
+        raw[j][0] = tj_ld16_stream(src);
+      } else {
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
+        uint2 w2 = make_uint2(0, 0);
+        if (has_b) w2 = __ldg(reinterpret_cast<const uint2*>(src + 8));
+        raw[j][0] = make_uint4(w.x, w.y, w2.x, w2.y);
+      }
+    }
+    if (ES == 1) scale[j] = scales[page * p.c.scale_page + at * p.c.scale_slot + h * p.c.scale_head];
+  }
+#pragma unroll
+  for (int j = 0; j < BATCH; ++j) {
+    const long r = first + static_cast<long>(j) * per;
+    if (j >= p.batch || r >= p.rows || !on) continue;
+    float x[16];
+    if constexpr (CD == TJ_BF16) {
+      tj_unpack(raw[j][0], x, (const __nv_bfloat16*)nullptr);
+      tj_unpack(raw[j][1], x + 8, (const __nv_bfloat16*)nullptr);
+    } else if constexpr (CD == TJ_F16) {
+      tj_unpack(raw[j][0], x, (const __half*)nullptr);
+      tj_unpack(raw[j][1], x + 8, (const __half*)nullptr);
+    } else {
+      const uint32_t w[4] = {raw[j][0].x, raw[j][0].y, raw[j][0].z, raw[j][0].w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (CD == TJ_I8) {
+#pragma unroll
+          for (int b = 0; b < 4; ++b) x[4 * i + b] = static_cast<float>(static_cast<int8_t>(w[i] >> (8 * b)));
+        } else {
+          __nv_fp8x4_e4m3 q;
+          q.__x = w[i];
+          const float4 f = static_cast<float4>(q);
+          x[4 * i] = f.x;
+          x[4 * i + 1] = f.y;
+          x[4 * i + 2] = f.z;
+          x[4 * i + 3] = f.w;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) x[i] *= scale[j];
+    }
+    T* dst = out + r * dim + s * 16;
+    store8(dst, x);
+    if (has_b) store8(dst + 8, x + 8);
+  }
+}
+
+struct Setup {
+  std::once_flag once;
+  Device dev{};
+  cudaError_t err = cudaSuccess;
+};
+Setup g_devices[MAX_DEVICES];
+
+int current_device(Device* out) {
+  int d = 0;
+  const cudaError_t e = cudaGetDevice(&d);
+  if (e != cudaSuccess) return refuse(TJ_ERR_CUDA, "serving", cudaGetErrorString(e));
+  if (d < 0 || d >= MAX_DEVICES) return refuse(TJ_ERR_INVALID, "serving", "device index out of range");
+  Setup& s = g_devices[d];
+  try {
+    std::call_once(s.once, [&] {
+      void* w = nullptr;
+      s.err = cudaGetSymbolAddress(&w, tj_serving_words);
+      if (s.err == cudaSuccess) s.err = cudaDeviceGetAttribute(&s.dev.sms, cudaDevAttrMultiProcessorCount, d);
+      s.dev.index = d;
+      s.dev.status = static_cast<int*>(w);
+    });
+  } catch (...) {  // nothing may pass a C entry
+    return refuse(TJ_ERR_CUDA, "serving", "the device's set-up failed");
+  }
+  if (s.err != cudaSuccess) return refuse(TJ_ERR_CUDA, "serving", cudaGetErrorString(s.err));
+  *out = s.dev;
+  return TJ_OK;
+}
+
+const char* rows_fault(const tj_rows& a, bool write) {
+  if (a.dtype != TJ_F32 && a.dtype != TJ_F16 && a.dtype != TJ_BF16) return "rows must be f32, f16 or bf16";
+  if (a.tokens < 0 || a.q_heads < 0 || a.kv_heads < 0) return "negative extent";
+  if (a.dim <= 0 || a.dim % 8 || a.dim > 512) return "head dim must be a multiple of 8, at most 512";
+  if (a.rot < 0 || a.rot % 2 || a.rot > a.dim) return "rot must be even, from 0 to the head dim";
+  if (a.rot && (!a.positions || !a.table || a.table_rows <= 0)) return "rotary positions need positions and a table";
+  if (a.q && !a.q_out) return "q needs an output";
+  const int unit = 16 / element_size(a.dtype);
+  const auto bad = [&](const void* p, int64_t t, int64_t h) {
+    return p && (reinterpret_cast<uintptr_t>(p) % 16 || t % unit || h % unit);
+  };
+  if (bad(a.q, a.q_token, a.q_head) || bad(a.k, a.k_token, a.k_head) || bad(a.v, a.v_token, a.v_head) ||
+      bad(a.q_out, a.qo_token, a.qo_head) || bad(a.k_out, a.ko_token, a.ko_head) || reinterpret_cast<uintptr_t>(a.table) % 16)
+    return "rows must start on 16-byte boundaries";
+  if (write) {
+    if (!a.k || !a.v || !a.slots) return "a cache write needs k, v and slots";
+    if (a.cache.dim != a.dim || a.cache.heads != a.kv_heads) return "k and v do not have the cache's heads and head dim";
+    return cache_fault(a.cache);
+  }
+  if (!a.q && !a.k) return "nothing to rotate";
+  if (a.v || a.slots) return "a rotation takes neither v nor slots";
+  if (a.k && !a.k_out) return "k needs an output";
+  if (!a.rot) return "rot must be positive";
+  return nullptr;
+}
+
+template <class T> void launch_rows(const RowsParams& p, int mode, unsigned grid, cudaStream_t st) {
+  switch (mode) {
+    case 0: rows_kernel<T, 0><<<grid, 128, 0, st>>>(p); break;
+    case 1: rows_kernel<T, 1><<<grid, 128, 0, st>>>(p); break;
+    case 2: rows_kernel<T, 2><<<grid, 128, 0, st>>>(p); break;
+    default: rows_kernel<T, 3><<<grid, 128, 0, st>>>(p); break;
+  }
+}
+
+int run_rows(const char* name, int op, const tj_rows* a, bool write, void* stream) {
+  if (!a) return refuse(TJ_ERR_INVALID, name, "NULL arguments");
+  if (const char* why = rows_fault(*a, write)) return refuse(TJ_ERR_INVALID, name, why);
+  Device dev;
+  if (const int rc = current_device(&dev)) return rc;
+  const long rows = (a->q ? a->q_heads : 0) + (a->k ? a->kv_heads : 0) + (a->v ? a->kv_heads : 0);
+  if (a->tokens == 0 || rows == 0) return TJ_OK;
+  RowsParams p;
+  p.a = *a;
+  p.status = dev.status;
+  p.op = op;
+  p.slots = static_cast<int>((a->dim + 15) / 16);
+  int mode = 0;
+  if (a->rot) mode = a->interleaved ? (a->rot % 8 ? 3 : 2) : (a->rot % 16 ? 3 : 1);
+  if (mode == 1) p.slots = static_cast<int>(a->rot / 16 + ((a->dim - a->rot) / 8 + 1) / 2);
+  p.lanes_log2 = 0;
+  while ((1 << p.lanes_log2) < p.slots) ++p.lanes_log2;
+  const int per = 32 >> p.lanes_log2;
+  p.iters = static_cast<int>((rows + per - 1) / per);
+  // four iterations a warp (their loads in flight together); with few tokens one each, so that
+  // the rows of a single-token step spread over the multiprocessors
+  const bool few = a->tokens * p.iters < 16L * dev.sms;
+  p.segs = few ? p.iters : (p.iters + 3) / 4;
+  const long warps = a->tokens * p.segs, grid = (warps + 3) / 4;
+  if (grid > 0x7fffffffL) return refuse(TJ_ERR_INVALID, name, "too many rows");
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (a->dtype == TJ_F32)
+    launch_rows<float>(p, mode, static_cast<unsigned>(grid), st);
+  else if (a->dtype == TJ_F16)
+    launch_rows<__half>(p, mode, static_cast<unsigned>(grid), st);
+  else
+    launch_rows<__nv_bfloat16>(p, mode, static_cast<unsigned>(grid), st);
+  return launched(name);
+}
+
+template <class T> void launch_read(const ReadParams& p, dim3 grid, cudaStream_t st) {
+  switch (p.c.dtype) {
+    case TJ_F16: read_kernel<T, TJ_F16><<<grid, 128, 0, st>>>(p); break;
+    case TJ_BF16: read_kernel<T, TJ_BF16><<<grid, 128, 0, st>>>(p); break;
+    case TJ_I8: read_kernel<T, TJ_I8><<<grid, 128, 0, st>>>(p); break;
+    default: read_kernel<T, TJ_E4M3><<<grid, 128, 0, st>>>(p); break;
+  }
+}
+
+}  // namespace tjs
+
+extern "C" int tj_b200_rotary(const tj_rows* args, void* stream) {
+  return tjs::run_rows("tj_b200_rotary", tjs::OP_ROTARY, args, false, stream);
+}
+
+extern "C" int tj_b200_cache_write(const tj_rows* args, void* stream) {
+  return tjs::run_rows("tj_b200_cache_write", tjs::OP_CACHE_WRITE, args, true, stream);
+}
+
+extern "C" int tj_b200_cache_read(const tj_kv_cache* cache, const int32_t* slots, int64_t count, void* k_out, void* v_out,
+                                  int32_t dtype, void* stream) {
+  using namespace tjs;
+  const char* name = "tj_b200_cache_read";
+  if (!cache) return refuse(TJ_ERR_INVALID, name, "NULL cache");
+  if (const char* why = cache_fault(*cache)) return refuse(TJ_ERR_INVALID, name, why);
+  if (dtype != TJ_F32 && dtype != TJ_F16 && dtype != TJ_BF16) return refuse(TJ_ERR_INVALID, name, "rows must be f32, f16 or bf16");
+  if (count < 0) return refuse(TJ_ERR_INVALID, name, "negative extent");
+  if (count == 0) return TJ_OK;
+  if (!slots || !k_out || !v_out) return refuse(TJ_ERR_INVALID, name, "NULL pointer");
+  if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) % 16)
+    return refuse(TJ_ERR_INVALID, name, "rows must start on 16-byte boundaries");
+  Device dev;
+  if (const int rc = current_device(&dev)) return rc;
+  ReadParams p;
+  p.c = *cache;
+  p.slots = slots;
+  p.out[0] = k_out;
+  p.out[1] = v_out;
+  p.rows = count * cache->heads;
+  p.status = dev.status;
+  p.slots_per_row = static_cast<int>((cache->dim + 15) / 16);
+  p.lanes_log2 = 0;
+  while ((1 << p.lanes_log2) < p.slots_per_row) ++p.lanes_log2;
+  const int per = 32 >> p.lanes_log2;
+  p.batch = p.rows < 32L * per * dev.sms ? 1 : 4;
+  const long grid = (p.rows + 4L * per * p.batch - 1) / (4L * per * p.batch);
+  if (grid > 0x7fffffffL) return refuse(TJ_ERR_INVALID, name, "too many rows");
+  const dim3 g(static_cast<unsigned>(grid), 2);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == TJ_F32)
+    launch_read<float>(p, g, st);
+  else if (dtype == TJ_F16)
+    launch_read<__half>(p, g, st);
+  else
+    launch_read<__nv_bfloat16>(p, g, st);
+  return launched(name);
+}
+
+// Waits for `stream`, reads the status words back and clears them.
+extern "C" int tj_b200_serving_status(int32_t* code, int32_t* where, void* stream) {
+  using namespace tjs;
+  const char* name = "tj_b200_serving_status";
+  if (!code || !where) return refuse(TJ_ERR_INVALID, name, "NULL pointer");
+  *code = *where = 0;
+  Device dev;
+  if (const int rc = current_device(&dev)) return rc;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  int words[4] = {0, 0, 0, 0};
+  cudaError_t e = cudaMemcpyAsync(words, dev.status, sizeof(words), cudaMemcpyDeviceToHost, st);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  if (e == cudaSuccess && words[0]) {
+    e = cudaMemsetAsync(dev.status, 0, sizeof(words), st);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(st);
+  }
+  if (e != cudaSuccess) return refuse(TJ_ERR_CUDA, name, cudaGetErrorString(e));
+  *code = words[0];
+  *where = words[1];
+  if (!words[0]) return TJ_OK;
+  return refuse(TJ_ERR_DEVICE_STATUS, name, "a kernel met an index out of range");
+}

@@ -1,0 +1,179 @@
+// Attention of new tokens over a paged cache: what both kernels share.
+//
+//   o[i, h] = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(scale q_i k_j - max),   j visible to i
+//
+// Token i of a sequence's n new tokens stands at position len - n + i; it sees the keys at
+// positions up to its own (causal) and, with a window w, only the last w of those.  The G query
+// heads that share a cached head are packed with the tokens into rows r = i * G + g, so a key or a
+// value is read once for all of them.
+//
+// An 8-bit cache holds k = ks * code, v = vs * code with one scale for each (token, head).  The
+// codes are exact in bf16 and f16, so they enter the matrix products as they are; ks multiplies the
+// score's column, and vs enters the exponent:  t = log2e * scale * ks * (q . code) + log2 vs,
+// P = 2^(t - m) with m the running maximum of t, and the sum adds P / vs.  So P, rounded to 16 bits
+// for the product with the codes, is at most 1 whatever the scales are.
+#pragma once
+#include "serving_common.cuh"
+
+namespace tjs {
+
+struct AttnParams {
+  tj_paged_attention a;
+  int* status;
+  float scale_log2;  // scale * log2 e
+  int group;         // query heads of a cached head
+  int page_shift;    // log2 page_size, or -1
+  int target;        // CTAs that the work is to be cut into, all heads together
+  int min_chunk;     // keys of a chunk at least
+  float* part_o;     // [grid][rows][dim] sums of P V, not yet divided
+  float2* part_ml;   // [grid][rows] (maximum, sum)
+  int* counters;     // [grid] chunks done, zero between calls
+};
+
+// log2 vs is held at this or above: a row of zeros has vs = 0
+constexpr float MIN_LOG2_SCALE = -40.0f;
+
+struct Seq {
+  int start, n, len;  // first new token, new tokens, keys
+};
+TJ_DEV Seq sequence(const AttnParams& p, int b) {
+  Seq s;
+  const int reach = static_cast<int>(min(p.a.table_width * p.a.cache.page_size, static_cast<int64_t>(0x7fffffff)));
+  s.len = max(0, min(p.a.kv_lens[b], reach));
+  if (p.a.q_starts) {
+    const int t = static_cast<int>(p.a.tokens);
+    s.start = min(max(p.a.q_starts[b], 0), t);
+    s.n = min(max(p.a.q_starts[b + 1], s.start), t) - s.start;
+  } else {
+    s.start = b;
+    s.n = 1;
+  }
+  return s;
+}
+
+// keys that some of the tokens [t0, t1] of a sequence see
+TJ_DEV void key_range(const AttnParams& p, const Seq& s, int t0, int t1, int& lo, int& hi) {
+  hi = p.a.causal ? max(0, min(s.len, s.len - s.n + t1 + 1)) : s.len;
+  lo = p.a.window > 0 ? static_cast<int>(max(static_cast<int64_t>(0), s.len - s.n + t0 - p.a.window + 1)) : 0;
+  lo = min(lo, hi);
+}
+// the same of one row's token
+TJ_DEV void row_range(const AttnParams& p, const Seq& s, int t, int& lo, int& hi) { key_range(p, s, t, t, lo, hi); }
+
+// A CTA's piece of the work: row tile `tile` of sequence `b`, chunk `c` of its keys.
+struct Piece {
+  int b, tile, c, chunk;
+  bool some;
+};
+
+// The work is cut on the device, so that neither lengths nor a plan pass through the host: every
+// warp adds up the sequences' (row tiles x keys), divides by the wanted number of CTAs for the
+// chunk, and finds the piece of unit `unit` among the sequences' counts.  `per_tile` rows are a
+// tile; chunks are multiples of `step` keys.
+TJ_DEV Piece find_piece(const AttnParams& p, int unit, int per_tile, int step) {
+  const int lane = threadIdx.x & 31;
+  const int batch = static_cast<int>(p.a.batch), per = (batch + 31) / 32;
+  const int b0 = min(lane * per, batch), b1 = min(b0 + per, batch);
+  const int tokens_per_tile = (per_tile + p.group - 1) / p.group + 1;
+  auto tiles = [&](const Seq& s) { return (s.n * p.group + per_tile - 1) / per_tile; };
+  auto span = [&](const Seq& s) {
+    return p.a.window > 0 ? static_cast<int>(min(static_cast<int64_t>(s.len), p.a.window + tokens_per_tile)) : s.len;
+  };
+  long work = 0;
+  for (int b = b0; b < b1; ++b) {
+    const Seq s = sequence(p, b);
+    work += static_cast<long>(tiles(s)) * span(s);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
+  const long want = (work * p.a.cache.heads + p.target - 1) / p.target;
+  Piece g;
+  g.chunk = static_cast<int>((max(want, static_cast<long>(p.min_chunk)) + step - 1) / step * step);
+  auto count = [&](const Seq& s) { return tiles(s) * max(1, (span(s) + g.chunk - 1) / g.chunk); };
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) mine += count(sequence(p, b));
+  int before = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, before, o);
+    if (lane >= o) before += v;
+  }
+  before -= mine;
+  const bool owner = unit >= before && unit < before + mine;
+  const unsigned who = __ballot_sync(0xffffffffu, owner);
+  g.some = who != 0;
+  if (!g.some) return g;
+  int fb = 0, ft = 0, fc = 0;
+  if (owner) {
+    int left = unit - before;
+    for (int b = b0; b < b1; ++b) {
+      const Seq s = sequence(p, b);
+      const int n = count(s);
+      if (left < n) {
+        const int cuts = max(1, (span(s) + g.chunk - 1) / g.chunk);
+        fb = b;
+        ft = left / cuts;
+        fc = left - ft * cuts;
+        break;
+      }
+      left -= n;
+    }
+  }
+  const int src = __ffs(who) - 1;
+  g.b = __shfl_sync(0xffffffffu, fb, src);
+  g.tile = __shfl_sync(0xffffffffu, ft, src);
+  g.c = __shfl_sync(0xffffffffu, fc, src);
+  return g;
+}
+
+TJ_DEV float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Two codes, each in one byte of a 16-bit half of `w` (the low byte for i8, the high one for e4m3;
+// the other byte is anything), as two exact 16-bit floats.
+template <class T, int CD> struct Codes;
+// i8 -> bf16: 0x4300 | low 7 bits is 128 + them; less 128, or 256 where the sign bit is set
+template <> struct Codes<__nv_bfloat16, TJ_I8> {
+  static TJ_DEV uint32_t make(uint32_t w) {
+    const uint32_t x = (w & 0x007f007fu) | 0x43004300u, y = (w & 0x00800080u) | 0x43004300u;
+    const __nv_bfloat162 d = __hsub2(reinterpret_cast<const __nv_bfloat162&>(x), reinterpret_cast<const __nv_bfloat162&>(y));
+    return reinterpret_cast<const uint32_t&>(d);
+  }
+};
+// i8 -> f16: 0x6400 | (code + 128) is 1024 + that
+template <> struct Codes<__half, TJ_I8> {
+  static TJ_DEV uint32_t make(uint32_t w) {
+    const uint32_t x = (w & 0x00ff00ffu) ^ 0x64806480u, y = 0x64806480u;
+    const __half2 d = __hsub2(reinterpret_cast<const __half2&>(x), reinterpret_cast<const __half2&>(y));
+    return reinterpret_cast<const uint32_t&>(d);
+  }
+};
+// e4m3 -> bf16: the code's exponent and mantissa in place, then 2^(127 - 7) for the bias
+template <> struct Codes<__nv_bfloat16, TJ_E4M3> {
+  static TJ_DEV uint32_t make(uint32_t w) {
+    const uint32_t x = (w & 0x80008000u) | ((w & 0x7f007f00u) >> 4), k = 0x7b807b80u;
+    const __nv_bfloat162 d = __hmul2(reinterpret_cast<const __nv_bfloat162&>(x), reinterpret_cast<const __nv_bfloat162&>(k));
+    return reinterpret_cast<const uint32_t&>(d);
+  }
+};
+template <> struct Codes<__half, TJ_E4M3> {  // 2^(15 - 7)
+  static TJ_DEV uint32_t make(uint32_t w) {
+    const uint32_t x = (w & 0x80008000u) | ((w & 0x7f007f00u) >> 1), k = 0x5c005c00u;
+    const __half2 d = __hmul2(reinterpret_cast<const __half2&>(x), reinterpret_cast<const __half2&>(k));
+    return reinterpret_cast<const uint32_t&>(d);
+  }
+};
+
+// P is made 2^shift times as large before it is rounded to 16 bits, and so is the sum: f16 has no
+// normal numbers below 2^-14, and a key whose probability is small can have the larger value.
+template <class T> constexpr float P_SHIFT = 0.0f;
+template <> constexpr float P_SHIFT<__half> = 14.0f;
+
+template <class T> TJ_DEV uint32_t pack2(float lo, float hi);
+template <> TJ_DEV uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return tj_pack_bf16x2(lo, hi); }
+template <> TJ_DEV uint32_t pack2<__half>(float lo, float hi) { return tj_pack_f16x2(lo, hi); }
+
+}  // namespace tjs

@@ -1,0 +1,69 @@
+// Shared by the serving operators (rotary positions, paged cache, attention over the cache):
+// argument checks, the device status words, and the 8-bit cache formats.
+#pragma once
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include <cstdio>
+#include <mutex>
+
+#include "../../../include/tj_b200.h"
+#include "../kernels/tj_common.cuh"
+
+// defined in tj_b200_runtime.cpp (same library, not exported)
+void tj_b200_internal_set_error(const char* msg);
+
+namespace tjs {
+
+constexpr int MAX_DEVICES = 64;
+
+// Where a status word's `where` points: operator * 16 + site.
+enum : int { SITE_SLOT = 1, SITE_POSITION = 2, SITE_PAGE = 3, SITE_LENGTH = 4 };
+enum : int { OP_ROTARY = 0, OP_CACHE_WRITE = 1, OP_CACHE_READ = 2, OP_ATTENTION = 3 };
+
+// cache_rows.cu: the current device's status words and its multiprocessor count.
+struct Device {
+  int index;
+  int* status;
+  int sms;
+};
+int current_device(Device* out);
+
+inline int refuse(int code, const char* op, const char* why) {
+  char buf[512];
+  snprintf(buf, sizeof(buf), "%s: %s", op, why);
+  tj_b200_internal_set_error(buf);
+  return code;
+}
+inline int launched(const char* op) {
+  const cudaError_t e = cudaGetLastError();
+  return e == cudaSuccess ? TJ_OK : refuse(TJ_ERR_CUDA, op, cudaGetErrorString(e));
+}
+
+inline int element_size(int64_t dtype) {
+  switch (dtype) {
+    case TJ_F32: return 4;
+    case TJ_F16: case TJ_BF16: return 2;
+    case TJ_I8: case TJ_E4M3: return 1;
+  }
+  return 0;
+}
+
+// NULL if the cache's description is sound, else what is wrong with it.
+inline const char* cache_fault(const tj_kv_cache& c) {
+  if (!c.k || !c.v) return "NULL cache pointer";
+  if (c.dtype != TJ_F16 && c.dtype != TJ_BF16 && c.dtype != TJ_I8 && c.dtype != TJ_E4M3) return "bad cache dtype";
+  const bool quantised = c.dtype == TJ_I8 || c.dtype == TJ_E4M3;
+  if (quantised != (c.k_scale != nullptr) || quantised != (c.v_scale != nullptr))
+    return "an i8 or e4m3 cache has scales, a 16-bit one has none";
+  if (c.pages <= 0 || c.page_size <= 0 || c.heads <= 0 || c.dim <= 0) return "cache extents must be positive";
+  if (c.pages * c.page_size > 0x7fffffffLL) return "more than 2^31 - 1 cache slots";
+  if (c.dim % 8 || c.dim > 512) return "head dim must be a multiple of 8, at most 512";
+  const int es = element_size(c.dtype), unit = es == 1 ? 8 : 16;
+  if ((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) % 16 || c.page_stride * es % unit ||
+      c.slot_stride * es % unit || c.head_stride * es % unit)
+    return "cache rows must start on 16-byte (8-bit caches: 8-byte) boundaries";
+  return nullptr;
+}
+
+}  // namespace tjs

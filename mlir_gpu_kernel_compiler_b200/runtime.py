@@ -25,7 +25,8 @@ EXPORTS = (
     "tj_b200_program_info", "tj_b200_destroy", "tj_b200_last_error", "tj_b200_abi_version",
     "tj_b200_driver_available", "tj_b200_time_kernels", "tj_b200_linear_f32_noalloc",
     "tj_b200_linear_f32_noalloc_status", "tj_b200_ipc_export", "tj_b200_ipc_open", "tj_b200_ipc_close",
-    "tj_b200_set_pdl",
+    "tj_b200_set_pdl", "tj_b200_rotary", "tj_b200_cache_write", "tj_b200_cache_read", "tj_b200_paged_attention",
+    "tj_b200_paged_attention_workspace", "tj_b200_serving_status",
 )
 
 
@@ -107,6 +108,13 @@ def library(path: str | Path | None = None) -> ctypes.CDLL:
         lib.tj_b200_ipc_open.restype = ctypes.c_int
         lib.tj_b200_ipc_close.argtypes = [vp, u64, i32]
         lib.tj_b200_ipc_close.restype = ctypes.c_int
+        # the serving operators' structures are 8-byte fields throughout, packed by ``serving``
+        for op in ("rotary", "cache_write", "paged_attention"):
+            getattr(lib, f"tj_b200_{op}").argtypes = [ctypes.c_char_p, vp]
+        lib.tj_b200_cache_read.argtypes = [ctypes.c_char_p, vp, ctypes.c_int64, vp, vp, i32, vp]
+        lib.tj_b200_paged_attention_workspace.argtypes = [ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64),
+                                                          ctypes.POINTER(ctypes.c_int64)]
+        lib.tj_b200_serving_status.argtypes = [ctypes.POINTER(i32), ctypes.POINTER(i32), vp]
         lib.tj_b200_set_pdl.argtypes = [vp, i32]
         lib.tj_b200_set_pdl.restype = ctypes.c_int
         lib.tj_b200_set_graph.argtypes = [vp, i32]

@@ -1,8 +1,8 @@
 """Build steps: the C++ runtime library and the per-kernel sm_100a cubins.
 
-* ``runtime_library()`` — ``libtj_b200.so`` (the C ABI of ``include/tj_b200.h``),
-  built in-tree with g++ from ``csrc/tj_b200_runtime.cpp``.  It links no CUDA
-  library; libcuda is opened at run time.
+* ``build_runtime()`` — ``libtj_b200.so`` (the C ABI of ``include/tj_b200.h``), built in-tree
+  from ``csrc/tj_b200_runtime.cpp`` (libcuda is opened at run time), the allocation-free
+  linear entry point and the serving operators in ``csrc/serving``.
 * ``compile_cubins(sources)`` — nvcc ``-gencode arch=compute_100a,code=sm_100a``
   per kernel translation unit, in parallel, cached on disk by a hash of the
   source, the kernel headers, the flags and the nvcc version (the reference
@@ -27,6 +27,7 @@ PKG = Path(__file__).resolve().parent
 REPO = PKG.parent
 CSRC = PKG / "csrc"
 KDIR = CSRC / "kernels"
+SERVING = CSRC / "serving"
 INCLUDE = REPO / "include"
 LIB_PATH = PKG / "_lib" / "libtj_b200.so"
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
@@ -169,30 +170,56 @@ def compile_cubins(sources: list[tuple[str, str]], extra_flags: tuple = ()) -> l
     return [done[s] for _, s in sources]
 
 
+def _runtime_sources() -> list[tuple[Path, list[Path]]]:
+    """The library's translation units and the headers each is rebuilt for."""
+    hdr = INCLUDE / "tj_b200.h"
+    kernels, serving = sorted(KDIR.glob("*.cuh")), sorted(SERVING.glob("*.cuh"))
+    return [(CSRC / "tj_b200_runtime.cpp", [hdr]), (CSRC / "tj_b200_noalloc.cu", [hdr, *kernels]),
+            *((f, [hdr, *kernels, *serving]) for f in sorted(SERVING.glob("*.cu")))]
+
+
 def build_runtime(force: bool = False, extra_flags: tuple = (), variant: str = "") -> Path:
     """Compile ``libtj_b200.so`` in-tree: the driver-API runtime (host C++; libcuda is opened
-    at run time) plus the allocation-free linear entry point (``tj_b200_noalloc.cu``, sm_100a,
-    static CUDA runtime).  The library loads on machines without a GPU.  ``variant`` names a
-    separately built copy with ``extra_flags`` (``libtj_b200_<variant>.so``; e.g. the
-    failure-path test build); the product library is the one without."""
+    at run time), the allocation-free linear entry point (``tj_b200_noalloc.cu``) and the serving
+    operators (``csrc/serving``), both sm_100a with the static CUDA runtime.  Each source becomes
+    an object file, rebuilt only when it, its headers or the flags change.  The library loads on
+    machines without a GPU.  ``variant`` names a separately built copy with ``extra_flags``
+    (``libtj_b200_<variant>.so``; e.g. the failure-path test build); the product library is the
+    one without."""
     with _lock:
-        src = CSRC / "tj_b200_runtime.cpp"
-        na = CSRC / "tj_b200_noalloc.cu"
-        hdr = INCLUDE / "tj_b200.h"
         out = LIB_PATH if not variant else LIB_PATH.with_name(f"libtj_b200_{variant}.so")
         stamp = out.with_suffix(".hash")
-        h = hashlib.sha256(src.read_bytes() + na.read_bytes() + hdr.read_bytes() + _headers_hash().encode()
-                           + " ".join(extra_flags).encode()).hexdigest()
-        if not force and out.exists() and stamp.exists() and stamp.read_text() == h:
+        flags = ["-O2", "-std=c++17", *ARCH_FLAGS, "-lineinfo", "-Xcompiler", "-fPIC,-fvisibility=hidden,-Wall",
+                 "--expt-relaxed-constexpr", *extra_flags, f"-I{INCLUDE}", f"-I{KDIR}"]
+        units = []
+        for src, headers in _runtime_sources():
+            h = hashlib.sha256(" ".join(flags).encode() + nvcc_version().encode())
+            for f in (src, *headers):
+                h.update(f.read_bytes())
+            units.append((src, out.parent / "obj" / f"{src.stem}.{h.hexdigest()[:24]}.o"))
+        key = "\n".join(o.name for _, o in units)
+        if not force and out.exists() and stamp.exists() and stamp.read_text() == key:
             return out
-        out.parent.mkdir(parents=True, exist_ok=True)
+        obj_dir = out.parent / "obj"
+        obj_dir.mkdir(parents=True, exist_ok=True)
+
+        def compile_unit(unit):
+            src, obj = unit
+            if obj.exists() and not force:
+                return
+            tmp = obj.with_suffix(f".{os.getpid()}.tmp")
+            r = subprocess.run([nvcc(), "-c", *flags, str(src), "-o", str(tmp)], capture_output=True, text=True)
+            if r.returncode != 0:
+                raise BuildError(f"runtime build failed ({src.name}):\n{r.stderr[-4000:]}")
+            os.replace(tmp, obj)
+
+        with ThreadPoolExecutor(max_workers=max(1, min(len(units), os.cpu_count() or 4))) as ex:
+            list(ex.map(compile_unit, units))
         tmp = out.with_suffix(f".{os.getpid()}.tmp")
-        cmd = [nvcc(), "-O2", "-std=c++17", "-shared", *ARCH_FLAGS, "-Xcompiler", "-fPIC,-fvisibility=hidden,-Wall",
-               "--expt-relaxed-constexpr", *extra_flags, f"-I{INCLUDE}", f"-I{KDIR}", str(src), str(na), "-o",
-               str(tmp), "-ldl", "-lpthread"]
+        cmd = [nvcc(), "-shared", *ARCH_FLAGS, *(str(o) for _, o in units), "-o", str(tmp), "-ldl", "-lpthread"]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
-            raise BuildError(f"runtime build failed:\n{r.stderr[-4000:]}")
+            raise BuildError(f"runtime link failed:\n{r.stderr[-4000:]}")
         os.replace(tmp, out)
-        stamp.write_text(h)
+        stamp.write_text(key)
         return out
