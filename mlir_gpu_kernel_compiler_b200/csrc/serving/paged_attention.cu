@@ -1,11 +1,14 @@
 // Host side of the attention over a paged cache: checks, the choice of kernel, the launch.
 #include "paged_attention_rows.cuh"
+#include "paged_attention_tiles.cuh"
 
 namespace tjs {
 
 struct Plan {
+  bool tiles;      // the tensor-core kernel of many rows
   long grid;
-  int rows;    // of a tile
+  long slots;      // partial results kept at once
+  int rows;        // of a tile
   int target;
   int min_chunk;
 };
@@ -25,33 +28,55 @@ const char* attention_fault(const tj_paged_attention& a) {
   return nullptr;
 }
 
-Plan plan_rows(const tj_paged_attention& a, const Device& dev) {
+Plan plan(const tj_paged_attention& a, const Device& dev) {
   Plan p;
   const long group = a.q_heads / a.cache.heads;
   const bool q8 = a.cache.dtype == TJ_I8 || a.cache.dtype == TJ_E4M3;
+  p.tiles = a.max_new * group > 16;
+  if (p.tiles) {
+    p.rows = TILE_ROWS;
+    p.grid = dev.sms;
+    p.slots = 2 * p.grid;  // a CTA's first and last segment
+    p.target = p.min_chunk = 0;
+    return p;
+  }
   p.rows = 16;
   const long tiles = a.q_starts ? a.tokens * group / 16 + a.batch : a.batch * ((group + 15) / 16);
   p.target = dev.sms * (a.cache.dim == 64 ? 4 : 3) * 2;
   p.min_chunk = q8 ? 256 : 128;
   p.grid = a.cache.heads * (tiles + 1) + p.target;
+  p.slots = p.grid;
   return p;
 }
 
-template <class T, int CD> void launch_rows_kernel(const AttnParams& p, unsigned grid, cudaStream_t st) {
-  if (p.a.cache.dim == 64)
-    attention_rows<T, CD, 64><<<grid, 128, 0, st>>>(p);
-  else
-    attention_rows<T, CD, 128><<<grid, 128, 0, st>>>(p);
+template <class T, int CD, int D> cudaError_t launch_dim(const AttnParams& p, const Plan& plan, const Device& dev, cudaStream_t st) {
+  const unsigned grid = static_cast<unsigned>(plan.grid);
+  if (!plan.tiles) {
+    attention_rows<T, CD, D><<<grid, 128, 0, st>>>(p);
+    return cudaSuccess;
+  }
+  static bool ready[MAX_DEVICES];  // the shared-memory limit is raised once a device; doing so twice is harmless
+  constexpr int smem = Tiles<T, CD, D>::SMEM;
+  if (!ready[dev.index]) {
+    const cudaError_t e = cudaFuncSetAttribute(attention_tiles<T, CD, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    ready[dev.index] = true;
+  }
+  attention_tiles<T, CD, D><<<grid, 512, smem, st>>>(p);
+  return cudaSuccess;
 }
-template <class T> void launch_rows_type(const AttnParams& p, unsigned grid, cudaStream_t st) {
+template <class T, int CD> cudaError_t launch_cache(const AttnParams& p, const Plan& plan, const Device& dev, cudaStream_t st) {
+  return p.a.cache.dim == 64 ? launch_dim<T, CD, 64>(p, plan, dev, st) : launch_dim<T, CD, 128>(p, plan, dev, st);
+}
+template <class T> cudaError_t launch_type(const AttnParams& p, const Plan& plan, const Device& dev, cudaStream_t st) {
   switch (p.a.cache.dtype) {
-    case TJ_I8: launch_rows_kernel<T, TJ_I8>(p, grid, st); break;
-    case TJ_E4M3: launch_rows_kernel<T, TJ_E4M3>(p, grid, st); break;
-    default: launch_rows_kernel<T, TJ_BF16>(p, grid, st); break;
+    case TJ_I8: return launch_cache<T, TJ_I8>(p, plan, dev, st);
+    case TJ_E4M3: return launch_cache<T, TJ_E4M3>(p, plan, dev, st);
+    default: return launch_cache<T, TJ_BF16>(p, plan, dev, st);
   }
 }
 
-int64_t part_bytes(const tj_paged_attention& a, const Plan& p) { return p.grid * p.rows * (a.cache.dim * 4 + 8); }
+int64_t part_bytes(const tj_paged_attention& a, const Plan& p) { return p.slots * p.rows * (a.cache.dim * 4 + 8); }
 
 }  // namespace tjs
 
@@ -63,9 +88,9 @@ extern "C" int tj_b200_paged_attention_workspace(const tj_paged_attention* args,
   if (const char* why = attention_fault(*args)) return refuse(TJ_ERR_INVALID, name, why);
   Device dev;
   if (const int rc = current_device(&dev)) return rc;
-  const Plan plan = plan_rows(*args, dev);
-  *workspace_bytes = part_bytes(*args, plan);
-  *counters_count = plan.grid;
+  const Plan need = plan(*args, dev);
+  *workspace_bytes = part_bytes(*args, need);
+  *counters_count = need.grid;
   return TJ_OK;
 }
 
@@ -83,10 +108,10 @@ extern "C" int tj_b200_paged_attention(const tj_paged_attention* args, void* str
     return refuse(TJ_ERR_INVALID, name, "rows must start on 16-byte boundaries");
   Device dev;
   if (const int rc = current_device(&dev)) return rc;
-  const Plan plan = plan_rows(a, dev);
-  if (a.workspace_bytes < part_bytes(a, plan) || a.counters_count < plan.grid)
+  const Plan how = plan(a, dev);
+  if (a.workspace_bytes < part_bytes(a, how) || a.counters_count < how.grid)
     return refuse(TJ_ERR_INVALID, name, "workspace or counters too small");
-  if (plan.grid > 0x7fffffffL) return refuse(TJ_ERR_INVALID, name, "too many rows");
+  if (how.grid > 0x7fffffffL) return refuse(TJ_ERR_INVALID, name, "too many rows");
   AttnParams p;
   p.a = a;
   p.status = dev.status;
@@ -95,15 +120,13 @@ extern "C" int tj_b200_paged_attention(const tj_paged_attention* args, void* str
   p.page_shift = -1;
   for (int i = 0; i < 31; ++i)
     if (a.cache.page_size == (1LL << i)) p.page_shift = i;
-  p.target = plan.target;
-  p.min_chunk = plan.min_chunk;
+  p.target = how.target;
+  p.min_chunk = how.min_chunk;
   p.part_o = static_cast<float*>(a.workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + plan.grid * plan.rows * a.cache.dim);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + how.slots * how.rows * a.cache.dim);
   p.counters = a.counters;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a.dtype == TJ_BF16)
-    launch_rows_type<__nv_bfloat16>(p, static_cast<unsigned>(plan.grid), st);
-  else
-    launch_rows_type<__half>(p, static_cast<unsigned>(plan.grid), st);
+  const cudaError_t e = a.dtype == TJ_BF16 ? launch_type<__nv_bfloat16>(p, how, dev, st) : launch_type<__half>(p, how, dev, st);
+  if (e != cudaSuccess) return refuse(TJ_ERR_CUDA, name, cudaGetErrorString(e));
   return launched(name);
 }
