@@ -108,7 +108,7 @@ def library(path: str | Path | None = None) -> ctypes.CDLL:
         lib.tj_b200_ipc_open.restype = ctypes.c_int
         lib.tj_b200_ipc_close.argtypes = [vp, u64, i32]
         lib.tj_b200_ipc_close.restype = ctypes.c_int
-        # the serving operators' structures are 8-byte fields throughout, packed by ``serving``
+        # the serving operators' structures: 8-byte fields, passed as bytes (``serving`` has a binding of its own)
         for op in ("rotary", "cache_write", "paged_attention"):
             getattr(lib, f"tj_b200_{op}").argtypes = [ctypes.c_char_p, vp]
         lib.tj_b200_cache_read.argtypes = [ctypes.c_char_p, vp, ctypes.c_int64, vp, vp, i32, vp]

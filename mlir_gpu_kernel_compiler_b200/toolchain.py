@@ -223,3 +223,36 @@ def build_runtime(force: bool = False, extra_flags: tuple = (), variant: str = "
         os.replace(tmp, out)
         stamp.write_text(key)
         return out
+
+
+def build_serving_module() -> Path:
+    """Compile ``_serving.so`` in-tree: the Python binding of the serving operators
+    (``csrc/serving/serving_module.cpp``), against the installed torch."""
+    import sys
+
+    import torch
+
+    with _lock:
+        src, hdr = SERVING / "serving_module.cpp", INCLUDE / "tj_b200.h"
+        out = LIB_PATH.with_name("_serving.so")
+        stamp = out.with_suffix(".hash")
+        h = hashlib.sha256(f"{torch.__version__} {torch.__file__} {sys.version} v1".encode() + src.read_bytes() + hdr.read_bytes()).hexdigest()
+        if out.exists() and stamp.exists() and stamp.read_text() == h:
+            return out
+        out.parent.mkdir(parents=True, exist_ok=True)
+        tmp = out.with_suffix(f".{os.getpid()}.tmp")
+        import sysconfig
+
+        from torch.utils import cpp_extension
+
+        includes = [*cpp_extension.include_paths(device_type="cuda"), sysconfig.get_paths()["include"]]
+        cmd = ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", "-fvisibility=hidden",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-isystem{i}" for i in includes),
+               str(src), "-o", str(tmp), *(f"-L{i}" for i in cpp_extension.library_paths(device_type="cuda")),
+               "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python", "-ldl"]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:
+            raise BuildError(f"serving module build failed:\n{r.stderr[-4000:]}")
+        os.replace(tmp, out)
+        stamp.write_text(h)
+        return out

@@ -1,5 +1,6 @@
 """The serving operators without a GPU: the layout of the C structures, and what is refused before a launch."""
 import ctypes
+import struct
 import subprocess
 from pathlib import Path
 
@@ -10,6 +11,10 @@ from mlir_gpu_kernel_compiler_b200 import runtime as rt
 from mlir_gpu_kernel_compiler_b200 import serving
 
 HEADER = Path(__file__).resolve().parents[1] / "include" / "tj_b200.h"
+# the C structures are 8-byte fields throughout
+CACHE = struct.Struct("=15q")       # tj_kv_cache
+ROWS = struct.Struct("=27q")        # tj_rows, without its cache
+ATTENTION = struct.Struct("=21qd2q")  # tj_paged_attention, without its cache
 
 
 def test_packed_structures_match_the_header(tmp_path):
@@ -21,16 +26,16 @@ def test_packed_structures_match_the_header(tmp_path):
     exe = tmp_path / "sz"
     subprocess.run(["gcc", str(src), "-o", str(exe)], check=True)
     vals = [int(x) for x in subprocess.run([str(exe)], capture_output=True, text=True, check=True).stdout.split()]
-    c, r, a = serving._CACHE.size, serving._TJ_ROWS.size, serving._ATTENTION.size
+    c, r, a = CACHE.size, ROWS.size, ATTENTION.size
     assert vals == [c, r, r + c, 24 * 8, a, 21 * 8, a + c]
 
 
 def _cache(dtype=4, k=4096, v=8192, ks=4096, vs=4096, pages=4, page=16, heads=2, dim=64, strides=(2048, 128, 64), scale=(32, 2, 1)):
-    return serving._CACHE.pack(k, v, ks, vs, pages, page, heads, dim, *strides, *scale, dtype)
+    return CACHE.pack(k, v, ks, vs, pages, page, heads, dim, *strides, *scale, dtype)
 
 
 def _rows(q=0, k=4096, v=4096, q2=0, k2=0, slots=4096, pos=0, table=0, tokens=3, hq=0, hk=2, dim=64, rot=0, rows=0, stride=128, dtype=2):
-    return serving._TJ_ROWS.pack(q, k, v, q2, k2, slots, pos, table, tokens, hq, hk, dim, rot, rows, *[stride, 64] * 5, dtype, 0, 0)
+    return ROWS.pack(q, k, v, q2, k2, slots, pos, table, tokens, hq, hk, dim, rot, rows, *[stride, 64] * 5, dtype, 0, 0)
 
 
 BAD_CACHES = [(dict(k=0), b"NULL"), (dict(dtype=9), b"dtype"), (dict(ks=0), b"scales"), (dict(dtype=2), b"scales"), (dict(pages=0), b"positive"),
@@ -50,7 +55,7 @@ def test_c_entries_refuse_bad_caches(how, why):
 
 def test_c_entries_refuse_bad_rows():
     lib = rt.library()
-    none = bytes(serving._CACHE.size)
+    none = bytes(CACHE.size)
     for args, why in [(_rows(dtype=3) + _cache(), b"f32, f16 or bf16"), (_rows(dim=72) + _cache(), b"cache's heads"),
                       (_rows(hk=3) + _cache(), b"cache's heads"), (_rows(slots=0) + _cache(), b"slots"), (_rows(k=4100) + _cache(), b"boundaries"),
                       (_rows(stride=130) + _cache(), b"boundaries"), (_rows(rot=3) + _cache(), b"even"), (_rows(rot=66) + _cache(), b"even"),
@@ -73,7 +78,7 @@ def test_c_entry_refuses_bad_attention():
     lib = rt.library()
 
     def args(q=4096, out=4096, starts=4096, tokens=5, batch=2, heads=4, max_new=3, width=4, dtype=2, window=0, scale=0.125, stride=256, ws=4096, cache=None):
-        return serving._ATTENTION.pack(q, out, 0, 4096, 4096, starts, ws, 4096, tokens, batch, heads, max_new, width, width, stride, 64, stride, 64,
+        return ATTENTION.pack(q, out, 0, 4096, 4096, starts, ws, 4096, tokens, batch, heads, max_new, width, width, stride, 64, stride, 64,
                                        dtype, 1, window, scale, 1 << 40, 1 << 30) + (cache or _cache())
 
     for how, why in [(dict(dtype=0), b"f16 or bf16"), (dict(cache=_cache(dtype=1, ks=0, vs=0)), b"q's type"),
