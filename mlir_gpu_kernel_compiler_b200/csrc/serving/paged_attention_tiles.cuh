@@ -2,26 +2,35 @@
 // products run on the tensor cores through tcgen05 with their sums in TMEM.
 //
 // What bounds it: a key meets 256 rows, 2 x 256 products for each of its elements, so the cache is
-// cheap and the kernel is made of the tensor cores' two products a block (128 keys: 2 x 512 clocks a
-// row tile at head dim 128) and of 128 exponentials a row and block (16 a clock and SM: 1024 clocks a
-// row tile).  Both are about the same, and each row tile needs them in turn; two row tiles in
-// antiphase keep both units busy.  Warps (512 threads, one CTA an SM):
-//   0-3, 4-7   softmax of row tile 0, 1: a thread is a row.  It reads its 128 scores out of TMEM,
-//              keeps a running maximum (moved, and the sums in TMEM rescaled, only when a block
-//              exceeds it by more than 2^RAISE) and sum, and writes P over the scores, 16 bits each.
-//   8-11       producers: warp w brings keys 32 w .. 32 w + 31 of each block: pages are looked up one
-//              key a lane, rows copied asynchronously (16-bit caches) or converted to 16 bits on the
-//              way (8-bit ones), in the 128-byte-swizzled layout that the matrix unit reads.  Pages may
-//              have any size and the cache any strides, as no copy spans two rows.
-//   12         issues the matrix instructions: per block, tile 0's P V then its next scores, then tile
-//              1's; a tile's next scores overwrite its P, and follow the product that reads it.
+// cheap and the kernel is made of the tensor cores' two products and of 64 exponentials a row and block
+// of 64 keys (16 a clock and SM: 512 clocks a row tile).  A row tile's scores of the next block are made
+// while its softmax works on this one, in a second buffer; so softmax and tensor cores never wait for
+// one another's round trip (with 128 keys a block there is TMEM for one buffer only: 4000 clocks for 128
+// keys of both tiles, half of them waiting).  The price is a narrower product for the scores, 49 clocks
+// a step of 16 where the tensor cores need 32, as shared memory has to give 6 KB for it: 2590 clocks
+// for 128 keys at head dim 128.  Warps (512 threads, one CTA an SM):
+//   0-3, 4-7   softmax of row tile 0, 1: a thread is a row.  It reads its 64 scores out of TMEM, keeps a
+//              running maximum (moved, and the sums in TMEM rescaled, only when a block exceeds it by
+//              more than 2^RAISE) and sum, and writes P over the scores, 16 bits each.
+//   8-11       producers of the keys (8, 9) and values (10, 11): a warp brings 32 rows of each block.
+//              Pages are looked up one key a lane, rows copied asynchronously (16-bit caches) or
+//              converted to 16 bits on the way (8-bit ones), in the 128-byte-swizzled layout that the
+//              matrix unit reads.  Pages may have any size and the cache any strides, as no copy spans
+//              two rows.
+//   12, 13     issue the matrix instructions of row tile 0, 1: per block P V, then the scores of the
+//              block after the next over the P that it has read.  (One warp for both was the bound, 2400
+//              clocks a block: a wait for a barrier takes 140 clocks even when it is over, as it queues
+//              behind the softmax warps' exponentials.)
+//   14         looks the next segment up.
 //
 // The work, (tile, block) pairs of all sequences and heads in a row, is cut into as many equal parts as
-// there are SMs (each at least 4 blocks): a CTA takes a tile's end, whole tiles and a tile's beginning.
+// there are SMs (each at least 512 keys): a CTA takes a tile's end, whole tiles and a tile's beginning.
 // Parts of one tile are joined by the CTA whose part comes last, in the tile's order.
 //
 // Every wait is bounded (TJ_WAIT_NS): one that runs out raises the CTA's abort flag and the status word.
 #pragma once
+#include <limits.h>
+
 #include <type_traits>
 
 #include "../kernels/attention_sm100.cuh"
@@ -29,10 +38,11 @@
 
 namespace tjs {
 
-constexpr int TILE_ROWS = 256, TILE_KEYS = 128;
+constexpr int TILE_ROWS = 256, TILE_KEYS = 64;
 
 // The linear order of the work, in keys x group.  A tile weighs its keys, and one block more for what a
-// tile costs by itself.
+// tile costs by itself.  Positions are cut without 64-bit divisions, which a lone warp takes
+// hundreds of clocks for.
 struct TileWork {
   long per_head;  // of a sequence: all its tiles
   long base;      // a tile's weight without what grows along the sequence
@@ -40,8 +50,7 @@ struct TileWork {
   int rows;
   bool grows;     // causal without a window: tile t sees 256 (t + 1) / group tokens more
   TJ_DEV long before(int t) const {  // weight of the tiles before t
-    if (!grows) return base * t;
-    return t < tiles ? base * t + static_cast<long>(TILE_ROWS / 2) * t * (t + 1) : per_head;
+    return base * t + (grows ? static_cast<long>(TILE_ROWS / 2) * t * (t + 1) : 0);
   }
 };
 TJ_DEV TileWork tile_work(const AttnParams& p, const Seq& s) {
@@ -55,8 +64,7 @@ TJ_DEV TileWork tile_work(const AttnParams& p, const Seq& s) {
   else if (p.a.window > 0)
     span = min(span, static_cast<long>(p.a.window) + TILE_ROWS / p.group);
   w.base = p.group * (span + TILE_KEYS);
-  w.per_head = w.base * w.tiles;
-  if (w.grows && w.tiles) w.per_head += static_cast<long>(TILE_ROWS / 2) * (w.tiles - 1) * w.tiles + w.rows;
+  w.per_head = w.before(w.tiles);
   return w;
 }
 
@@ -77,6 +85,22 @@ TJ_DEV long total_work(const AttnParams& p) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   return mine * p.a.cache.heads;
+}
+
+// The work in `parts` equal parts: part c begins at begin(c).
+struct Cut {
+  long total, parts, share, rest;
+  TJ_DEV Cut(long t, long n) : total(t), parts(n), share(t / n), rest(t - share * n) {}
+  TJ_DEV long begin(long c) const { return share * c + min(c, rest); }
+  TJ_DEV long part_of(long pos) const {
+    const long wide = (share + 1) * rest;
+    return pos < wide ? pos / (share + 1) : rest + (pos - wide) / share;
+  }
+};
+// How many of a tile's `blocks` key blocks lie before place `a` of its weight: roundings to nearest
+// keep the order, so neighbours that ask with the same place agree, and a = weight gives all.
+TJ_DEV int blocks_before(long a, long weight, int blocks) {
+  return static_cast<int>(static_cast<float>(blocks) * __fdiv_rn(static_cast<float>(a), static_cast<float>(weight)));
 }
 
 // the tile at `pos` of the linear order (0 <= pos < total), found by a warp
@@ -106,7 +130,9 @@ TJ_DEV TilePart find_tile(const AttnParams& p, long pos) {
   g.s = sequence(p, g.b);
   const TileWork w = tile_work(p, g.s);
   const long in_seq = pos - g.start;
-  g.head = static_cast<int>(in_seq / w.per_head);
+  g.head = static_cast<int>(static_cast<float>(in_seq) / static_cast<float>(w.per_head));  // off by one at the most
+  while (g.head > 0 && in_seq < g.head * w.per_head) --g.head;
+  while (in_seq >= (g.head + 1) * w.per_head) ++g.head;
   const long in_head = in_seq - g.head * w.per_head;
   int lo = 0, hi = w.tiles - 1;
   while (lo < hi) {
@@ -119,7 +145,6 @@ TJ_DEV TilePart find_tile(const AttnParams& p, long pos) {
   g.tile = lo;
   g.start += g.head * w.per_head + w.before(lo);
   g.weight = w.before(lo + 1) - w.before(lo);
-  if (lo + 1 == w.tiles) g.weight = w.per_head - w.before(lo);
   return g;
 }
 
@@ -129,6 +154,16 @@ TJ_DEV void cp_async16(uint32_t dst, const void* src, bool on) {
 }
 TJ_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> TJ_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+// 16 columns of a warp's 32 lanes out of TMEM
+TJ_DEV void tmem_ld16(uint32_t addr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+        "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr)
+      : "memory");
+}
 template <int N> TJ_DEV void regs_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N> TJ_DEV void regs_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 TJ_DEV void st_shared16(uint32_t dst, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
@@ -141,538 +176,721 @@ TJ_DEV uint32_t swizzled(int rows, int row, int piece) {
   return static_cast<uint32_t>((piece >> 3) * rows * 128 + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
 }
 
+// A producer warp's rows of 8-bit codes as 16-bit floats into a swizzled operand.
+template <class T, int CD, int D, int N>
+TJ_DEV void store_rows(uint32_t dst, const uint4 (&raw)[N], int row0) {
+  constexpr int LPR = D / 16, PER = 32 / LPR;
+  const int lane = threadIdx.x & 31, piece = lane % LPR;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int r = row0 + i * PER + lane / LPR;
+    uint32_t h[2][4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const uint32_t x = e == 0 ? raw[i].x : e == 1 ? raw[i].y : e == 2 ? raw[i].z : raw[i].w;
+      h[e >> 1][(e & 1) * 2] = Codes<T, CD>::make(__byte_perm(x, 0, CD == TJ_I8 ? 0x4140 : 0x1404));
+      h[e >> 1][(e & 1) * 2 + 1] = Codes<T, CD>::make(__byte_perm(x, 0, CD == TJ_I8 ? 0x4342 : 0x3424));
+    }
+    // at head dim 128 a row's lanes reach both panels, whose banks are the same: the upper half
+    // stores its odd piece first
+    const bool swap = D == 128 && piece >= LPR / 2;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int o = swap ? e ^ 1 : e;
+      st_shared16(dst + swizzled(TILE_KEYS, r, piece * 2 + o), swap ? h[e ^ 1][0] : h[e][0], swap ? h[e ^ 1][1] : h[e][1],
+                  swap ? h[e ^ 1][2] : h[e][2], swap ? h[e ^ 1][3] : h[e][3]);
+    }
+  }
+}
+
+// 2^x of a pair on the FMA pipes: x = j + f, j its nearest integer (added to the exponent), |f| <= 1/2 and
+// 2^f by a polynomial of degree 4 fitted here (least squares reweighted towards the largest relative error,
+// which is 2.6e-6; its mean is 4e-8).  The units for exponentials make 16 a clock and SM and are as
+// busy as the tensor cores, so some of the pairs take this way.  x <= 127; below -126 it is 2^-126.
+TJ_DEV void exp2_pair(uint64_t x, float& e0, float& e1) {
+  using namespace tja;
+  float x0, x1;
+  f2_unpack(x, x0, x1);
+  x = f2_pack(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
+  const uint64_t magic = f2_pack(12582912.0f, 12582912.0f), unmagic = f2_pack(-12582912.0f, -12582912.0f);  // 1.5 * 2^23
+  const uint64_t t = f2_add(x, magic);
+  const uint64_t f = f2_fma(f2_add(t, unmagic), f2_pack(-1.0f, -1.0f), x);
+  auto c = [](float v) { return f2_pack(v, v); };
+  uint64_t y = f2_fma(c(0.009570102207362652f), f, c(0.05591786280274391f));
+  y = f2_fma(y, f, c(0.240247443318367f));
+  y = f2_fma(y, f, c(0.6931217908859253f));
+  y = f2_fma(y, f, c(0.9999992847442627f));
+  float t0, t1, y0, y1;
+  f2_unpack(t, t0, t1);
+  f2_unpack(y, y0, y1);
+  e0 = __int_as_float(__float_as_int(y0) + (__float_as_int(t0) << 23));
+  e1 = __int_as_float(__float_as_int(y1) + (__float_as_int(t1) << 23));
+}
+
 template <class T, int CD, int D> struct Tiles {
   static constexpr bool Q8 = CD == TJ_I8 || CD == TJ_E4M3;
-  static constexpr int STAGES = D == 128 ? 2 : 4;
-  static constexpr int SCALES = STAGES + 2;  // scale rows outlive their block's operands
+  static constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
+  // An 8-bit cache's value scales: bf16 has f32's range, so P is simply multiplied by vs before it is
+  // rounded (arrays ks, vs); f16 has vs in the exponent (arrays ks, log2 vs, 1 / vs).  Every softmax
+  // thread reads these arrays for every block, so one fewer counts.
+  static constexpr bool MUL_V = Q8 && BF, EXP_V = Q8 && !BF;
+  static constexpr int ARRAYS = MUL_V ? 2 : EXP_V ? 3 : 0;
+  static constexpr int STAGES = D == 128 ? 4 : 8;
+  // Scale rows outlive their block's operands: a tile's softmax is up to two blocks behind its scores.
+  // Block j + SCALES takes over from block j when the scores of block j + 2 are made, which follow its P.
+  static constexpr int SCALES = STAGES + 2;
   static constexpr uint32_t Q_BYTES = 128 * D * 2, KV_BYTES = TILE_KEYS * D * 2;
-  static constexpr int SMEM = 1024 + 2 * Q_BYTES + 2 * STAGES * KV_BYTES + (Q8 ? SCALES * 3 * TILE_KEYS * 4 : 0) + 512;
-  // TMEM columns: S_0, S_1 (128 each; P, 64 columns, over them), O_0, O_1 (D each)
+  static constexpr int SMEM = 1024 + 2 * Q_BYTES + 2 * STAGES * KV_BYTES + SCALES * ARRAYS * TILE_KEYS * 4 + 768;
+  // registers of a softmax, producer and other thread; at launch all have 128
+  static constexpr int REGS_S = 152, REGS_P = 104, REGS_M = 104;
+  static_assert(256 * REGS_S + 128 * REGS_P + 128 * REGS_M <= 512 * 128, "no more than the block was launched with");
+  // TMEM columns: scores of tile t, buffer b at (2 t + b) 64 (P, 32 columns, over them); O_t at 256 + t D
   static constexpr uint32_t TMEM = 512;
+#ifndef TJS_EMU
+#define TJS_EMU 0
+#endif
+  // exponentials of every 16 pairs that go to the FMA pipes: see exp2_pair
+  static constexpr int EMU = TJS_EMU;
   static constexpr float SHIFT = P_SHIFT<T> > 11.0f ? 11.0f : P_SHIFT<T>;  // with RAISE: P < 2^16
   static constexpr float RAISE = P_SHIFT<T> > 0.0f ? 4.0f : 8.0f;
 };
 
-// A CTA's shared memory and its piece of the work.
+// A row's P = 2^(x c + b) (8-bit caches: x + b) of a block: summed into ll, rounded to 16 bits and
+// written over the scores at tS.
+template <class T, class C, int EMU>
+TJ_DEV void probabilities(const float (&x)[64], uint64_t c, uint64_t b, const float* sc, uint64_t& ll, uint32_t tS) {
+  using namespace tja;
+#pragma unroll
+  for (int g = 0; g < 2; ++g) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const int i = g * 32 + 2 * k;
+      const uint64_t xx = f2_pack(x[i], x[i + 1]);
+      const uint64_t e = C::Q8 ? f2_add(xx, b) : f2_fma(xx, c, b);
+      float e0, e1;
+      if (k * EMU % 16 < EMU) {
+        exp2_pair(e, e0, e1);
+      } else {
+        f2_unpack(e, e0, e1);
+        e0 = exp2_fast(e0);
+        e1 = exp2_fast(e1);
+      }
+      if constexpr (C::EXP_V) {
+        const float2 inv = *reinterpret_cast<const float2*>(sc + 2 * TILE_KEYS + i);
+        ll = f2_fma(f2_pack(e0, e1), f2_pack(inv.x, inv.y), ll);
+      } else {
+        ll = f2_add(ll, f2_pack(e0, e1));
+      }
+      if constexpr (C::MUL_V) {
+        const float2 vs = *reinterpret_cast<const float2*>(sc + TILE_KEYS + i);
+        e0 *= vs.x;
+        e1 *= vs.y;
+      }
+      pk[k] = pack2<T>(e0, e1);
+    }
+    tmem_st16(tS + 16 * g, pk);
+  }
+}
+
+// What a CTA does between two of its barriers: blocks of one tile.
+struct Segment {
+  Seq s;
+  int b, head;
+  int r0, rows;     // first packed row of the tile, rows of it
+  int lo, hi;       // keys that some row sees
+  int key0, nb;     // first key and number of blocks of this segment (0: no segment)
+  int all;          // blocks of the tile
+  int later;        // the tile began in an earlier part
+  long start, weight;
+};
+
+// A CTA's shared memory.
 template <class T, int CD, int D> struct TilesShared {
   using C = Tiles<T, CD, D>;
-  static constexpr int STAGES = C::STAGES;
-  uint8_t *sQ, *sK, *sV;
-  float* scales;  // [SCALES][3][128]: ks, log2 vs, 1 / vs
-  uint64_t *q_full, *k_full, *v_full, *k_empty, *v_empty, *s_full, *p_ready, *o_done, *drain;
-  uint32_t* tmem_slot;
-  volatile int* abort_flag;
-  int* s_last;
-  long total, parts, from, to;
-  TJ_DEV TilesShared(uint8_t* raw) {
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-    sQ = smem;
-    sK = sQ + 2 * C::Q_BYTES;
-    sV = sK + STAGES * C::KV_BYTES;
-    scales = reinterpret_cast<float*>(sV + STAGES * C::KV_BYTES);
-    q_full = reinterpret_cast<uint64_t*>(scales + (C::Q8 ? C::SCALES * 3 * TILE_KEYS : 0));
-    k_full = q_full + 1;
-    v_full = k_full + STAGES;
-    k_empty = v_full + STAGES;
-    v_empty = k_empty + STAGES;
-    s_full = v_empty + STAGES;  // [2]
-    p_ready = s_full + 2;       // [2]
-    o_done = p_ready + 2;
-    drain = o_done + 1;
-    tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
-    abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    s_last = reinterpret_cast<int*>(tmem_slot + 2);
+  static constexpr uint32_t Q = 0, K = Q + 2 * C::Q_BYTES, V = K + C::STAGES * C::KV_BYTES, SCALE = V + C::STAGES * C::KV_BYTES,
+                            BARS = SCALE + C::SCALES * C::ARRAYS * TILE_KEYS * 4, Q_FULL = BARS, K_FULL = Q_FULL + 8,
+                            V_FULL = K_FULL + 8 * C::STAGES, K_EMPTY = V_FULL + 8 * C::STAGES, V_EMPTY = K_EMPTY + 8 * C::STAGES,
+                            S_FULL = V_EMPTY + 8 * C::STAGES,  // [2 tiles][2 buffers]
+                            P_READY = S_FULL + 32,             // [2 tiles][2 buffers]
+                            PV_DONE = P_READY + 32,            // [2 tiles][2 buffers]
+                            SC_FULL = PV_DONE + 32,            // [SCALES], 8-bit caches
+                            DRAIN = SC_FULL + 8 * C::SCALES, SLOT = DRAIN + 16, ABORT = SLOT + 4, LAST = ABORT + 4,
+                            SEGMENT = (LAST + 4 + 15) / 16 * 16, END = SEGMENT + 2 * sizeof(Segment);
+  static_assert(END + 1024 <= C::SMEM, "shared memory");
+  uint8_t* base;
+  TJ_DEV explicit TilesShared(uint8_t* raw) {
+    base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+  }
+  TJ_DEV uint32_t at(uint32_t offset) const { return tjg::smem_u32(base) + offset; }
+  TJ_DEV float* scales(int it) const {  // [ARRAYS][128]: ks, vs or log2 vs, 1 / vs
+    return reinterpret_cast<float*>(base + SCALE) + (it % C::SCALES) * C::ARRAYS * TILE_KEYS;
+  }
+  TJ_DEV volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(base + ABORT); }
+  TJ_DEV volatile int* last() const { return reinterpret_cast<volatile int*>(base + LAST); }
+  TJ_DEV volatile uint32_t* tmem_slot() const { return reinterpret_cast<volatile uint32_t*>(base + SLOT); }
+  // volatile: read where it is needed, not kept in registers over the blocks
+  TJ_DEV volatile Segment& segment(int seg) const { return reinterpret_cast<volatile Segment*>(base + SEGMENT)[seg & 1]; }
+  TJ_DEV int* slots() const { return reinterpret_cast<int*>(base + K); }  // while the parts of a tile are joined
+  // Several barriers at once: the polls, each some 140 clocks behind the softmax warps' exponentials, overlap.
+  TJ_DEV bool wait3(uint32_t b0, int ph0, uint32_t b1, int ph1, uint32_t b2, int ph2, const AttnParams& p, int site) const {
+    const bool x = tjg::mbar_try_wait(at(b0), ph0 & 1), y = tjg::mbar_try_wait(at(b1), ph1 & 1), z = tjg::mbar_try_wait(at(b2), ph2 & 1);
+    if (__all_sync(0xffffffffu, x & y & z)) return true;
+    return wait(b0, ph0, p, site) && wait(b1, ph1, p, site + 1) && wait(b2, ph2, p, site + 2);
+  }
+  TJ_DEV bool wait(uint32_t bar, int phase, const AttnParams& p, int site) const {
+    return tjg::mbar_wait_warp(at(bar), static_cast<uint32_t>(phase) & 1u, abort_flag(), p.status, OP_ATTENTION * 16 + site);
   }
 };
 
-enum class Role { softmax, producer, matrix };
-
-// The segments of a CTA as one of its roles goes through them.
-template <Role ROLE, class T, int CD, int D>
-TJ_DEV void tiles_role(const AttnParams& p, const TilesShared<T, CD, D>& sh, uint32_t tmem) {
-  using namespace tjg;
-  using C = Tiles<T, CD, D>;
-  constexpr bool Q8 = C::Q8;
-  constexpr int STAGES = C::STAGES, ES = Q8 ? 1 : 2;
-  constexpr uint32_t Q_BYTES = C::Q_BYTES, KV_BYTES = C::KV_BYTES;
-  constexpr bool BF = std::is_same<T, __nv_bfloat16>::value;
-  constexpr uint32_t IDESC_S = idesc_f16(BF, 128, TILE_KEYS, false, false), IDESC_O = idesc_f16(BF, 128, D, false, true);
-  constexpr int WHERE = OP_ATTENTION * 16;
-  uint8_t *const sQ = sh.sQ, *const sK = sh.sK, *const sV = sh.sV;
-  float* const scales = sh.scales;
-  uint64_t *const q_full = sh.q_full, *const k_full = sh.k_full, *const v_full = sh.v_full, *const k_empty = sh.k_empty,
-                  *const v_empty = sh.v_empty, *const s_full = sh.s_full, *const p_ready = sh.p_ready, *const o_done = sh.o_done,
-                  *const drain = sh.drain;
-  volatile int* const abort_flag = sh.abort_flag;
-  int* const s_last = sh.s_last;
-  const long total = sh.total, parts = sh.parts, from = sh.from, to = sh.to;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // segments, and key blocks of row tile 0 and 1, before this segment: barrier phases run on
-  int seg = 0, blocks = 0, blocks1 = 0;
-  bool failed = false;
-  for (long pos = from; pos < to && !failed;) {
+// The next segment at or after `pos` (moved on), by a whole warp.
+TJ_DEV void next_segment(const AttnParams& p, long& pos, long to, volatile Segment& out) {
+  Segment g;
+  g.nb = 0;
+  while (pos < to && g.nb == 0) {
     const TilePart w = find_tile(p, pos);
     const long a0 = pos - w.start, a1 = min(w.weight, to - w.start);
     pos = w.start + a1;
-    const int r0 = w.tile * TILE_ROWS, rows = min(TILE_ROWS, w.s.n * p.group - r0);
-    int lo, hi;
-    key_range(p, w.s, r0 / p.group, (r0 + rows - 1) / p.group, lo, hi);
-    const int first = lo / TILE_KEYS, all = max(1, (hi + TILE_KEYS - 1) / TILE_KEYS - first);
-    const int j0 = static_cast<int>(a0 * all / w.weight), nb = static_cast<int>(a1 * all / w.weight) - j0;
-    if (nb == 0) continue;
-    const bool whole = nb == all;
-    const int key0 = (first + j0) * TILE_KEYS;
-    const int ntiles = rows > 128 ? 2 : 1;
+    g.s = w.s;
+    g.b = w.b;
+    g.head = w.head;
+    g.r0 = w.tile * TILE_ROWS;
+    g.rows = min(TILE_ROWS, w.s.n * p.group - g.r0);
+    key_range(p, w.s, g.r0 / p.group, (g.r0 + g.rows - 1) / p.group, g.lo, g.hi);
+    const int first = g.lo / TILE_KEYS;
+    g.all = max(1, (g.hi + TILE_KEYS - 1) / TILE_KEYS - first);
+    const int j0 = blocks_before(a0, w.weight, g.all);
+    g.nb = blocks_before(a1, w.weight, g.all) - j0;
+    g.key0 = (first + j0) * TILE_KEYS;
+    g.later = a0 > 0;
+    g.start = w.start;
+    g.weight = w.weight;
+  }
+  if ((threadIdx.x & 31) == 0) {
+    if (g.nb) {
+      out.s.start = g.s.start;
+      out.s.n = g.s.n;
+      out.s.len = g.s.len;
+      out.b = g.b;
+      out.head = g.head;
+      out.r0 = g.r0;
+      out.rows = g.rows;
+      out.lo = g.lo;
+      out.hi = g.hi;
+      out.key0 = g.key0;
+      out.all = g.all;
+      out.later = g.later;
+      out.start = g.start;
+      out.weight = g.weight;
+    }
+    out.nb = g.nb;
+  }
+  __syncwarp();
+}
 
-    if constexpr (ROLE == Role::producer) {
-      // ---------------- producers ----------------
-      const int pw = warp - 8, tid = threadIdx.x - 256;
-      bool ok = true;
-      // queries: the packed rows' heads
-      {
-        constexpr int LPR = D / 8;  // 16-byte pieces of a row
-        const int piece = tid % LPR;
-        for (int r = tid / LPR; r < ntiles * 128; r += 128 / LPR) {
-          const bool on = r < rows;
-          const int rr = r0 + (on ? r : 0), tok = rr / p.group, hd = w.head * p.group + rr - tok * p.group;
-          const T* src = static_cast<const T*>(p.a.q) + (w.s.start + tok) * p.a.q_token + hd * p.a.q_head + piece * 8;
-          cp_async16(smem_u32(sQ) + (r >> 7) * Q_BYTES + swizzled(128, r & 127, piece), src, on);
-        }
-        cp_async_commit();
+// (token, query head) of packed row r of a sequence
+TJ_DEV void row_of(const AttnParams& p, int head, int r, int& tok, int& hd) {
+  tok = r / p.group;
+  hd = head * p.group + r - tok * p.group;
+}
+
+// The end of a segment, by every thread of the CTA: false if a wait ran out.  A tile in several parts is
+// joined, in the order of its parts, by the CTA that makes its blocks complete.
+template <class T, int CD, int D>
+TJ_DEV bool end_segment(const AttnParams& p, const TilesShared<T, CD, D>& sh, const Cut& cut, int seg) {
+  using C = Tiles<T, CD, D>;
+  volatile Segment& g = sh.segment(seg);
+  __syncwarp();
+  const int nb = g.nb, all = g.all;
+  const bool whole = nb == all;
+  if (!whole) __threadfence();
+  __syncthreads();
+  tjg::tc_fence_after();
+  if (*sh.abort_flag()) return false;
+  if (whole) return true;
+  const long start = g.start, weight = g.weight;
+  const int c0 = static_cast<int>(cut.part_of(start)), n = static_cast<int>(cut.part_of(start + weight - 1)) - c0 + 1;
+  if (threadIdx.x == 0) {
+    const int done = atomicAdd(p.counters + c0, nb) + nb;
+    *sh.last() = done == all;
+    if (done == all) p.counters[c0] = 0;  // ready for the next call
+  }
+  // where each part of the tile was left (-1: it had no block); as many as CTAs at the most
+  if (threadIdx.x < n) {
+    const int c = c0 + threadIdx.x;
+    const long b0 = max(0L, cut.begin(c) - start), b1 = min(weight, cut.begin(c + 1) - start);
+    sh.slots()[threadIdx.x] = blocks_before(b0, weight, all) == blocks_before(b1, weight, all) ? -1 : 2 * c + (b0 > 0 ? 0 : 1);
+  }
+  __syncthreads();
+  if (*sh.last()) {
+    __threadfence();
+    const int r0 = g.r0, rows = g.rows, head = g.head, first_token = g.s.start;
+    constexpr int V4 = D / 4;
+    for (int e = threadIdx.x; e < rows * V4; e += 512) {
+      const int r = e / V4, col = (e - r * V4) * 4;
+      float best = -INFINITY, sum = 0.0f;
+      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+      for (int c = 0; c < n; ++c) {
+        if (sh.slots()[c] < 0) continue;
+        const long slot = static_cast<long>(sh.slots()[c]) * TILE_ROWS + r;
+        const float2 ml = __ldcg(p.part_ml + slot);
+        if (ml.x == -INFINITY) continue;
+        const float next = fmaxf(best, ml.x), f = exp2_fast(best - next), k = exp2_fast(ml.x - next);
+        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot * D + col));
+        acc = make_float4(acc.x * f + v.x * k, acc.y * f + v.y * k, acc.z * f + v.z * k, acc.w * f + v.w * k);
+        sum = sum * f + ml.y * k;
+        best = next;
       }
-      const int* table = p.a.page_table + w.b * p.a.table_row;
-      const char* kbase = static_cast<const char*>(p.a.cache.k) + w.head * p.a.cache.head_stride * ES;
-      const char* vbase = static_cast<const char*>(p.a.cache.v) + w.head * p.a.cache.head_stride * ES;
-      auto look_up = [&](int j, long& off, long& scale_off) {
-        const int key = key0 + j * TILE_KEYS + pw * 32 + lane;
-        off = scale_off = -1;
-        if (j < nb && key >= lo && key < hi) {
-          const int pg = p.page_shift >= 0 ? key >> p.page_shift : key / static_cast<int>(p.a.cache.page_size);
-          const int sl = key - pg * static_cast<int>(p.a.cache.page_size);
-          const int page = table[pg];
-          if (page >= 0 && page < p.a.cache.pages) {
-            off = (page * p.a.cache.page_stride + sl * p.a.cache.slot_stride) * ES;
-            scale_off = page * p.a.cache.scale_page + sl * p.a.cache.scale_slot + w.head * p.a.cache.scale_head;
-          } else {
-            tj_report(p.status, TJ_STATUS_BOUNDS, WHERE + SITE_PAGE);
-          }
-        }
-      };
-      long off, soff;
-      look_up(0, off, soff);
-      if constexpr (!Q8) {
-        constexpr int LPR = D / 8, PER = 32 / LPR;  // lanes of a row, rows of a warp's instruction
-        const int piece = lane % LPR;
-        auto copy = [&](uint8_t* dst, const char* base) {
-#pragma unroll
-          for (int i = 0; i < 32 / PER; ++i) {
-            const int r = i * PER + lane / LPR;
-            const long ro = __shfl_sync(0xffffffffu, off, r);
-            cp_async16(smem_u32(dst) + swizzled(TILE_KEYS, pw * 32 + r, piece), base + (ro < 0 ? 0 : ro) + piece * 16, ro >= 0);
-          }
-          cp_async_commit();
-        };
-        auto arrive = [&](uint64_t* bar) {
-          fence_proxy_async_smem();
-          mbar_arrive(smem_u32(bar));
-        };
-        for (int j = 0; j < nb; ++j) {
-          const int it = blocks + j, s = it % STAGES;
-          const uint32_t ph = (it / STAGES) & 1;
-          ok = mbar_wait_warp(smem_u32(&k_empty[s]), ph ^ 1u, abort_flag, p.status, WHERE + 5);
-          if (!ok) break;
-          copy(sK + s * KV_BYTES, kbase);
-          if (j == 0) {
-            cp_async_wait<1>();
-            arrive(q_full);
-          } else {
-            cp_async_wait<1>();  // the block before's values
-            arrive(&v_full[(it - 1) % STAGES]);
-          }
-          ok = mbar_wait_warp(smem_u32(&v_empty[s]), ph ^ 1u, abort_flag, p.status, WHERE + 6);
-          if (!ok) break;
-          copy(sV + s * KV_BYTES, vbase);
-          look_up(j + 1, off, soff);
-          cp_async_wait<1>();
+      const bool none = best == -INFINITY;
+      const float inv = none ? 0.0f : 1.0f / sum;
+      int tok, hd;
+      row_of(p, head, r0 + r, tok, hd);
+      T* dst = static_cast<T*>(p.a.out) + (first_token + tok) * p.a.out_token + hd * p.a.out_head + col;
+      uint2 y;
+      y.x = pack2<T>(none ? 0.0f : acc.x * inv, none ? 0.0f : acc.y * inv);
+      y.y = pack2<T>(none ? 0.0f : acc.z * inv, none ? 0.0f : acc.w * inv);
+      *reinterpret_cast<uint2*>(dst) = y;
+      if (p.a.lse && col == 0)
+        p.a.lse[(first_token + tok) * p.a.q_heads + hd] = none ? -INFINITY : (best - C::SHIFT + log2f(sum)) * 0.69314718055994531f;
+    }
+    __syncthreads();  // the slots lie where the next keys go
+  }
+  return true;
+}
+
+// ---- producers: the queries of a segment, then its keys and values block by block ------------------------------
+template <class T, int CD, int D>
+TJ_DEV void produce(const AttnParams& p, const TilesShared<T, CD, D>& sh, int seg, int blocks) {
+  using namespace tjg;
+  using C = Tiles<T, CD, D>;
+  using S = TilesShared<T, CD, D>;
+  constexpr int STAGES = C::STAGES, ES = C::Q8 ? 1 : 2;
+  volatile Segment& g = sh.segment(seg);
+  const int warp = (threadIdx.x >> 5) - 8, tid = threadIdx.x - 256, lane = threadIdx.x & 31;
+  const bool keys = warp < 2;         // this warp brings keys, or values
+  const int row0 = (warp & 1) * 32;  // its rows of a block
+  const int nb = g.nb, key0 = g.key0 + row0, lo = g.lo, hi = g.hi, head = g.head;
+  {
+    constexpr int LPR = D / 8;  // 16-byte pieces of a row
+    const int piece = tid % LPR, rows = g.rows, r0 = g.r0, first_token = g.s.start, last = rows > 128 ? 256 : 128;
+    for (int r = tid / LPR; r < last; r += 128 / LPR) {
+      int tok, hd;
+      row_of(p, head, r0 + (r < rows ? r : 0), tok, hd);
+      const T* src = static_cast<const T*>(p.a.q) + (first_token + tok) * p.a.q_token + hd * p.a.q_head + piece * 8;
+      cp_async16(sh.at(S::Q) + (r >> 7) * C::Q_BYTES + swizzled(128, r & 127, piece), src, r < rows);
+    }
+    cp_async_commit();
+  }
+  const int* table = p.a.page_table + g.b * p.a.table_row;
+  const char* base = static_cast<const char*>(keys ? p.a.cache.k : p.a.cache.v) + head * p.a.cache.head_stride * ES;
+  const uint32_t full = keys ? S::K_FULL : S::V_FULL, empty = keys ? S::K_EMPTY : S::V_EMPTY, dst0 = sh.at(keys ? S::K : S::V);
+  // This lane's key of block j: its page (looked up a block before it is used), then the byte offset
+  // of its row and its place among the scales (-1: not there).
+  const int page_size = static_cast<int>(p.a.cache.page_size);
+  auto page_of = [&](int j) {
+    const int key = key0 + j * TILE_KEYS + lane;
+    if (j >= nb || key < lo || key >= hi) return INT_MIN;
+    return table[p.page_shift >= 0 ? key >> p.page_shift : key / page_size];
+  };
+  long off, soff;
+  auto place = [&](int j, int page) {
+    off = soff = -1;
+    if (page >= 0 && page < p.a.cache.pages) {
+      const int key = key0 + j * TILE_KEYS + lane;
+      const int slot = p.page_shift >= 0 ? key & (page_size - 1) : key % page_size;
+      off = (page * p.a.cache.page_stride + slot * p.a.cache.slot_stride) * ES;
+      if (C::Q8) soff = page * p.a.cache.scale_page + slot * p.a.cache.scale_slot + head * p.a.cache.scale_head;
+    } else if (page != INT_MIN) {
+      tj_report(p.status, TJ_STATUS_BOUNDS, OP_ATTENTION * 16 + SITE_PAGE);
+    }
+  };
+  auto arrive = [&](uint32_t bar) {
+    fence_proxy_async_smem();
+    mbar_arrive(sh.at(bar));
+  };
+  auto announce = [&](int it) {
 #ifdef TJ_TEST_STALL_FIRST_LOAD
-          // failure-path test build only: the first keys never arrive, so the wait for them runs out
-          if (it == 0) continue;
+    // failure-path test build only: the first keys never arrive, so the wait for them runs out
+    if (it == 0 && keys) return;
 #endif
-          arrive(&k_full[s]);
-        }
-        cp_async_wait<0>();
-        if (ok) arrive(&v_full[(blocks + nb - 1) % STAGES]);
-      } else {
-        constexpr int LPR = D / 16, PER = 32 / LPR, N = 32 / PER;
-        const int piece = lane % LPR;  // 16 codes: two pieces of the 16-bit row
-        uint4 kr[N], vr[N];
-        float ks, vs;
-        auto load = [&]() {
+    arrive(full + 8 * (it % STAGES));
+  };
+  place(0, page_of(0));
+  int next_page = page_of(1);
+  if constexpr (!C::Q8) {
+    constexpr int LPR = D / 8, PER = 32 / LPR;  // lanes of a row, rows of a warp's instruction
+    const int piece = lane % LPR;
+    for (int j = 0; j < nb; ++j) {
+      const int it = blocks + j, s = it % STAGES;
+      if (!sh.wait(empty + 8 * s, it / STAGES + 1, p, 5)) break;
+      const uint32_t dst = dst0 + s * C::KV_BYTES;
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const long ro = __shfl_sync(0xffffffffu, off, i * PER + lane / LPR);
-            kr[i] = vr[i] = make_uint4(0, 0, 0, 0);
-            if (ro >= 0) {
-              kr[i] = tj_ld16_stream(kbase + ro + piece * 16);
-              vr[i] = tj_ld16_stream(vbase + ro + piece * 16);
-            }
-          }
-          ks = vs = 0.0f;
-          if (soff >= 0) {
-            ks = __ldg(p.a.cache.k_scale + soff);
-            vs = __ldg(p.a.cache.v_scale + soff);
-          }
-        };
-        auto store = [&](uint8_t* dst, const uint4 (&raw)[N]) {
+      for (int i = 0; i < 32 / PER; ++i) {
+        const int r = i * PER + lane / LPR;
+        const long ro = __shfl_sync(0xffffffffu, off, r);
+        cp_async16(dst + swizzled(TILE_KEYS, row0 + r, piece), base + (ro < 0 ? 0 : ro) + piece * 16, ro >= 0);
+      }
+      cp_async_commit();
+      cp_async_wait<1>();  // the copy before this one is there
+      if (j == 0)
+        arrive(S::Q_FULL);
+      else
+        announce(it - 1);
+      place(j + 1, next_page);
+      next_page = page_of(j + 2);
+    }
+    cp_async_wait<0>();
+    if (!*sh.abort_flag()) announce(blocks + nb - 1);
+  } else {
+    constexpr int LPR = D / 16, PER = 32 / LPR, N = 32 / PER;
+    const int piece = lane % LPR;  // 16 codes: two pieces of the 16-bit row
+    uint4 raw[N];
+    float ks, vs;
+    auto load = [&]() {
 #pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const int r = pw * 32 + i * PER + lane / LPR;
-            uint32_t h[2][4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const uint32_t x = e == 0 ? raw[i].x : e == 1 ? raw[i].y : e == 2 ? raw[i].z : raw[i].w;
-              h[e >> 1][(e & 1) * 2] = Codes<T, CD>::make(__byte_perm(x, 0, CD == TJ_I8 ? 0x4140 : 0x1404));
-              h[e >> 1][(e & 1) * 2 + 1] = Codes<T, CD>::make(__byte_perm(x, 0, CD == TJ_I8 ? 0x4342 : 0x3424));
-            }
-            // at head dim 128 a row's lanes reach both panels, whose banks are the same: the upper
-            // half stores its odd piece first
-            const bool swap = D == 128 && piece >= LPR / 2;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int o = swap ? e ^ 1 : e;
-              st_shared16(smem_u32(dst) + swizzled(TILE_KEYS, r, piece * 2 + o), swap ? h[e ^ 1][0] : h[e][0],
-                          swap ? h[e ^ 1][1] : h[e][1], swap ? h[e ^ 1][2] : h[e][2], swap ? h[e ^ 1][3] : h[e][3]);
-            }
-          }
-        };
-        load();
-        cp_async_wait<0>();
-        fence_proxy_async_smem();
-        mbar_arrive(smem_u32(q_full));
-        for (int j = 0; j < nb; ++j) {
-          const int it = blocks + j, s = it % STAGES;
-          const uint32_t ph = (it / STAGES) & 1;
-          look_up(j + 1, off, soff);
-          ok = mbar_wait_warp(smem_u32(&k_empty[s]), ph ^ 1u, abort_flag, p.status, WHERE + 5);
-          if (!ok) break;
-          float* sc = scales + (it % C::SCALES) * 3 * TILE_KEYS + pw * 32 + lane;
+      for (int i = 0; i < N; ++i) {
+        const long ro = __shfl_sync(0xffffffffu, off, i * PER + lane / LPR);
+        raw[i] = make_uint4(0, 0, 0, 0);
+        if (ro >= 0) raw[i] = tj_ld16_stream(base + ro + piece * 16);
+      }
+      ks = vs = 0.0f;
+      if (keys && soff >= 0) {  // the keys' producers bring both scales
+        ks = __ldg(p.a.cache.k_scale + soff);
+        vs = __ldg(p.a.cache.v_scale + soff);
+      }
+    };
+    load();
+    place(1, next_page);
+    next_page = page_of(2);
+    cp_async_wait<0>();
+    arrive(S::Q_FULL);
+    for (int j = 0; j < nb; ++j) {
+      const int it = blocks + j, s = it % STAGES;
+      if (!sh.wait(empty + 8 * s, it / STAGES + 1, p, 5)) break;
+      if (keys) {
+        float* sc = sh.scales(it) + row0 + lane;
+        sc[0] = ks * p.scale_log2;
+        if constexpr (C::MUL_V) sc[TILE_KEYS] = vs;
+        if constexpr (C::EXP_V) {
           const float lv = fmaxf(__log2f(vs), MIN_LOG2_SCALE);
-          sc[0] = ks * p.scale_log2;
           sc[TILE_KEYS] = lv;
           sc[2 * TILE_KEYS] = exp2_fast(-lv);
-          store(sK + s * KV_BYTES, kr);
-          fence_proxy_async_smem();
-          mbar_arrive(smem_u32(&k_full[s]));
-          ok = mbar_wait_warp(smem_u32(&v_empty[s]), ph ^ 1u, abort_flag, p.status, WHERE + 6);
-          if (!ok) break;
-          store(sV + s * KV_BYTES, vr);
-          fence_proxy_async_smem();
-          mbar_arrive(smem_u32(&v_full[s]));
-          if (j + 1 < nb) load();
         }
+        mbar_arrive(sh.at(S::SC_FULL + 8 * (it % C::SCALES)));
       }
-    } else if constexpr (ROLE == Role::matrix) {
-      if (warp == 12) {
-      // ---------------- matrix instructions ----------------
-      const uint64_t dq = desc_sw128(smem_u32(sQ), 16, 1024), dk = desc_sw128(smem_u32(sK), 16, 1024),
-                     dv = desc_sw128(smem_u32(sV), TILE_KEYS * 128, 1024);
-      bool ok = mbar_wait_warp(smem_u32(q_full), seg & 1, abort_flag, p.status, WHERE + 7);
-      bool issued = false;
-      auto scores = [&](int t, int s) {
-        const uint64_t a = dq + ((t * Q_BYTES) >> 4), b = dk + ((s * KV_BYTES) >> 4);
-#pragma unroll
-        for (int k = 0; k < D / 16; ++k) {
-          const uint32_t step = (k >> 2) * (128 * 128 >> 4) + (k & 3) * 2;
-          umma_f16_elect(tmem + t * 128, a + step, b + step, IDESC_S, k > 0);
-        }
-        umma_commit_elect(smem_u32(&s_full[t]));
-        issued = true;
-      };
-      auto values = [&](int t, int s, bool acc) {
-        const uint64_t b = dv + ((s * KV_BYTES) >> 4);
-#pragma unroll
-        for (int k = 0; k < TILE_KEYS / 16; ++k)
-          tja::umma_f16_ts_elect(tmem + 256 + t * D, tmem + t * 128 + k * 8, b + ((k * 16 * 128) >> 4), IDESC_O, (acc || k > 0) ? 1u : 0u);
-      };
-      if (ok) ok = mbar_wait_warp(smem_u32(&k_full[blocks % STAGES]), (blocks / STAGES) & 1, abort_flag, p.status, WHERE + 8);
-      if (ok) {
-        tc_fence_after();
-        for (int t = 0; t < ntiles; ++t) scores(t, blocks % STAGES);
-        umma_commit_elect(smem_u32(&k_empty[blocks % STAGES]));
-      }
-      for (int j = 0; j < nb && ok; ++j) {
-        const int it = blocks + j, s = it % STAGES, s1 = (it + 1) % STAGES;
-        ok = mbar_wait_warp(smem_u32(&v_full[s]), (it / STAGES) & 1, abort_flag, p.status, WHERE + 9);
-        for (int t = 0; t < ntiles && ok; ++t) {
-          ok = mbar_wait_warp(smem_u32(&p_ready[t]), ((t == 0 ? blocks : blocks1) + j) & 1, abort_flag, p.status, WHERE + 10);
-          if (!ok) break;
-          tc_fence_after();
-          values(t, s, j > 0);
-          if (t == ntiles - 1) umma_commit_elect(smem_u32(&v_empty[s]));
-          if (j + 1 < nb) {
-            if (t == 0) ok = mbar_wait_warp(smem_u32(&k_full[s1]), ((it + 1) / STAGES) & 1, abort_flag, p.status, WHERE + 8);
-            if (!ok) break;
-            tc_fence_after();
-            scores(t, s1);
-            if (t == ntiles - 1) umma_commit_elect(smem_u32(&k_empty[s1]));
-          }
-        }
-      }
-      if (ok) umma_commit_elect(smem_u32(o_done));
-      if (!ok && issued) {
-        umma_commit_elect(smem_u32(drain));
-        volatile int no_abort = 0;
-        mbar_wait_warp(smem_u32(drain), 0, &no_abort, p.status, WHERE + 11, 200000000ull);
-      }
-      }
-    } else {
-      // ---------------- softmax ----------------
-      const int t = warp >> 2, q = warp & 3, r = t * 128 + q * 32 + lane;
-      const uint32_t at = static_cast<uint32_t>(q * 32) << 16;
-      const uint32_t tS = tmem + at + t * 128, tO = tmem + at + 256 + t * D;
-      if (t < ntiles) {
-        const int rr = min(r, rows - 1), tok = (r0 + rr) / p.group, hd = w.head * p.group + (r0 + rr) - tok * p.group;
-        int rlo, rhi;
-        row_range(p, w.s, tok, rlo, rhi);
-        // keys that every row of this warp sees need no mask
-        const int clo = __reduce_max_sync(0xffffffffu, rlo), chi = __reduce_min_sync(0xffffffffu, rhi);
-        float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;
-        bool ok = true;
-        for (int j = 0; j < nb; ++j) {
-          const int it = blocks + j, kb = key0 + j * TILE_KEYS;
-          ok = mbar_wait_warp(smem_u32(&s_full[t]), ((t == 0 ? blocks : blocks1) + j) & 1, abort_flag, p.status, WHERE + 12);
-          if (Q8 && ok)  // the scales were written before the keys' barrier
-            ok = mbar_wait_warp(smem_u32(&k_full[it % STAGES]), (it / STAGES) & 1, abort_flag, p.status, WHERE + 12);
-          if (!ok) break;
-          tc_fence_after();
-          uint32_t raw[128];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) tja::tmem_ld32_async(tS + 32 * i, raw + 32 * i);
-          asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-          float x[128];
-#pragma unroll
-          for (int i = 0; i < 128; ++i) {
-            asm volatile("" : "+r"(raw[i]));  // not before the wait
-            x[i] = __uint_as_float(raw[i]);
-          }
-          const float* sc = scales + (it % C::SCALES) * 3 * TILE_KEYS;
-          if constexpr (Q8) {
-#pragma unroll
-            for (int i = 0; i < 128; i += 4) {
-              const float4 k = *reinterpret_cast<const float4*>(sc + i), v = *reinterpret_cast<const float4*>(sc + TILE_KEYS + i);
-              x[i] = fmaf(x[i], k.x, v.x);
-              x[i + 1] = fmaf(x[i + 1], k.y, v.y);
-              x[i + 2] = fmaf(x[i + 2], k.z, v.z);
-              x[i + 3] = fmaf(x[i + 3], k.w, v.w);
-            }
-          }
-          if (kb < clo || kb + TILE_KEYS > chi) {
-            const int a = rlo - kb, b = rhi - kb;
-#pragma unroll
-            for (int i = 0; i < 128; ++i)
-              if (i < a || i >= b) x[i] = -INFINITY;
-          }
-          float h0 = x[0], h1 = x[1], h2 = x[2], h3 = x[3];
-#pragma unroll
-          for (int i = 4; i < 124; i += 8) {
-            h0 = tja::fmax3(h0, x[i], x[i + 4]);
-            h1 = tja::fmax3(h1, x[i + 1], x[i + 5]);
-            h2 = tja::fmax3(h2, x[i + 2], x[i + 6]);
-            h3 = tja::fmax3(h3, x[i + 3], x[i + 7]);
-          }
-          h0 = tja::fmax3(h0, x[124], x[125]);
-          h1 = tja::fmax3(h1, x[126], x[127]);
-          const float c = Q8 ? 1.0f : p.scale_log2;
-          const float top = tja::fmax3(h0, h1, fmaxf(h2, h3)) * c;
-          float alpha = 1.0f;
-          const bool raise = top > m + C::RAISE || (m == -INFINITY && top > m);
-          if (raise) {
-            alpha = exp2_fast(m - top);
-            m = top;
-            l0 *= alpha;
-            l1 *= alpha;
-          }
-          const float base = (m == -INFINITY ? 0.0f : m) - C::SHIFT;
-          const uint64_t cc = tja::f2_pack(c, c), nb2 = tja::f2_pack(-base, -base);
-#pragma unroll
-          for (int g = 0; g < 4; ++g) {
-            uint32_t pk[16];
-            uint64_t ll = tja::f2_pack(l0, l1);
-#pragma unroll
-            for (int k = 0; k < 16; ++k) {
-              const int i = g * 32 + 2 * k;
-              float e0, e1;
-              if constexpr (Q8)
-                tja::f2_unpack(tja::f2_add(tja::f2_pack(x[i], x[i + 1]), nb2), e0, e1);
-              else
-                tja::f2_unpack(tja::f2_fma(tja::f2_pack(x[i], x[i + 1]), cc, nb2), e0, e1);
-              e0 = exp2_fast(e0);
-              e1 = exp2_fast(e1);
-              if constexpr (Q8) {
-                const float2 inv = *reinterpret_cast<const float2*>(sc + 2 * TILE_KEYS + i);
-                ll = tja::f2_fma(tja::f2_pack(e0, e1), tja::f2_pack(inv.x, inv.y), ll);
-              } else {
-                ll = tja::f2_add(ll, tja::f2_pack(e0, e1));
-              }
-              pk[k] = pack2<T>(e0, e1);
-            }
-            tja::f2_unpack(ll, l0, l1);
-            tja::tmem_st16(tS + 16 * g, pk);
-          }
-          if (j > 0 && __any_sync(0xffffffffu, raise)) {
-            // the scores' barrier followed the previous product's, so O is at rest
-#pragma unroll 1
-            for (int i = 0; i < D; i += 32) {
-              float o[32];
-              tmem_ld32(tO + i, o);
-#pragma unroll
-              for (int k = 0; k < 32; ++k) o[k] *= alpha;
-              tja::tmem_st32_wait(tO + i, o);
-            }
-          }
-          tja::tmem_wait_st();
-          tc_fence_before();
-          mbar_arrive(smem_u32(&p_ready[t]));
-        }
-        if (ok) ok = mbar_wait_warp(smem_u32(o_done), seg & 1, abort_flag, p.status, WHERE + 13);
-        if (ok) {
-          tc_fence_after();
-          const float l = l0 + l1;
-          if (l != l && m == -INFINITY) m = 0.0f;  // only NaN scores: the row is NaN, not empty
-          const bool none = m == -INFINITY;
-          if (whole) {
-            const float inv = none ? 0.0f : 1.0f / l;
-            T* dst = static_cast<T*>(p.a.out) + (w.s.start + tok) * p.a.out_token + hd * p.a.out_head;
-#pragma unroll 1
-            for (int i = 0; i < D; i += 32) {
-              float o[32];
-              tmem_ld32(tO + i, o);
-              if (r < rows) {
-#pragma unroll
-                for (int k = 0; k < 32; ++k) o[k] = none ? 0.0f : o[k] * inv;
-#pragma unroll
-                for (int k = 0; k < 32; k += 8) tj_store_vec(dst + i + k, o + k);
-              }
-            }
-            if (p.a.lse && r < rows)
-              p.a.lse[(w.s.start + tok) * p.a.q_heads + hd] = none ? -INFINITY : (m - C::SHIFT + log2f(l)) * 0.69314718055994531f;
-          } else {
-            const long slot = (2L * blockIdx.x + (a0 > 0 ? 0 : 1)) * TILE_ROWS + r;
-#pragma unroll 1
-            for (int i = 0; i < D; i += 32) {
-              float o[32];
-              tmem_ld32(tO + i, o);
-              if (r < rows)
-#pragma unroll
-                for (int k = 0; k < 32; k += 4)
-                  __stcg(reinterpret_cast<float4*>(p.part_o + slot * D + i + k), make_float4(o[k], o[k + 1], o[k + 2], o[k + 3]));
-            }
-            if (r < rows) __stcg(p.part_ml + slot, make_float2(m, l));
-          }
-          tc_fence_before();
-        }
-      }
-    }
-    ++seg;
-    blocks += nb;
-    if (ntiles == 2) blocks1 += nb;
-    __syncwarp();
-    if (!whole) __threadfence();
-    __syncthreads();
-    tc_fence_after();
-    failed = *abort_flag != 0;
-    if (!whole && !failed) {
-      const int c0 = static_cast<int>(((w.start + 1) * parts - 1) / total),
-                c1 = static_cast<int>(((w.start + w.weight) * parts - 1) / total);
-      if (threadIdx.x == 0) {
-        const int done = atomicAdd(p.counters + c0, nb) + nb;
-        *s_last = done == all;
-        if (done == all) p.counters[c0] = 0;  // ready for the next call
-      }
-      __syncthreads();
-      if (*s_last) {
-        __threadfence();
-        constexpr int V4 = D / 4;
-        for (int e = threadIdx.x; e < rows * V4; e += 512) {
-          const int r = e / V4, col = (e - r * V4) * 4;
-          float best = -INFINITY, sum = 0.0f;
-          float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-          for (int c = c0; c <= c1; ++c) {
-            const long pc = total * c / parts, b0 = max(0L, pc - w.start), b1 = min(w.weight, total * (c + 1) / parts - w.start);
-            if (b0 * all / w.weight == b1 * all / w.weight) continue;
-            const long slot = (2L * c + (b0 > 0 ? 0 : 1)) * TILE_ROWS + r;
-            const float2 ml = __ldcg(p.part_ml + slot);
-            if (ml.x == -INFINITY) continue;
-            const float next = fmaxf(best, ml.x), f = exp2_fast(best - next), g = exp2_fast(ml.x - next);
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot * D + col));
-            acc = make_float4(acc.x * f + v.x * g, acc.y * f + v.y * g, acc.z * f + v.z * g, acc.w * f + v.w * g);
-            sum = sum * f + ml.y * g;
-            best = next;
-          }
-          const bool none = best == -INFINITY;
-          const float inv = none ? 0.0f : 1.0f / sum;
-          const int tok = (r0 + r) / p.group, hd = w.head * p.group + (r0 + r) - tok * p.group;
-          T* dst = static_cast<T*>(p.a.out) + (w.s.start + tok) * p.a.out_token + hd * p.a.out_head + col;
-          uint2 y;
-          y.x = pack2<T>(none ? 0.0f : acc.x * inv, none ? 0.0f : acc.y * inv);
-          y.y = pack2<T>(none ? 0.0f : acc.z * inv, none ? 0.0f : acc.w * inv);
-          *reinterpret_cast<uint2*>(dst) = y;
-          if (p.a.lse && col == 0)
-            p.a.lse[(w.s.start + tok) * p.a.q_heads + hd] = none ? -INFINITY : (best - C::SHIFT + log2f(sum)) * 0.69314718055994531f;
-        }
-      }
+      store_rows<T, CD, D>(dst0 + s * C::KV_BYTES, raw, row0);
+      announce(it);
+      load();  // the next block's
+      place(j + 2, next_page);
+      next_page = page_of(j + 3);
     }
   }
+}
+
+// ---- matrix instructions -----------------------------------------------------------------------------------------
+// Four steps of 16 of the scores' product, both operands K-major: 32 bytes a step.
+TJ_DEV void umma_scores4(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n .reg .b64 a, b;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n"
+      " add.s64 a, %1, 2;\n add.s64 b, %2, 2;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n"
+      " add.s64 a, %1, 4;\n add.s64 b, %2, 4;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n"
+      " add.s64 a, %1, 6;\n add.s64 b, %2, 6;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, 1;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+// Four steps of 16 keys of P V: P 8 columns of TMEM a step, V 16 rows of 128 bytes.
+TJ_DEV void umma_values4(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n .reg .pred p, e;\n .reg .b64 b;\n .reg .b32 a;\n elect.sync _|e, 0xffffffff;\n setp.ne.b32 p, %4, 0;\n"
+      " @e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n"
+      " add.s32 a, %1, 8;\n add.s64 b, %2, 128;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, 1;\n"
+      " add.s32 a, %1, 16;\n add.s64 b, %2, 256;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, 1;\n"
+      " add.s32 a, %1, 24;\n add.s64 b, %2, 384;\n @e tcgen05.mma.cta_group::1.kind::f16 [%0], [a], b, %3, 1;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Row tile t's products.  blocks: key blocks before this segment; tile_blocks: those of them that the tile had.
+// A stage of keys or values is free when both tiles are done with it: two arrivals, both by tile 0's
+// warp where there is no tile 1.
+template <class T, int CD, int D>
+TJ_DEV void multiply(const AttnParams& p, const TilesShared<T, CD, D>& sh, uint32_t tmem, int seg, int t, int blocks, int tile_blocks) {
+  using namespace tjg;
+  using C = Tiles<T, CD, D>;
+  using S = TilesShared<T, CD, D>;
+  constexpr int STAGES = C::STAGES;
+  constexpr uint32_t IDESC_S = idesc_f16(C::BF, 128, TILE_KEYS, false, false), IDESC_O = idesc_f16(C::BF, 128, D, false, true);
+  const int nb = sh.segment(seg).nb;
+  const bool alone = sh.segment(seg).rows <= 128;
+  const uint64_t dq = desc_sw128(sh.at(S::Q) + t * C::Q_BYTES, 16, 1024), dk = desc_sw128(sh.at(S::K), 16, 1024),
+                 dv = desc_sw128(sh.at(S::V), TILE_KEYS * 128, 1024);
+  const uint32_t tS = tmem + t * 128, tO = tmem + 256 + t * D;
+  const uint32_t s_full = sh.at(S::S_FULL + 16 * t), pv_done = sh.at(S::PV_DONE + 16 * t);
+  auto release = [&](uint32_t bar) {
+    umma_commit_elect(bar);
+    if (alone) umma_commit_elect(bar);
+  };
+  bool issued = false;
+  auto scores = [&](int j) {
+    const int buf = (tile_blocks + j) & 1, s = (blocks + j) % STAGES;
+    const uint64_t b = dk + ((s * C::KV_BYTES) >> 4);
+#pragma unroll
+    for (int k = 0; k < D / 64; ++k)
+      umma_scores4(tS + buf * 64, dq + k * (128 * 128 >> 4), b + k * (TILE_KEYS * 128 >> 4), IDESC_S, k > 0);
+    umma_commit_elect(s_full + 8 * buf);
+    release(sh.at(S::K_EMPTY + 8 * s));
+    issued = true;
+  };
+  bool ok = sh.wait(S::Q_FULL, seg, p, 7);
+  for (int j = 0; j < min(nb, 2) && ok; ++j) {
+    ok = sh.wait(S::K_FULL + 8 * ((blocks + j) % STAGES), (blocks + j) / STAGES, p, 8);
+    if (!ok) break;
+    tc_fence_after();
+    scores(j);
+  }
+  for (int j = 0; j < nb && ok; ++j) {
+    const int it = blocks + j, s = it % STAGES, use = tile_blocks + j, buf = use & 1;
+    const int ahead = j + 2 < nb ? it + 2 : it;  // keys that have arrived stand for none
+    ok = sh.wait3(S::K_FULL + 8 * (ahead % STAGES), ahead / STAGES, S::V_FULL + 8 * s, it / STAGES, S::P_READY + 8 * (2 * t + buf), use >> 1, p, 8);
+    if (!ok) break;
+    tc_fence_after();
+    umma_values4(tO, tS + buf * 64, dv + ((s * C::KV_BYTES) >> 4), IDESC_O, j > 0);
+    if (j + 2 < nb) scores(j + 2);
+    umma_commit_elect(pv_done + 8 * buf);
+    release(sh.at(S::V_EMPTY + 8 * s));
+  }
+  if (!ok && issued) {
+    umma_commit_elect(sh.at(S::DRAIN + 8 * t));
+    volatile int no_abort = 0;
+    mbar_wait_warp(sh.at(S::DRAIN + 8 * t), 0, &no_abort, p.status, OP_ATTENTION * 16 + 11, 200000000ull);
+  }
+}
+
+// ---- softmax -------------------------------------------------------------------------------------------------------
+// tile_blocks: blocks of this warp's row tile before the segment
+template <class T, int CD, int D>
+TJ_DEV void softmax(const AttnParams& p, const TilesShared<T, CD, D>& sh, uint32_t tmem, int seg, int blocks, int tile_blocks) {
+  using namespace tjg;
+  using C = Tiles<T, CD, D>;
+  using S = TilesShared<T, CD, D>;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int t = warp >> 2, q = warp & 3, r = t * 128 + q * 32 + lane;
+  const uint32_t lanes = tmem + (static_cast<uint32_t>(q * 32) << 16);
+  const uint32_t tO = lanes + 256 + t * D;
+  volatile Segment& g = sh.segment(seg);
+  const int nb = g.nb;
+  int rlo, rhi;
+  {
+    Seq s;
+    s.start = g.s.start;
+    s.n = g.s.n;
+    s.len = g.s.len;
+    row_range(p, s, (g.r0 + min(r, g.rows - 1)) / p.group, rlo, rhi);
+  }
+  // keys that every row of this warp sees need no mask; from here on relative to the segment's first key
+  rlo -= g.key0;
+  rhi -= g.key0;
+  const int clo = __reduce_max_sync(0xffffffffu, rlo), chi = __reduce_min_sync(0xffffffffu, rhi);
+  float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+  bool ok = true;
+  for (int j = 0; j < nb; ++j) {
+    const int it = blocks + j, use = tile_blocks + j, kb = j * TILE_KEYS;
+    const uint32_t tS = lanes + (2 * t + (use & 1)) * 64;
+    ok = sh.wait(S::S_FULL + 8 * (2 * t + (use & 1)), use >> 1, p, 12);
+    if (C::Q8 && ok) ok = sh.wait(S::SC_FULL + 8 * (it % C::SCALES), it / C::SCALES, p, 15);
+    if (!ok) break;
+    tc_fence_after();
+    uint32_t raw[64];
+    tja::tmem_ld64(tS, raw);
+    float x[64];
+#pragma unroll
+    for (int i = 0; i < 64; ++i) x[i] = __uint_as_float(raw[i]);
+    const float* sc = sh.scales(it);
+    if constexpr (C::Q8) {
+#pragma unroll
+      for (int i = 0; i < 64; i += 4) {
+        const float4 k = *reinterpret_cast<const float4*>(sc + i);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if constexpr (C::EXP_V) v = *reinterpret_cast<const float4*>(sc + TILE_KEYS + i);
+        x[i] = fmaf(x[i], k.x, v.x);
+        x[i + 1] = fmaf(x[i + 1], k.y, v.y);
+        x[i + 2] = fmaf(x[i + 2], k.z, v.z);
+        x[i + 3] = fmaf(x[i + 3], k.w, v.w);
+      }
+    }
+    const bool masked = kb < clo || kb + TILE_KEYS > chi;  // the same for the warp
+    if (masked) {
+      const int a = rlo - kb, b = rhi - kb;
+#pragma unroll
+      for (int i = 0; i < 64; ++i)
+        if (i < a || i >= b) x[i] = -INFINITY;
+    }
+    float h0 = x[0], h1 = x[1], h2 = x[2], h3 = x[3];
+#pragma unroll
+    for (int i = 4; i < 60; i += 8) {
+      h0 = tja::fmax3(h0, x[i], x[i + 4]);
+      h1 = tja::fmax3(h1, x[i + 1], x[i + 5]);
+      h2 = tja::fmax3(h2, x[i + 2], x[i + 6]);
+      h3 = tja::fmax3(h3, x[i + 3], x[i + 7]);
+    }
+    h0 = tja::fmax3(h0, x[60], x[61]);
+    h1 = tja::fmax3(h1, x[62], x[63]);
+    const float c = C::Q8 ? 1.0f : p.scale_log2;
+    const float top = tja::fmax3(h0, h1, fmaxf(h2, h3)) * c;
+    float alpha = 1.0f;
+    const bool raise = top > m + C::RAISE || (m == -INFINITY && top > m);
+    if (raise) {
+      alpha = exp2_fast(m - top);
+      m = top;
+      l0 *= alpha;
+      l1 *= alpha;
+    }
+    if (j > 0 && __any_sync(0xffffffffu, raise)) {
+      // O at rest.  (A phase is waited for only when the one before it is known to be over: the scores
+      // of block j were made after P V of block j - 2.)
+      ok = sh.wait(S::PV_DONE + 8 * (2 * t + ((use - 1) & 1)), (use - 1) >> 1, p, 14);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll 1
+      for (int i = 0; i < D; i += 16) {
+        uint32_t o[16];
+        tmem_ld16(tO + i, o);
+#pragma unroll
+        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+        tja::tmem_st16_wait(tO + i, o);
+      }
+    }
+    const float base = (m == -INFINITY ? 0.0f : m) - C::SHIFT;
+    const uint64_t cc = tja::f2_pack(c, c), nb2 = tja::f2_pack(-base, -base);
+    uint64_t ll = tja::f2_pack(l0, l1);
+    // hidden keys have to be exactly 0: a masked block's exponentials are all the unit's
+    if (C::EMU == 0 || masked)
+      probabilities<T, C, 0>(x, cc, nb2, sc, ll, tS);
+    else
+      probabilities<T, C, C::EMU>(x, cc, nb2, sc, ll, tS);
+    tja::f2_unpack(ll, l0, l1);
+    tja::tmem_wait_st();
+    tc_fence_before();
+    mbar_arrive(sh.at(S::P_READY + 8 * (2 * t + (use & 1))));
+  }
+  const int last = tile_blocks + nb - 1;
+  if (!ok || !sh.wait(S::PV_DONE + 8 * (2 * t + (last & 1)), last >> 1, p, 13)) return;
+  tc_fence_after();
+  const float l = l0 + l1;
+  if (l != l && m == -INFINITY) m = 0.0f;  // only NaN scores: the row is NaN, not empty
+  const bool none = m == -INFINITY, mine_to_write = r < g.rows;
+  if (nb == g.all) {
+    const float inv = none ? 0.0f : 1.0f / l;
+    int tok, hd;
+    row_of(p, g.head, g.r0 + r, tok, hd);
+    tok += g.s.start;
+    T* dst = static_cast<T*>(p.a.out) + tok * p.a.out_token + hd * p.a.out_head;
+#pragma unroll 1
+    for (int i = 0; i < D; i += 16) {
+      uint32_t o[16];
+      tmem_ld16(tO + i, o);
+      if (mine_to_write) {
+        float y[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) y[k] = none ? 0.0f : __uint_as_float(o[k]) * inv;
+        tj_store_vec(dst + i, y);
+        tj_store_vec(dst + i + 8, y + 8);
+      }
+    }
+    if (p.a.lse && mine_to_write)
+      p.a.lse[static_cast<long>(tok) * p.a.q_heads + hd] = none ? -INFINITY : (m - C::SHIFT + log2f(l)) * 0.69314718055994531f;
+  } else {
+    const long slot = (2L * blockIdx.x + (g.later ? 0 : 1)) * TILE_ROWS + r;
+    float* dst = p.part_o + slot * D;
+#pragma unroll 1
+    for (int i = 0; i < D; i += 16) {
+      uint32_t o[16];
+      tmem_ld16(tO + i, o);
+      if (mine_to_write)
+#pragma unroll
+        for (int k = 0; k < 16; k += 4)
+          __stcg(reinterpret_cast<uint4*>(dst + i + k), make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]));
+    }
+    if (mine_to_write) __stcg(p.part_ml + slot, make_float2(m, l));
+  }
+  tc_fence_before();
 }
 
 template <class T, int CD, int D>
 __global__ void __launch_bounds__(512, 1) attention_tiles(const __grid_constant__ AttnParams p) {
   using namespace tjg;
   using C = Tiles<T, CD, D>;
+  using S = TilesShared<T, CD, D>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  TilesShared<T, CD, D> sh(smem_raw);
+  const S sh(smem_raw);
   const int warp = threadIdx.x >> 5;
-  sh.total = total_work(p);
-  sh.parts = min(static_cast<long>(gridDim.x), max(1L, sh.total / (4L * TILE_KEYS * p.group)));
-  if (sh.total == 0 || blockIdx.x >= sh.parts) return;
-  sh.from = sh.total * blockIdx.x / sh.parts;
-  sh.to = sh.total * (blockIdx.x + 1) / sh.parts;
+  const long total = total_work(p);
+  const Cut cut(total, min(static_cast<long>(gridDim.x), max(1L, total / (512L * p.group))));
+  if (total == 0 || blockIdx.x >= cut.parts) return;
+  long pos = cut.begin(blockIdx.x);
+  const long to = cut.begin(blockIdx.x + 1);
 
   if (threadIdx.x == 0) {
-    mbar_init(smem_u32(sh.q_full), 128);
+    mbar_init(sh.at(S::Q_FULL), 128);
     for (int s = 0; s < C::STAGES; ++s) {
-      mbar_init(smem_u32(&sh.k_full[s]), 128);
-      mbar_init(smem_u32(&sh.v_full[s]), 128);
-      mbar_init(smem_u32(&sh.k_empty[s]), 1);
-      mbar_init(smem_u32(&sh.v_empty[s]), 1);
+      mbar_init(sh.at(S::K_FULL + 8 * s), 64);
+      mbar_init(sh.at(S::V_FULL + 8 * s), 64);
+      mbar_init(sh.at(S::K_EMPTY + 8 * s), 2);
+      mbar_init(sh.at(S::V_EMPTY + 8 * s), 2);
     }
-    for (int t = 0; t < 2; ++t) {
-      mbar_init(smem_u32(&sh.s_full[t]), 1);
-      mbar_init(smem_u32(&sh.p_ready[t]), 128);
+    for (int s = 0; s < C::SCALES; ++s) mbar_init(sh.at(S::SC_FULL + 8 * s), 64);
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(sh.at(S::S_FULL + 8 * i), 1);
+      mbar_init(sh.at(S::P_READY + 8 * i), 128);
+      mbar_init(sh.at(S::PV_DONE + 8 * i), 1);
     }
-    mbar_init(smem_u32(sh.o_done), 1);
-    mbar_init(smem_u32(sh.drain), 1);
-    *sh.abort_flag = 0;
+    mbar_init(sh.at(S::DRAIN), 1);
+    mbar_init(sh.at(S::DRAIN + 8), 1);
+    *sh.abort_flag() = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 12) {
-    tmem_alloc(smem_u32(sh.tmem_slot), C::TMEM);
+    tmem_alloc(sh.at(S::SLOT), C::TMEM);
     tmem_relinquish();
   }
+  if (warp == 14) next_segment(p, pos, to, sh.segment(0));
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem = *sh.tmem_slot;
-  // 512 threads of 128 registers at launch: 2 x 168 + 112 + 64 = 4 x 128 of them afterwards
+  const uint32_t tmem = *sh.tmem_slot();
+  // every role goes through the same segments; `blocks` and the like count on over them, as the
+  // barriers' phases do
+  int blocks = 0;
   if (warp < 8) {
-    regs_inc<168>();
-    tiles_role<Role::softmax, T, CD, D>(p, sh, tmem);
+    regs_inc<C::REGS_S>();
+    int tile_blocks = 0;
+    for (int seg = 0; sh.segment(seg).nb; ++seg) {
+      const bool busy = warp < 4 || sh.segment(seg).rows > 128;
+      if (busy) softmax<T, CD, D>(p, sh, tmem, seg, blocks, tile_blocks);
+      blocks += sh.segment(seg).nb;
+      if (busy) tile_blocks += sh.segment(seg).nb;
+      if (!end_segment<T, CD, D>(p, sh, cut, seg)) break;
+    }
   } else if (warp < 12) {
-    regs_dec<112>();
-    tiles_role<Role::producer, T, CD, D>(p, sh, tmem);
+    regs_dec<C::REGS_P>();
+    for (int seg = 0; sh.segment(seg).nb; ++seg) {
+      produce<T, CD, D>(p, sh, seg, blocks);
+      blocks += sh.segment(seg).nb;
+      if (!end_segment<T, CD, D>(p, sh, cut, seg)) break;
+    }
   } else {
-    regs_dec<64>();
-    tiles_role<Role::matrix, T, CD, D>(p, sh, tmem);
+    regs_dec<C::REGS_M>();
+    int tile_blocks = 0;
+    for (int seg = 0; sh.segment(seg).nb; ++seg) {
+      const bool busy = warp == 12 || (warp == 13 && sh.segment(seg).rows > 128);
+      if (busy) multiply<T, CD, D>(p, sh, tmem, seg, warp - 12, blocks, tile_blocks);
+      if (warp == 14) next_segment(p, pos, to, sh.segment(seg + 1));
+      blocks += sh.segment(seg).nb;
+      if (busy) tile_blocks += sh.segment(seg).nb;
+      if (!end_segment<T, CD, D>(p, sh, cut, seg)) break;
+    }
   }
   __syncthreads();
   if (warp == 12) tmem_dealloc(tmem, C::TMEM);
