@@ -31,7 +31,6 @@ const char* attention_fault(const tj_paged_attention& a) {
 Plan plan(const tj_paged_attention& a, const Device& dev) {
   Plan p;
   const long group = a.q_heads / a.cache.heads;
-  const bool q8 = a.cache.dtype == TJ_I8 || a.cache.dtype == TJ_E4M3;
   p.tiles = a.max_new * group > 16;
   if (p.tiles) {
     p.rows = TILE_ROWS;
@@ -42,27 +41,36 @@ Plan plan(const tj_paged_attention& a, const Device& dev) {
   }
   p.rows = 16;
   const long tiles = a.q_starts ? a.tokens * group / 16 + a.batch : a.batch * ((group + 15) / 16);
-  p.target = dev.sms * (a.cache.dim == 64 ? 4 : 3) * 2;
-  p.min_chunk = q8 ? 256 : 128;
+#ifndef TJS_WAVES
+#define TJS_WAVES 3
+#define TJS_MINC 256
+#endif
+  p.target = dev.sms * 2 * TJS_WAVES;
+  p.min_chunk = TJS_MINC;
   p.grid = a.cache.heads * (tiles + 1) + p.target;
   p.slots = p.grid;
   return p;
 }
 
+// Raises a kernel's shared-memory limit, once a device (doing so twice is harmless).
+template <class K> cudaError_t allow(K kernel, int smem, bool (&ready)[MAX_DEVICES], const Device& dev) {
+  if (ready[dev.index]) return cudaSuccess;
+  const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  ready[dev.index] = e == cudaSuccess;
+  return e;
+}
 template <class T, int CD, int D> cudaError_t launch_dim(const AttnParams& p, const Plan& plan, const Device& dev, cudaStream_t st) {
   const unsigned grid = static_cast<unsigned>(plan.grid);
-  if (!plan.tiles) {
-    attention_rows<T, CD, D><<<grid, 128, 0, st>>>(p);
-    return cudaSuccess;
+  static bool rows_ready[MAX_DEVICES], tiles_ready[MAX_DEVICES];
+  if (plan.tiles) {
+    constexpr int smem = Tiles<T, CD, D>::SMEM;
+    if (const cudaError_t e = allow(attention_tiles<T, CD, D>, smem, tiles_ready, dev)) return e;
+    attention_tiles<T, CD, D><<<grid, 512, smem, st>>>(p);
+  } else {
+    constexpr int smem = Rows<T, CD, D>::SMEM;
+    if (const cudaError_t e = allow(attention_rows<T, CD, D>, smem, rows_ready, dev)) return e;
+    attention_rows<T, CD, D><<<grid, 128, smem, st>>>(p);
   }
-  static bool ready[MAX_DEVICES];  // the shared-memory limit is raised once a device; doing so twice is harmless
-  constexpr int smem = Tiles<T, CD, D>::SMEM;
-  if (!ready[dev.index]) {
-    const cudaError_t e = cudaFuncSetAttribute(attention_tiles<T, CD, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    if (e != cudaSuccess) return e;
-    ready[dev.index] = true;
-  }
-  attention_tiles<T, CD, D><<<grid, 512, smem, st>>>(p);
   return cudaSuccess;
 }
 template <class T, int CD> cudaError_t launch_cache(const AttnParams& p, const Plan& plan, const Device& dev, cudaStream_t st) {

@@ -1,19 +1,25 @@
 // Attention over a paged cache for few rows (single tokens, a few drafted ones): a tile is 16 rows.
 //
 // What bounds it: the cache is read once and a key meets at most 16 rows, 2 x 16 products for each
-// of its bytes at the most, far below the tensor cores' rate; so it is HBM, and the kernel is made
-// of loads.  Keys and values go from global memory straight into the registers that the matrix
-// instruction wants, 16 bytes a load and no shared memory: the order of the head dimension inside a
-// product is free as long as both operands agree, so a thread's 16 bytes of a key serve as its
-// fragments of two (16-bit) or four (8-bit) steps, and the query's fragments are gathered in that
-// order once.  A value's 16 bytes are eight (sixteen) columns of the output, which fixes the order of
-// its columns, undone when it is stored; two keys' bytes are paired by one byte permutation.
+// of its bytes at the most, far below the tensor cores' rate; so it is HBM, and the kernel has to keep
+// enough reads in flight.  Each warp has a ring of its own in shared memory (24 KB, two CTAs of four
+// warps an SM: 192 KB) that asynchronous copies fill two or more blocks ahead, so the main loop has no
+// barrier.  (With the loads straight into registers, where a block's are in flight only until it is
+// used, 64 single tokens over 8192 keys took 387 us, 3700 GB/s.)
 //
-// A warp takes every fourth block of KS keys of its CTA's chunk with a running maximum and sum of
-// its own, so the main loop has no barrier; the four warps' results are joined at the end, and the
-// chunks of a row tile by the CTA that finishes last (in the order of the chunks, so results do not
-// depend on which that is).
+// The order of the head dimension inside a product is free as long as both operands agree, so 16
+// bytes of a key serve a thread as its fragments of two (16-bit) or four (8-bit) steps, read with one
+// instruction, and the query's fragments are gathered in that order once.  A value's 16 bytes are
+// eight (sixteen) columns of the output, which fixes the order of its columns, undone when it is stored;
+// two keys' elements are paired by a byte permutation.  The pieces of a row are permuted by its number
+// so that both ways of reading are free of bank conflicts.
+//
+// A warp takes every fourth block of KS keys of its CTA's chunk with a running maximum and sum of its
+// own; the four warps' results are joined at the end, and the chunks of a row tile by the CTA that
+// finishes last (in the order of the chunks, so results do not depend on which that is).
 #pragma once
+#include <limits.h>
+
 #include "paged_attention.cuh"
 
 namespace tjs {
@@ -32,21 +38,61 @@ template <> TJ_DEV void mma16816<__half>(float (&c)[4], const uint32_t (&a)[4], 
 
 TJ_DEV uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w; }
 
+TJ_DEV void copy16(uint32_t dst, const void* src, bool on) {
+  const int bytes = on ? 16 : 0;  // 0: zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+TJ_DEV void copy4(uint32_t dst, const void* src, bool on) {
+  const int bytes = on ? 4 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+TJ_DEV uint4 lds16(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+TJ_DEV uint2 lds8(uint32_t a) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(a) : "memory");
+  return v;
+}
+
+template <class T, int CD, int D> struct Rows {
+  static constexpr bool Q8 = CD == TJ_I8 || CD == TJ_E4M3;
+  static constexpr int ES = Q8 ? 1 : 2;
+  static constexpr int ROW = D * ES;                            // bytes of a key
+  static constexpr int KS = !Q8 && D == 128 ? 16 : 32;          // keys of a warp's block
+  static constexpr int BLOCK = 2 * KS * ROW;                    // bytes of its keys and values
+  static constexpr int STAGES = 24576 / BLOCK;
+  static constexpr int SCALES = Q8 ? STAGES * KS * 3 * 4 : 0;   // ks; vs or log2 vs; 1 / vs
+  static constexpr int WARP = STAGES * BLOCK + SCALES;
+  static constexpr int SMEM = 4 * WARP;
+  static constexpr bool MUL_V = Q8 && P_SHIFT<T> == 0.0f;       // bf16: P times vs; f16: vs in the exponent
+  // the 16-byte piece of a row in a block; rows of 4 pieces share a line of 8
+  static TJ_DEV uint32_t piece(int row, int i) {
+    constexpr int PIECES = ROW / 16;
+    if (PIECES == 4) return ((row >> 1) * 8 + ((((row & 1) << 2) | i) ^ (((row >> 1) & 3) << 1))) * 16;
+    return (row * PIECES + (i ^ ((((row >> 1) & 3) << 1) ^ ((row & 1) << 2)))) * 16;
+  }
+};
+
 template <class T, int CD, int D>
-__global__ void __launch_bounds__(128, D == 64 ? 4 : 3) attention_rows(const __grid_constant__ AttnParams p) {
-  constexpr bool Q8 = CD == TJ_I8 || CD == TJ_E4M3;
-  constexpr int KS = Q8 ? 32 : 16;       // keys of a warp's block
+__global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__ AttnParams p) {
+  using R = Rows<T, CD, D>;
+  constexpr bool Q8 = R::Q8;
+  constexpr int KS = R::KS, ES = R::ES, STAGES = R::STAGES;
   constexpr int NT = KS / 8;             // score tiles of 8 keys
-  constexpr int ES = Q8 ? 1 : 2;
-  constexpr int KC = D * ES / 64;        // 16-byte pieces of a key a thread holds
+  constexpr int KC = D * ES / 64;        // 16-byte pieces of a key a thread reads
   constexpr int STEPS = Q8 ? 4 : 2;      // products' steps of 16 that a piece serves
-  constexpr int VB = D * ES / 8;         // bytes of a value a thread holds: 32, 16 or 8
+  constexpr int VB = D * ES / 8;         // bytes of a value a thread reads: 32, 16 or 8
   constexpr int VC = VB > 16 ? 2 : 1;    // ... as loads (of 16 bytes, or one of 8)
   constexpr int VW = VB / 4;             // ... as words
   constexpr int OT = D / 8;              // output tiles of 8 columns
   constexpr int PITCH = D + 4;
 
-  __shared__ float s_o[4][16][PITCH];
+  extern __shared__ __align__(128) uint8_t ring[];
+  float(*const s_o)[16][PITCH] = reinterpret_cast<float(*)[16][PITCH]>(ring);  // when the loop is done
+  static_assert(4 * 16 * PITCH * 4 <= R::SMEM, "the warps' results lie over the ring");
   __shared__ float s_m[4][16], s_l[4][16];
   __shared__ int s_last;
 
@@ -74,7 +120,8 @@ __global__ void __launch_bounds__(128, D == 64 ? 4 : 3) attention_rows(const __g
   for (int i = 0; i < 2; ++i) {
     const int r = g + 8 * i, tok = (r0 + r) / p.group, hd = h * p.group + (r0 + r) - tok * p.group;
     const bool on = r < rows;
-    rlo[i] = rhi[i] = 0;
+    rlo[i] = 0;  // a row that is not there sees all, and is not stored
+    rhi[i] = INT_MAX;
     if (on) row_range(p, s, tok, rlo[i], rhi[i]);
     const T* src = static_cast<const T*>(p.a.q) + (s.start + tok) * p.a.q_token + hd * p.a.q_head;
 #pragma unroll
@@ -92,6 +139,9 @@ __global__ void __launch_bounds__(128, D == 64 ? 4 : 3) attention_rows(const __g
     }
   }
 
+  // keys that all of the tile's rows see need no mask
+  const int mlo = __reduce_max_sync(0xffffffffu, max(rlo[0], rlo[1])), mhi = __reduce_min_sync(0xffffffffu, min(rhi[0], rhi[1]));
+
   float o[OT][4];
 #pragma unroll
   for (int i = 0; i < OT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
@@ -102,63 +152,78 @@ __global__ void __launch_bounds__(128, D == 64 ? 4 : 3) attention_rows(const __g
   const char* vbase = static_cast<const char*>(p.a.cache.v) + h * p.a.cache.head_stride * ES;
   const float* ksc = Q8 ? p.a.cache.k_scale + h * p.a.cache.scale_head : nullptr;
   const float* vsc = Q8 ? p.a.cache.v_scale + h * p.a.cache.scale_head : nullptr;
+  const uint32_t my_ring = static_cast<uint32_t>(__cvta_generic_to_shared(ring)) + warp * R::WARP;
 
-  // lane i < KS looks key base + i up: the byte offset of its row (-1: not there), and its scales
-  auto look_up = [&](int base, long& off, float& ks, float& vs) {
-    off = -1;
-    ks = vs = 0.0f;
+  // Lane i looks key base + i of a block up: its page a block ahead, then the byte offset of its row and
+  // its place among the scales (-1: not there).
+  const int page_size = static_cast<int>(p.a.cache.page_size);
+  auto page_of = [&](int base) {
     const int key = base + lane;
-    if (lane < KS && key < k1) {
-      const int pg = p.page_shift >= 0 ? key >> p.page_shift : key / static_cast<int>(p.a.cache.page_size);
-      const int sl = key - pg * static_cast<int>(p.a.cache.page_size);
-      const int page = table[pg];
-      if (page >= 0 && page < p.a.cache.pages) {
-        off = (page * p.a.cache.page_stride + sl * p.a.cache.slot_stride) * ES;
-        if (Q8) {
-          const long so = page * p.a.cache.scale_page + sl * p.a.cache.scale_slot;
-          ks = __ldg(ksc + so);
-          vs = __ldg(vsc + so);
-        }
-      } else {
-        tj_report(p.status, TJ_STATUS_BOUNDS, OP_ATTENTION * 16 + SITE_PAGE);
+    if (lane >= KS || key >= k1) return INT_MIN;
+    return table[p.page_shift >= 0 ? key >> p.page_shift : key / page_size];
+  };
+  auto fetch = [&](int stage, int base, int page) {
+    long off = -1, soff = -1;
+    if (page >= 0 && page < p.a.cache.pages) {
+      const int key = base + lane, slot = p.page_shift >= 0 ? key & (page_size - 1) : key % page_size;
+      off = (page * p.a.cache.page_stride + slot * p.a.cache.slot_stride) * ES;
+      if (Q8) soff = page * p.a.cache.scale_page + slot * p.a.cache.scale_slot;
+    } else if (page != INT_MIN) {
+      tj_report(p.status, TJ_STATUS_BOUNDS, OP_ATTENTION * 16 + SITE_PAGE);
+    }
+    if (base < k1) {
+      constexpr int PIECES = R::ROW / 16, PER = 32 / PIECES;  // lanes of a row, rows of a warp's instruction
+      const uint32_t dst = my_ring + stage * R::BLOCK;
+      const int i = lane % PIECES;
+#pragma unroll
+      for (int j = 0; j < KS / PER; ++j) {
+        const int r = j * PER + lane / PIECES;
+        const long ro = __shfl_sync(0xffffffffu, off, r);
+        const long src = (ro < 0 ? 0 : ro) + i * 16;
+        copy16(dst + R::piece(r, i), kbase + src, ro >= 0);
+        copy16(dst + KS * R::ROW + R::piece(r, i), vbase + src, ro >= 0);
+      }
+      if (Q8) {
+        const uint32_t s = my_ring + STAGES * R::BLOCK + (stage * KS * 3 + lane) * 4;
+        copy4(s, ksc + (soff < 0 ? 0 : soff), soff >= 0);
+        copy4(s + KS * 4, vsc + (soff < 0 ? 0 : soff), soff >= 0);
       }
     }
+    asm volatile("cp.async.commit_group;" ::: "memory");
   };
 
-  long off;
-  float ks, vs;
-  int base = k0 + warp * KS;
-  if (base < k1) look_up(base, off, ks, vs);
-  for (; base < k1; base += 4 * KS) {
-    uint4 kf[NT][KC];
+  const int first = k0 + warp * KS;
+  int ahead = first;  // the block to be fetched next
+  int page = page_of(ahead);
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      const long ro = __shfl_sync(0xffffffffu, off, 8 * j + g);
-#pragma unroll
-      for (int c = 0; c < KC; ++c)
-        kf[j][c] = ro >= 0 ? tj_ld16_stream(kbase + ro + (c * 4 + t) * 16) : make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < STAGES - 1; ++i) {
+    const int now = page;
+    page = page_of(ahead + 4 * KS);
+    fetch(i, ahead, now);
+    ahead += 4 * KS;
+  }
+  int stage = 0;
+  for (int base = first; base < k1; base += 4 * KS) {
+    {
+      const int now = page;
+      page = page_of(ahead + 4 * KS);
+      fetch(stage == 0 ? STAGES - 1 : stage - 1, ahead, now);
+      ahead += 4 * KS;
     }
-    uint32_t vf[KS / 4][VW];  // [16-key step][key 2t, 2t + 1, 2t + 8, 2t + 9]
-#pragma unroll
-    for (int j = 0; j < KS / 4; ++j) {
-      const long ro = __shfl_sync(0xffffffffu, off, (j >> 2) * 16 + 2 * t + (j & 1) + ((j & 2) ? 8 : 0));
-      if (VB == 8) {
-        const uint2 x = ro >= 0 ? __ldg(reinterpret_cast<const uint2*>(vbase + ro + g * 8)) : make_uint2(0, 0);
-        vf[j][0] = x.x;
-        vf[j][1] = x.y;
-      } else {
-#pragma unroll
-        for (int c = 0; c < VC; ++c) {
-          const uint4 x = ro >= 0 ? tj_ld16_stream(vbase + ro + (c * 8 + g) * 16) : make_uint4(0, 0, 0, 0);
-          vf[j][(4 * c) % VW] = x.x;
-          vf[j][(4 * c + 1) % VW] = x.y;
-          vf[j][(4 * c + 2) % VW] = x.z;
-          vf[j][(4 * c + 3) % VW] = x.w;
-        }
+    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    __syncwarp();
+    const uint32_t kblock = my_ring + stage * R::BLOCK, vblock = kblock + KS * R::ROW;
+    float* const scale = reinterpret_cast<float*>(ring + warp * R::WARP + STAGES * R::BLOCK) + stage * KS * 3;
+    if constexpr (Q8) {
+      scale[lane] *= p.scale_log2;
+      if constexpr (!R::MUL_V) {
+        const float lv = fmaxf(__log2f(scale[KS + lane]), MIN_LOG2_SCALE);
+        scale[KS + lane] = lv;
+        scale[2 * KS + lane] = exp2_fast(-lv);
       }
+      __syncwarp();
     }
-    const float my_ks = ks, my_vs = vs;
-    if (base + 4 * KS < k1) look_up(base + 4 * KS, off, ks, vs);
+    if (++stage == STAGES) stage = 0;
 
     float sc[NT][4];
 #pragma unroll
@@ -166,41 +231,39 @@ __global__ void __launch_bounds__(128, D == 64 ? 4 : 3) attention_rows(const __g
       sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
 #pragma unroll
       for (int c = 0; c < KC; ++c) {
+        const uint4 kf = lds16(kblock + R::piece(8 * j + g, c * 4 + t));
         if constexpr (Q8) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t x = word(kf[j][c], e);
+            const uint32_t x = word(kf, e);
             const uint32_t b0 = Codes<T, CD>::make(__byte_perm(x, 0, CD == TJ_I8 ? 0x4140 : 0x1404));
             const uint32_t b1 = Codes<T, CD>::make(__byte_perm(x, 0, CD == TJ_I8 ? 0x4342 : 0x3424));
             mma16816<T>(sc[j], qa[c * 4 + e], b0, b1);
           }
         } else {
-          mma16816<T>(sc[j], qa[c * 2], kf[j][c].x, kf[j][c].y);
-          mma16816<T>(sc[j], qa[c * 2 + 1], kf[j][c].z, kf[j][c].w);
+          mma16816<T>(sc[j], qa[c * 2], kf.x, kf.y);
+          mma16816<T>(sc[j], qa[c * 2 + 1], kf.z, kf.w);
         }
       }
     }
-    // t = scaled score (+ log2 vs); masked keys -inf
-    float inv[NT][2];
-    const float lane_lv = Q8 ? fmaxf(__log2f(my_vs), MIN_LOG2_SCALE) : 0.0f;
-    const float lane_inv = Q8 ? exp2_fast(-lane_lv) : 1.0f, lane_k = my_ks * p.scale_log2;
+    // t = scaled score (f16 over an 8-bit cache: + log2 vs); masked keys -inf
+    const bool masked = base < mlo || base + KS > mhi;  // the same for the warp
     float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
+      float2 kfac = make_float2(p.scale_log2, p.scale_log2), lv = make_float2(0.0f, 0.0f);
+      if constexpr (Q8) {
+        kfac = *reinterpret_cast<const float2*>(scale + 8 * j + 2 * t);
+        if constexpr (!R::MUL_V) lv = *reinterpret_cast<const float2*>(scale + KS + 8 * j + 2 * t);
+      }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int kk = 8 * j + 2 * t + e, key = base + kk;
-        float kfac = p.scale_log2, lv = 0.0f;
-        if (Q8) {
-          kfac = __shfl_sync(0xffffffffu, lane_k, kk);
-          lv = __shfl_sync(0xffffffffu, lane_lv, kk);
-          inv[j][e] = __shfl_sync(0xffffffffu, lane_inv, kk);
-        }
+        const int key = base + 8 * j + 2 * t + e;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float& x = sc[j][2 * i + e];
-          x = Q8 ? fmaf(x, kfac, lv) : x * kfac;
-          if (key < rlo[i] || key >= rhi[i] || key >= k1) x = -INFINITY;
+          x = Q8 && !R::MUL_V ? fmaf(x, e ? kfac.y : kfac.x, e ? lv.y : lv.x) : x * (e ? kfac.y : kfac.x);
+          if (masked && (key < rlo[i] || key >= rhi[i])) x = -INFINITY;
           mx[i] = fmaxf(mx[i], x);
         }
       }
@@ -230,17 +293,41 @@ __global__ void __launch_bounds__(128, D == 64 ? 4 : 3) attention_rows(const __g
       }
     }
 #pragma unroll
-    for (int j = 0; j < NT; ++j)
+    for (int j = 0; j < NT; ++j) {
+      float2 vs = make_float2(1.0f, 1.0f);  // what turns P into P vs, or P vs into P
+      if constexpr (Q8) vs = *reinterpret_cast<const float2*>(scale + (R::MUL_V ? 1 : 2) * KS + 8 * j + 2 * t);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        sc[j][e] = exp2_fast(sc[j][e] - base_m[e >> 1]);
-        l[e >> 1] += Q8 ? sc[j][e] * inv[j][e & 1] : sc[j][e];
+        const float prob = exp2_fast(sc[j][e] - base_m[e >> 1]), scaled = Q8 ? prob * (e & 1 ? vs.y : vs.x) : prob;
+        l[e >> 1] += R::MUL_V ? prob : scaled;
+        sc[j][e] = R::MUL_V ? scaled : prob;
       }
+    }
 #pragma unroll
     for (int k16 = 0; k16 < KS / 16; ++k16) {
       const uint32_t pa[4] = {pack2<T>(sc[2 * k16][0], sc[2 * k16][1]), pack2<T>(sc[2 * k16][2], sc[2 * k16][3]),
                               pack2<T>(sc[2 * k16 + 1][0], sc[2 * k16 + 1][1]), pack2<T>(sc[2 * k16 + 1][2], sc[2 * k16 + 1][3])};
-      const uint32_t(&va)[VW] = vf[4 * k16], (&vb)[VW] = vf[4 * k16 + 1], (&vc)[VW] = vf[4 * k16 + 2], (&vd)[VW] = vf[4 * k16 + 3];
+      uint32_t va[VW], vb[VW], vc[VW], vd[VW];  // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the step
+      auto value = [&](uint32_t (&v)[VW], int row) {
+        if constexpr (VB == 8) {
+          const uint2 x = lds8(vblock + R::piece(row, g >> 1) + (g & 1) * 8);
+          v[0] = x.x;
+          v[1] = x.y;
+        } else {
+#pragma unroll
+          for (int c = 0; c < VC; ++c) {
+            const uint4 x = lds16(vblock + R::piece(row, c * 8 + g));
+            v[(4 * c) % VW] = x.x;
+            v[(4 * c + 1) % VW] = x.y;
+            v[(4 * c + 2) % VW] = x.z;
+            v[(4 * c + 3) % VW] = x.w;
+          }
+        }
+      };
+      value(va, k16 * 16 + 2 * t);
+      value(vb, k16 * 16 + 2 * t + 1);
+      value(vc, k16 * 16 + 2 * t + 8);
+      value(vd, k16 * 16 + 2 * t + 9);
 #pragma unroll
       for (int j = 0; j < OT; ++j) {
         uint32_t b0, b1;
@@ -258,9 +345,11 @@ __global__ void __launch_bounds__(128, D == 64 ? 4 : 3) attention_rows(const __g
         mma16816<T>(o[j], pa, b0, b1);
       }
     }
+    __syncwarp();  // the block's place may be filled again
   }
 
   // join the four warps
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
