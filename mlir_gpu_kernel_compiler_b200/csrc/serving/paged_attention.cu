@@ -41,12 +41,13 @@ Plan plan(const tj_paged_attention& a, const Device& dev) {
   }
   p.rows = 16;
   const long tiles = a.q_starts ? a.tokens * group / 16 + a.batch : a.batch * ((group + 15) / 16);
-#ifndef TJS_WAVES
-#define TJS_WAVES 3
-#define TJS_MINC 256
-#endif
-  p.target = dev.sms * 2 * TJS_WAVES;
-  p.min_chunk = TJS_MINC;
+  // Two CTAs an SM.  Few row tiles are cut so that all pieces run at once (pieces: at most target + tiles;
+  // three sequences of 100000 keys and 4 heads: 65 us with as many pieces as CTAs fit, 84 us with three
+  // times as many, whose starts and joins cost more than they even out).  Many uneven ones in three waves
+  // (64 sequences, 8 heads: 242 us, with one wave 266).
+  const long slots = 2L * dev.sms, items = a.cache.heads * tiles;
+  p.target = static_cast<int>(items <= slots / 2 ? slots - items : 3 * slots);
+  p.min_chunk = 256;
   p.grid = a.cache.heads * (tiles + 1) + p.target;
   p.slots = p.grid;
   return p;

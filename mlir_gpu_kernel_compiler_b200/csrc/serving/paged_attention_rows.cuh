@@ -14,6 +14,11 @@
 // two keys' elements are paired by a byte permutation.  The pieces of a row are permuted by its number
 // so that both ways of reading are free of bank conflicts.
 //
+// An 8-bit cache's codes become f16, bf16 queries too (a row times the power of two that brings its
+// largest element near 2^10: exact but for elements 2^-24 of that): the byte permutations and masks run
+// at half rate and were the bound, and bf16 needs three for a pair of codes where f16 needs 1.5 (keys) and
+// 2 (values).
+//
 // A warp takes every fourth block of KS keys of its CTA's chunk with a running maximum and sum of its
 // own; the four warps' results are joined at the end, and the chunks of a row tile by the CTA that
 // finishes last (in the order of the chunks, so results do not depend on which that is).
@@ -58,16 +63,16 @@ TJ_DEV uint2 lds8(uint32_t a) {
 }
 
 template <class T, int CD, int D> struct Rows {
+  using C = typename std::conditional<CD == TJ_I8 || CD == TJ_E4M3, __half, T>::type;  // what is multiplied
   static constexpr bool Q8 = CD == TJ_I8 || CD == TJ_E4M3;
   static constexpr int ES = Q8 ? 1 : 2;
   static constexpr int ROW = D * ES;                            // bytes of a key
   static constexpr int KS = !Q8 && D == 128 ? 16 : 32;          // keys of a warp's block
   static constexpr int BLOCK = 2 * KS * ROW;                    // bytes of its keys and values
   static constexpr int STAGES = 24576 / BLOCK;
-  static constexpr int SCALES = Q8 ? STAGES * KS * 3 * 4 : 0;   // ks; vs or log2 vs; 1 / vs
+  static constexpr int SCALES = Q8 ? STAGES * KS * 3 * 4 : 0;   // ks, log2 vs, 1 / vs
   static constexpr int WARP = STAGES * BLOCK + SCALES;
   static constexpr int SMEM = 4 * WARP;
-  static constexpr bool MUL_V = Q8 && P_SHIFT<T> == 0.0f;       // bf16: P times vs; f16: vs in the exponent
   // the 16-byte piece of a row in a block; rows of 4 pieces share a line of 8
   static TJ_DEV uint32_t piece(int row, int i) {
     constexpr int PIECES = ROW / 16;
@@ -79,6 +84,7 @@ template <class T, int CD, int D> struct Rows {
 template <class T, int CD, int D>
 __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__ AttnParams p) {
   using R = Rows<T, CD, D>;
+  using C = typename R::C;
   constexpr bool Q8 = R::Q8;
   constexpr int KS = R::KS, ES = R::ES, STAGES = R::STAGES;
   constexpr int NT = KS / 8;             // score tiles of 8 keys
@@ -112,40 +118,6 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
   if (threadIdx.x == 0 && w.c == 0 && h == 0 &&
       (p.a.kv_lens[w.b] < 0 || p.a.kv_lens[w.b] > p.a.table_width * p.a.cache.page_size))
     tj_report(p.status, TJ_STATUS_BOUNDS, OP_ATTENTION * 16 + SITE_LENGTH);
-
-  // this thread's two rows, g and g + 8: their queries and the keys that they see
-  uint32_t qa[KC * STEPS][4];
-  int rlo[2], rhi[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = g + 8 * i, tok = (r0 + r) / p.group, hd = h * p.group + (r0 + r) - tok * p.group;
-    const bool on = r < rows;
-    rlo[i] = 0;  // a row that is not there sees all, and is not stored
-    rhi[i] = INT_MAX;
-    if (on) row_range(p, s, tok, rlo[i], rhi[i]);
-    const T* src = static_cast<const T*>(p.a.q) + (s.start + tok) * p.a.q_token + hd * p.a.q_head;
-#pragma unroll
-    for (int c = 0; c < KC; ++c) {
-      // the elements of piece c: 8 (16) of them from c * 32 + t * 8 (c * 64 + t * 16)
-      const T* at = src + (c * 4 + t) * (16 / ES);
-#pragma unroll
-      for (int v = 0; v < STEPS / 2; ++v) {
-        const uint4 x = on ? tj_ld16(at + 8 * v) : make_uint4(0, 0, 0, 0);
-        qa[c * STEPS + 2 * v][i] = x.x;
-        qa[c * STEPS + 2 * v][i + 2] = x.y;
-        qa[c * STEPS + 2 * v + 1][i] = x.z;
-        qa[c * STEPS + 2 * v + 1][i + 2] = x.w;
-      }
-    }
-  }
-
-  // keys that all of the tile's rows see need no mask
-  const int mlo = __reduce_max_sync(0xffffffffu, max(rlo[0], rlo[1])), mhi = __reduce_min_sync(0xffffffffu, min(rhi[0], rhi[1]));
-
-  float o[OT][4];
-#pragma unroll
-  for (int i = 0; i < OT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
   const int* table = p.a.page_table + w.b * p.a.table_row;
   const char* kbase = static_cast<const char*>(p.a.cache.k) + h * p.a.cache.head_stride * ES;
@@ -202,6 +174,67 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
     fetch(i, ahead, now);
     ahead += 4 * KS;
   }
+  // this thread's two rows, g and g + 8: their queries and the keys that they see
+  uint32_t qa[KC * STEPS][4];
+  int rlo[2], rhi[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = g + 8 * i, tok = (r0 + r) / p.group, hd = h * p.group + (r0 + r) - tok * p.group;
+    const bool on = r < rows;
+    rlo[i] = 0;  // a row that is not there sees all, and is not stored
+    rhi[i] = INT_MAX;
+    if (on) row_range(p, s, tok, rlo[i], rhi[i]);
+    const T* src = static_cast<const T*>(p.a.q) + (s.start + tok) * p.a.q_token + hd * p.a.q_head;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+      // the elements of piece c: 8 (16) of them from c * 32 + t * 8 (c * 64 + t * 16)
+      const T* at = src + (c * 4 + t) * (16 / ES);
+#pragma unroll
+      for (int v = 0; v < STEPS / 2; ++v) {
+        const uint4 x = on ? tj_ld16(at + 8 * v) : make_uint4(0, 0, 0, 0);
+        qa[c * STEPS + 2 * v][i] = x.x;
+        qa[c * STEPS + 2 * v][i + 2] = x.y;
+        qa[c * STEPS + 2 * v + 1][i] = x.z;
+        qa[c * STEPS + 2 * v + 1][i + 2] = x.w;
+      }
+    }
+  }
+
+  float unscale[2] = {1.0f, 1.0f};  // what the rows' queries were divided by
+  if constexpr (!std::is_same<T, C>::value) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      uint32_t top = 0;
+#pragma unroll
+      for (int c = 0; c < KC * STEPS; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) top = max(top, max((qa[c][i + e] & 0x7fffu) << 16, qa[c][i + e] & 0x7fff0000u));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^(10 - exponent); none for zeros, infinities and NaN
+      const int exponent = static_cast<int>(top >> 23) - 127;
+      const bool fine = top >= 0x00800000u && top < 0x7f800000u;
+      const float up = fine ? __int_as_float((127 + min(10 - exponent, 127)) << 23) : 1.0f;
+      unscale[i] = fine ? __int_as_float((127 - min(10 - exponent, 126)) << 23) : 1.0f;
+      if (fine && 10 - exponent > 126) unscale[i] = 1.0f / up;
+#pragma unroll
+      for (int c = 0; c < KC * STEPS; ++c)
+#pragma unroll
+        for (int e = 0; e < 4; e += 2) {
+          uint32_t& w = qa[c][i + e];
+          w = tj_pack_f16x2(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up);
+        }
+    }
+  }
+
+  // keys that all of the tile's rows see need no mask
+  const int mlo = __reduce_max_sync(0xffffffffu, max(rlo[0], rlo[1])), mhi = __reduce_min_sync(0xffffffffu, min(rhi[0], rhi[1]));
+
+  float o[OT][4];
+#pragma unroll
+  for (int i = 0; i < OT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
   int stage = 0;
   for (int base = first; base < k1; base += 4 * KS) {
     {
@@ -216,11 +249,9 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
     float* const scale = reinterpret_cast<float*>(ring + warp * R::WARP + STAGES * R::BLOCK) + stage * KS * 3;
     if constexpr (Q8) {
       scale[lane] *= p.scale_log2;
-      if constexpr (!R::MUL_V) {
-        const float lv = fmaxf(__log2f(scale[KS + lane]), MIN_LOG2_SCALE);
-        scale[KS + lane] = lv;
-        scale[2 * KS + lane] = exp2_fast(-lv);
-      }
+      const float lv = fmaxf(__log2f(scale[KS + lane]), MIN_LOG2_SCALE);
+      scale[KS + lane] = lv;
+      scale[2 * KS + lane] = exp2_fast(-lv);
       __syncwarp();
     }
     if (++stage == STAGES) stage = 0;
@@ -235,18 +266,17 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
         if constexpr (Q8) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t x = word(kf, e);
-            const uint32_t b0 = Codes<T, CD>::make(__byte_perm(x, 0, CD == TJ_I8 ? 0x4140 : 0x1404));
-            const uint32_t b1 = Codes<T, CD>::make(__byte_perm(x, 0, CD == TJ_I8 ? 0x4342 : 0x3424));
-            mma16816<T>(sc[j], qa[c * 4 + e], b0, b1);
+            uint32_t b0, b1;
+            codes4<C, CD>(word(kf, e), b0, b1);
+            mma16816<C>(sc[j], qa[c * 4 + e], b0, b1);
           }
         } else {
-          mma16816<T>(sc[j], qa[c * 2], kf.x, kf.y);
-          mma16816<T>(sc[j], qa[c * 2 + 1], kf.z, kf.w);
+          mma16816<C>(sc[j], qa[c * 2], kf.x, kf.y);
+          mma16816<C>(sc[j], qa[c * 2 + 1], kf.z, kf.w);
         }
       }
     }
-    // t = scaled score (f16 over an 8-bit cache: + log2 vs); masked keys -inf
+    // t = scaled score (8-bit cache: + log2 vs); masked keys -inf
     const bool masked = base < mlo || base + KS > mhi;  // the same for the warp
     float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
@@ -254,7 +284,7 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
       float2 kfac = make_float2(p.scale_log2, p.scale_log2), lv = make_float2(0.0f, 0.0f);
       if constexpr (Q8) {
         kfac = *reinterpret_cast<const float2*>(scale + 8 * j + 2 * t);
-        if constexpr (!R::MUL_V) lv = *reinterpret_cast<const float2*>(scale + KS + 8 * j + 2 * t);
+        lv = *reinterpret_cast<const float2*>(scale + KS + 8 * j + 2 * t);
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
@@ -262,7 +292,8 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
           float& x = sc[j][2 * i + e];
-          x = Q8 && !R::MUL_V ? fmaf(x, e ? kfac.y : kfac.x, e ? lv.y : lv.x) : x * (e ? kfac.y : kfac.x);
+          if (!std::is_same<T, C>::value) x *= unscale[i];
+          x = Q8 ? fmaf(x, e ? kfac.y : kfac.x, e ? lv.y : lv.x) : x * (e ? kfac.y : kfac.x);
           if (masked && (key < rlo[i] || key >= rhi[i])) x = -INFINITY;
           mx[i] = fmaxf(mx[i], x);
         }
@@ -278,7 +309,7 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
       moved |= next > m[i];
       const float from = next == -INFINITY ? 0.0f : next;
       alpha[i] = exp2_fast(m[i] - from);
-      base_m[i] = from - P_SHIFT<T>;
+      base_m[i] = from - P_SHIFT<C>;
       m[i] = next;
     }
     if (__any_sync(0xffffffffu, moved)) {
@@ -294,19 +325,18 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
     }
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      float2 vs = make_float2(1.0f, 1.0f);  // what turns P into P vs, or P vs into P
-      if constexpr (Q8) vs = *reinterpret_cast<const float2*>(scale + (R::MUL_V ? 1 : 2) * KS + 8 * j + 2 * t);
+      float2 inv = make_float2(1.0f, 1.0f);
+      if constexpr (Q8) inv = *reinterpret_cast<const float2*>(scale + 2 * KS + 8 * j + 2 * t);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const float prob = exp2_fast(sc[j][e] - base_m[e >> 1]), scaled = Q8 ? prob * (e & 1 ? vs.y : vs.x) : prob;
-        l[e >> 1] += R::MUL_V ? prob : scaled;
-        sc[j][e] = R::MUL_V ? scaled : prob;
+        sc[j][e] = exp2_fast(sc[j][e] - base_m[e >> 1]);
+        l[e >> 1] += Q8 ? sc[j][e] * (e & 1 ? inv.y : inv.x) : sc[j][e];
       }
     }
 #pragma unroll
     for (int k16 = 0; k16 < KS / 16; ++k16) {
-      const uint32_t pa[4] = {pack2<T>(sc[2 * k16][0], sc[2 * k16][1]), pack2<T>(sc[2 * k16][2], sc[2 * k16][3]),
-                              pack2<T>(sc[2 * k16 + 1][0], sc[2 * k16 + 1][1]), pack2<T>(sc[2 * k16 + 1][2], sc[2 * k16 + 1][3])};
+      const uint32_t pa[4] = {pack2<C>(sc[2 * k16][0], sc[2 * k16][1]), pack2<C>(sc[2 * k16][2], sc[2 * k16][3]),
+                              pack2<C>(sc[2 * k16 + 1][0], sc[2 * k16 + 1][1]), pack2<C>(sc[2 * k16 + 1][2], sc[2 * k16 + 1][3])};
       uint32_t va[VW], vb[VW], vc[VW], vd[VW];  // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the step
       auto value = [&](uint32_t (&v)[VW], int row) {
         if constexpr (VB == 8) {
@@ -335,14 +365,14 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
           // byte j % 4 of both keys' words, into both bytes of a half
           const int n = j & 3;
           const uint32_t sel = n | (n << 4) | ((n + 4) << 8) | ((n + 4) << 12);
-          b0 = Codes<T, CD>::make(__byte_perm(va[j >> 2], vb[j >> 2], sel));
-          b1 = Codes<T, CD>::make(__byte_perm(vc[j >> 2], vd[j >> 2], sel));
+          b0 = Codes<C, CD>::make(__byte_perm(va[j >> 2], vb[j >> 2], sel));
+          b1 = Codes<C, CD>::make(__byte_perm(vc[j >> 2], vd[j >> 2], sel));
         } else {
           const uint32_t sel = (j & 1) ? 0x7632 : 0x5410;
           b0 = __byte_perm(va[j >> 1], vb[j >> 1], sel);
           b1 = __byte_perm(vc[j >> 1], vd[j >> 1], sel);
         }
-        mma16816<T>(o[j], pa, b0, b1);
+        mma16816<C>(o[j], pa, b0, b1);
       }
     }
     __syncwarp();  // the block's place may be filled again
@@ -406,26 +436,61 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
     __syncthreads();
     if (!s_last) return;
     __threadfence();
-    if (r >= rows) return;
+    // the chunks' weights and the rows' sums, eight threads a row
+    float* const weight = reinterpret_cast<float*>(ring);  // [cuts][16], as far as it goes
+    float4* const sums = reinterpret_cast<float4*>(ring + R::SMEM / 2);
+    constexpr int MOST = R::SMEM / 2 / 64;
+    const int t8 = threadIdx.x & 7;
     best = -INFINITY;
-    for (int k = 0; k < cuts; ++k) best = fmaxf(best, __ldcg(p.part_ml + static_cast<long>(first + k * heads) * 16 + r).x);
+    if (r < rows)
+#pragma unroll 4
+      for (int k = t8; k < cuts; k += 8) best = fmaxf(best, __ldcg(p.part_ml + static_cast<long>(first + k * heads) * 16 + r).x);
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
     sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < W; ++i) acc[i] = 0.0f;
-    for (int k = 0; k < cuts; ++k) {
-      const long at = static_cast<long>(first + k * heads) * 16 + r;
-      const float2 ml = __ldcg(p.part_ml + at);
-      const float f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - best);
-      sum += ml.y * f;
-#pragma unroll
-      for (int i = 0; i < W; i += 4) {
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + at * D + c0 + i));
-        acc[i] += v.x * f;
-        acc[i + 1] += v.y * f;
-        acc[i + 2] += v.z * f;
-        acc[i + 3] += v.w * f;
+    // positions: 16 bytes of a row; where there are fewer than threads, they share the chunks
+    const int positions = rows * (D / 4);
+    int shares = 1;
+    while (shares * 2 * positions <= 128) shares *= 2;
+    for (int k0 = 0; k0 < cuts; k0 += MOST) {
+      const int n = min(MOST, cuts - k0);
+      __syncthreads();
+      if (r < rows)
+#pragma unroll 4
+        for (int k = t8; k < n; k += 8) {
+          const float2 ml = __ldcg(p.part_ml + static_cast<long>(first + (k0 + k) * heads) * 16 + r);
+          const float f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - best);
+          weight[k * 16 + r] = f;
+          sum += ml.y * f;
+        }
+      __syncthreads();
+      for (int at = threadIdx.x; at < positions * shares; at += 128) {
+        const int share = at / positions, pos = at - share * positions, row = pos / (D / 4), c4 = pos - row * (D / 4);
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 8
+        for (int k = share; k < n; k += shares) {
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + (static_cast<long>(first + (k0 + k) * heads) * 16 + row) * D) + c4);
+          const float f = weight[k * 16 + row];
+          v = make_float4(v.x + x.x * f, v.y + x.y * f, v.z + x.z * f, v.w + x.w * f);
+        }
+        sums[at] = v;
       }
+      __syncthreads();
+      if (r < rows)
+        for (int share = 0; share < shares; ++share)
+#pragma unroll
+          for (int i = 0; i < W; i += 4) {
+            const float4 v = sums[share * positions + r * (D / 4) + (c0 + i) / 4];
+            acc[i] += v.x;
+            acc[i + 1] += v.y;
+            acc[i + 2] += v.z;
+            acc[i + 3] += v.w;
+          }
     }
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   }
   if (r >= rows) return;
   const int tok = (r0 + r) / p.group, hd = h * p.group + (r0 + r) - tok * p.group;
@@ -440,7 +505,7 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
     tj_store_vec(dst + i, y);
   }
   if (p.a.lse && (threadIdx.x & 7) == 0)
-    p.a.lse[(s.start + tok) * p.a.q_heads + hd] = none ? -INFINITY : (best - P_SHIFT<T> + log2f(sum)) * 0.69314718055994531f;
+    p.a.lse[(s.start + tok) * p.a.q_heads + hd] = none ? -INFINITY : (best - P_SHIFT<C> + log2f(sum)) * 0.69314718055994531f;
 }
 
 }  // namespace tjs

@@ -188,8 +188,7 @@ TJ_DEV void store_rows(uint32_t dst, const uint4 (&raw)[N], int row0) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t x = e == 0 ? raw[i].x : e == 1 ? raw[i].y : e == 2 ? raw[i].z : raw[i].w;
-      h[e >> 1][(e & 1) * 2] = Codes<T, CD>::make(__byte_perm(x, 0, CD == TJ_I8 ? 0x4140 : 0x1404));
-      h[e >> 1][(e & 1) * 2 + 1] = Codes<T, CD>::make(__byte_perm(x, 0, CD == TJ_I8 ? 0x4342 : 0x3424));
+      codes4<T, CD>(x, h[e >> 1][(e & 1) * 2], h[e >> 1][(e & 1) * 2 + 1]);
     }
     // at head dim 128 a row's lanes reach both panels, whose banks are the same: the upper half
     // stores its odd piece first
