@@ -6,6 +6,7 @@ namespace tjs {
 
 struct Plan {
   bool tiles;      // the tensor-core kernel of many rows
+  bool wide;       // the kernel of few rows with one CTA an SM
   long grid;
   long slots;      // partial results kept at once
   int rows;        // of a tile
@@ -37,16 +38,17 @@ Plan plan(const tj_paged_attention& a, const Device& dev) {
     p.grid = dev.sms;
     p.slots = 2 * p.grid;  // a CTA's first and last segment
     p.target = p.min_chunk = 0;
+    p.wide = false;
     return p;
   }
   p.rows = 16;
   const long tiles = a.q_starts ? a.tokens * group / 16 + a.batch : a.batch * ((group + 15) / 16);
-  // Two CTAs an SM.  Few row tiles are cut so that all pieces run at once (pieces: at most target + tiles;
-  // three sequences of 100000 keys and 4 heads: 65 us with as many pieces as CTAs fit, 84 us with three
-  // times as many, whose starts and joins cost more than they even out).  Many uneven ones in three waves
-  // (64 sequences, 8 heads: 242 us, with one wave 266).
-  const long slots = 2L * dev.sms, items = a.cache.heads * tiles;
-  p.target = static_cast<int>(items <= slots / 2 ? slots - items : 3 * slots);
+  // Few row tiles are cut so that all pieces run at once, one CTA an SM (pieces: at most target + tiles).
+  // Many uneven ones are cut for three waves of smaller CTAs, which even out what one wave does not.
+  const bool q8 = a.cache.dtype == TJ_I8 || a.cache.dtype == TJ_E4M3;
+  const long items = a.cache.heads * tiles;
+  p.wide = items <= dev.sms / 2;
+  p.target = static_cast<int>(p.wide ? dev.sms - items : 3L * dev.sms * (q8 ? 3 : 2));
   p.min_chunk = 256;
   p.grid = a.cache.heads * (tiles + 1) + p.target;
   p.slots = p.grid;
@@ -60,17 +62,22 @@ template <class K> cudaError_t allow(K kernel, int smem, bool (&ready)[MAX_DEVIC
   ready[dev.index] = e == cudaSuccess;
   return e;
 }
+template <class T, int CD, int D, bool WIDE> cudaError_t launch_few(const AttnParams& p, unsigned grid, const Device& dev, cudaStream_t st) {
+  using R = Rows<T, CD, D, WIDE>;
+  static bool ready[MAX_DEVICES];
+  if (const cudaError_t e = allow(attention_rows<T, CD, D, WIDE>, R::SMEM, ready, dev)) return e;
+  attention_rows<T, CD, D, WIDE><<<grid, R::THREADS, R::SMEM, st>>>(p);
+  return cudaSuccess;
+}
 template <class T, int CD, int D> cudaError_t launch_dim(const AttnParams& p, const Plan& plan, const Device& dev, cudaStream_t st) {
   const unsigned grid = static_cast<unsigned>(plan.grid);
-  static bool rows_ready[MAX_DEVICES], tiles_ready[MAX_DEVICES];
+  static bool tiles_ready[MAX_DEVICES];
   if (plan.tiles) {
     constexpr int smem = Tiles<T, CD, D>::SMEM;
     if (const cudaError_t e = allow(attention_tiles<T, CD, D>, smem, tiles_ready, dev)) return e;
     attention_tiles<T, CD, D><<<grid, 512, smem, st>>>(p);
   } else {
-    constexpr int smem = Rows<T, CD, D>::SMEM;
-    if (const cudaError_t e = allow(attention_rows<T, CD, D>, smem, rows_ready, dev)) return e;
-    attention_rows<T, CD, D><<<grid, 128, smem, st>>>(p);
+    return plan.wide ? launch_few<T, CD, D, true>(p, grid, dev, st) : launch_few<T, CD, D, false>(p, grid, dev, st);
   }
   return cudaSuccess;
 }

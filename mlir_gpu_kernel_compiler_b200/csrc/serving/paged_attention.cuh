@@ -88,10 +88,15 @@ TJ_DEV Piece find_piece(const AttnParams& p, int unit, int per_tile, int step) {
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
-  const long want = (work * p.a.cache.heads + p.target - 1) / p.target;
+  // (in f32, rounded up generously: pieces may only become fewer; 64-bit divisions take hundreds of clocks)
+  const long want = static_cast<long>(static_cast<float>(work * p.a.cache.heads) / static_cast<float>(p.target) * 1.000001f) + 1;
   Piece g;
   g.chunk = static_cast<int>((max(want, static_cast<long>(p.min_chunk)) + step - 1) / step * step);
-  auto count = [&](const Seq& s) { return tiles(s) * max(1, (span(s) + g.chunk - 1) / g.chunk); };
+  auto cuts_of = [&](const Seq& s) {
+    const int n = span(s) + g.chunk - 1, q = static_cast<int>(__fdividef(static_cast<float>(n), static_cast<float>(g.chunk)));
+    return max(1, q + (n - q * g.chunk >= g.chunk) - (n - q * g.chunk < 0));  // the estimate is off by one at the most
+  };
+  auto count = [&](const Seq& s) { return tiles(s) * cuts_of(s); };
   int mine = 0;
   for (int b = b0; b < b1; ++b) mine += count(sequence(p, b));
   int before = mine;
@@ -110,9 +115,8 @@ TJ_DEV Piece find_piece(const AttnParams& p, int unit, int per_tile, int step) {
     int left = unit - before;
     for (int b = b0; b < b1; ++b) {
       const Seq s = sequence(p, b);
-      const int n = count(s);
+      const int cuts = cuts_of(s), n = tiles(s) * cuts;
       if (left < n) {
-        const int cuts = max(1, (span(s) + g.chunk - 1) / g.chunk);
         fb = b;
         ft = left / cuts;
         fc = left - ft * cuts;

@@ -2,9 +2,9 @@
 //
 // What bounds it: the cache is read once and a key meets at most 16 rows, 2 x 16 products for each
 // of its bytes at the most, far below the tensor cores' rate; so it is HBM, and the kernel has to keep
-// enough reads in flight.  Each warp has a ring of its own in shared memory (24 KB, two CTAs of four
-// warps an SM: 192 KB) that asynchronous copies fill two or more blocks ahead, so the main loop has no
-// barrier.  (With the loads straight into registers, where a block's are in flight only until it is
+// enough reads in flight.  Each warp has a ring of its own in shared memory (8 warps of 24 KB an SM, or
+// 12 of 16 KB for 8-bit caches, whose codes take more instructions) that asynchronous copies fill one or
+// more blocks ahead, so the main loop has no barrier.  (With the loads straight into registers, where a block's are in flight only until it is
 // used, 64 single tokens over 8192 keys took 387 us, 3700 GB/s.)
 //
 // The order of the head dimension inside a product is free as long as both operands agree, so 16
@@ -19,8 +19,8 @@
 // at half rate and were the bound, and bf16 needs three for a pair of codes where f16 needs 1.5 (keys) and
 // 2 (values).
 //
-// A warp takes every fourth block of KS keys of its CTA's chunk with a running maximum and sum of its
-// own; the four warps' results are joined at the end, and the chunks of a row tile by the CTA that
+// A CTA's warps take blocks of KS keys of its chunk in turn, with a running maximum and sum each; their
+// results are joined at the end, and the chunks of a row tile by the CTA that
 // finishes last (in the order of the chunks, so results do not depend on which that is).
 #pragma once
 #include <limits.h>
@@ -62,17 +62,19 @@ TJ_DEV uint2 lds8(uint32_t a) {
   return v;
 }
 
-template <class T, int CD, int D> struct Rows {
+template <class T, int CD, int D, bool WIDE> struct Rows {
   using C = typename std::conditional<CD == TJ_I8 || CD == TJ_E4M3, __half, T>::type;  // what is multiplied
   static constexpr bool Q8 = CD == TJ_I8 || CD == TJ_E4M3;
   static constexpr int ES = Q8 ? 1 : 2;
   static constexpr int ROW = D * ES;                            // bytes of a key
   static constexpr int KS = !Q8 && D == 128 ? 16 : 32;          // keys of a warp's block
   static constexpr int BLOCK = 2 * KS * ROW;                    // bytes of its keys and values
-  static constexpr int STAGES = 24576 / BLOCK;
+  // WIDE: an SM's warps are one CTA, for work in few pieces, which is then joined from fewer parts
+  static constexpr int WARPS = WIDE ? (Q8 ? 12 : 8) : 4, CTAS = (Q8 ? 12 : 8) / WARPS, THREADS = 32 * WARPS;
+  static constexpr int STAGES = (Q8 ? 16384 : 24576) / BLOCK;
   static constexpr int SCALES = Q8 ? STAGES * KS * 3 * 4 : 0;   // ks, log2 vs, 1 / vs
   static constexpr int WARP = STAGES * BLOCK + SCALES;
-  static constexpr int SMEM = 4 * WARP;
+  static constexpr int SMEM = WARPS * WARP;
   // the 16-byte piece of a row in a block; rows of 4 pieces share a line of 8
   static TJ_DEV uint32_t piece(int row, int i) {
     constexpr int PIECES = ROW / 16;
@@ -81,12 +83,12 @@ template <class T, int CD, int D> struct Rows {
   }
 };
 
-template <class T, int CD, int D>
-__global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__ AttnParams p) {
-  using R = Rows<T, CD, D>;
+template <class T, int CD, int D, bool WIDE>
+__global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, WIDE>::CTAS) attention_rows(const __grid_constant__ AttnParams p) {
+  using R = Rows<T, CD, D, WIDE>;
   using C = typename R::C;
   constexpr bool Q8 = R::Q8;
-  constexpr int KS = R::KS, ES = R::ES, STAGES = R::STAGES;
+  constexpr int KS = R::KS, ES = R::ES, STAGES = R::STAGES, WARPS = R::WARPS;
   constexpr int NT = KS / 8;             // score tiles of 8 keys
   constexpr int KC = D * ES / 64;        // 16-byte pieces of a key a thread reads
   constexpr int STEPS = Q8 ? 4 : 2;      // products' steps of 16 that a piece serves
@@ -98,14 +100,14 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
 
   extern __shared__ __align__(128) uint8_t ring[];
   float(*const s_o)[16][PITCH] = reinterpret_cast<float(*)[16][PITCH]>(ring);  // when the loop is done
-  static_assert(4 * 16 * PITCH * 4 <= R::SMEM, "the warps' results lie over the ring");
-  __shared__ float s_m[4][16], s_l[4][16];
+  static_assert(WARPS * 16 * PITCH * 4 <= R::SMEM, "the warps' results lie over the ring");
+  __shared__ float s_m[WARPS][16], s_l[WARPS][16];
   __shared__ int s_last;
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int heads = static_cast<int>(p.a.cache.heads);
   const int unit = blockIdx.x / heads, h = blockIdx.x - unit * heads;
-  const Piece w = find_piece(p, unit, 16, 4 * KS);
+  const Piece w = find_piece(p, unit, 16, WARPS * KS);
   if (!w.some) return;
   const Seq s = sequence(p, w.b);
   const int rows = min(16, s.n * p.group - w.tile * 16);
@@ -170,9 +172,9 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) {
     const int now = page;
-    page = page_of(ahead + 4 * KS);
+    page = page_of(ahead + WARPS * KS);
     fetch(i, ahead, now);
-    ahead += 4 * KS;
+    ahead += WARPS * KS;
   }
   // this thread's two rows, g and g + 8: their queries and the keys that they see
   uint32_t qa[KC * STEPS][4];
@@ -236,12 +238,12 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
   float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
 
   int stage = 0;
-  for (int base = first; base < k1; base += 4 * KS) {
+  for (int base = first; base < k1; base += WARPS * KS) {
     {
       const int now = page;
-      page = page_of(ahead + 4 * KS);
+      page = page_of(ahead + WARPS * KS);
       fetch(stage == 0 ? STAGES - 1 : stage - 1, ahead, now);
-      ahead += 4 * KS;
+      ahead += WARPS * KS;
     }
     asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
     __syncwarp();
@@ -378,7 +380,7 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
     __syncwarp();  // the block's place may be filled again
   }
 
-  // join the four warps
+  // join the warps
   asm volatile("cp.async.wait_group 0;" ::: "memory");
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
@@ -396,7 +398,9 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int r = g + 8 * i;
-    const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
+    float top = s_m[0][r];
+#pragma unroll
+    for (int k = 1; k < WARPS; ++k) top = fmaxf(top, s_m[k][r]);
     const float f = m[i] == -INFINITY ? 0.0f : exp2_fast(m[i] - top);
 #pragma unroll
     for (int j = 0; j < OT; ++j)
@@ -408,104 +412,117 @@ __global__ void __launch_bounds__(128, 2) attention_rows(const __grid_constant__
   }
   __syncthreads();
 
-  // 8 threads a row, D / 8 columns each
-  constexpr int W = D / 8;
-  const int r = threadIdx.x >> 3, c0 = (threadIdx.x & 7) * W;
-  const float top = fmaxf(fmaxf(s_m[0][r], s_m[1][r]), fmaxf(s_m[2][r], s_m[3][r]));
-  float sum = 0.0f, acc[W];
+  // Four columns of a row a thread.
+  const auto store = [&](int row, int col, float4 v, float best, float sum) {
+    int tok = (r0 + row) / p.group;
+    const int hd = h * p.group + (r0 + row) - tok * p.group;
+    tok += s.start;
+    const bool none = best == -INFINITY;  // nothing visible: zeros
+    const float div = 1.0f / sum;
+    uint2 y = make_uint2(0, 0);
+    if (!none) y = make_uint2(pack2<T>(v.x * div, v.y * div), pack2<T>(v.z * div, v.w * div));
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.a.out) + tok * p.a.out_token + hd * p.a.out_head + col) = y;
+    if (p.a.lse && col == 0)
+      p.a.lse[static_cast<long>(tok) * p.a.q_heads + hd] = none ? -INFINITY : (best - P_SHIFT<C> + log2f(sum)) * 0.69314718055994531f;
+  };
+  const int positions = rows * (D / 4);
+  for (int at = threadIdx.x; at < positions; at += R::THREADS) {
+    const int row = at / (D / 4), col = (at - row * (D / 4)) * 4;
+    float best = s_m[0][row], sum = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-  for (int i = 0; i < W; ++i) acc[i] = s_o[0][r][c0 + i] + s_o[1][r][c0 + i] + s_o[2][r][c0 + i] + s_o[3][r][c0 + i];
+    for (int k = 1; k < WARPS; ++k) best = fmaxf(best, s_m[k][row]);
 #pragma unroll
-  for (int k = 0; k < 4; ++k) sum += s_m[k][r] == -INFINITY ? 0.0f : s_l[k][r] * exp2_fast(s_m[k][r] - top);
-  float best = top;
-  if (cuts > 1) {
-    if (r < rows) {
-      float* po = p.part_o + (static_cast<long>(blockIdx.x) * 16 + r) * D + c0;
-#pragma unroll
-      for (int i = 0; i < W; i += 4) __stcg(reinterpret_cast<float4*>(po + i), make_float4(acc[i], acc[i + 1], acc[i + 2], acc[i + 3]));
-      if ((threadIdx.x & 7) == 0) __stcg(p.part_ml + static_cast<long>(blockIdx.x) * 16 + r, make_float2(top, sum));
+    for (int k = 0; k < WARPS; ++k) {
+      const float4 x = *reinterpret_cast<const float4*>(&s_o[k][row][col]);
+      v = make_float4(v.x + x.x, v.y + x.y, v.z + x.z, v.w + x.w);
+      sum += s_m[k][row] == -INFINITY ? 0.0f : s_l[k][row] * exp2_fast(s_m[k][row] - best);
     }
-    __threadfence();
-    __syncthreads();
-    const int first = blockIdx.x - w.c * heads;  // the tile's first chunk
-    if (threadIdx.x == 0) {
-      const int done = atomicAdd(p.counters + first, 1);
-      s_last = done == cuts - 1;
-      if (s_last) p.counters[first] = 0;  // ready for the next call
+    if (cuts == 1) {
+      store(row, col, v, best, sum);
+    } else {
+      const long slot = static_cast<long>(blockIdx.x) * 16 + row;
+      __stcg(reinterpret_cast<float4*>(p.part_o + slot * D + col), v);
+      if (col == 0) __stcg(p.part_ml + slot, make_float2(best, sum));
     }
-    __syncthreads();
-    if (!s_last) return;
-    __threadfence();
-    // the chunks' weights and the rows' sums, eight threads a row
-    float* const weight = reinterpret_cast<float*>(ring);  // [cuts][16], as far as it goes
-    float4* const sums = reinterpret_cast<float4*>(ring + R::SMEM / 2);
-    constexpr int MOST = R::SMEM / 2 / 64;
-    const int t8 = threadIdx.x & 7;
-    best = -INFINITY;
-    if (r < rows)
-#pragma unroll 4
-      for (int k = t8; k < cuts; k += 8) best = fmaxf(best, __ldcg(p.part_ml + static_cast<long>(first + k * heads) * 16 + r).x);
+  }
+  if (cuts == 1) return;
+  __threadfence();
+  __syncthreads();
+  const int first_cta = blockIdx.x - w.c * heads;  // the tile's first chunk
+  if (threadIdx.x == 0) {
+    const int done = atomicAdd(p.counters + first_cta, 1);
+    s_last = done == cuts - 1;
+    if (s_last) p.counters[first_cta] = 0;  // ready for the next call
+  }
+  __syncthreads();
+  if (!s_last) return;
+  __threadfence();
+  // The chunks, in order.  Where there are fewer positions than threads, threads share a position's
+  // chunks and are joined in shared memory.
+  int shares = 1;
+  while (shares * 2 * positions <= R::THREADS && shares * 2 <= cuts) shares *= 2;
+  float* const joint = reinterpret_cast<float*>(ring);  // [shares * positions][6]
+  for (int at = threadIdx.x; at < positions * shares; at += R::THREADS) {
+    const int share = at / positions, pos = at - share * positions, row = pos / (D / 4), col = (pos - row * (D / 4)) * 4;
+    float best = -INFINITY, sum = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    constexpr int GO = 8;  // chunks whose loads are in flight together
+    for (int k = share; k < cuts; k += GO * shares) {
+      float2 ml[GO];
+      float4 x[GO];
+      float top = best;
 #pragma unroll
-    for (int o = 4; o > 0; o >>= 1) best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
-    sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < W; ++i) acc[i] = 0.0f;
-    // positions: 16 bytes of a row; where there are fewer than threads, they share the chunks
-    const int positions = rows * (D / 4);
-    int shares = 1;
-    while (shares * 2 * positions <= 128) shares *= 2;
-    for (int k0 = 0; k0 < cuts; k0 += MOST) {
-      const int n = min(MOST, cuts - k0);
-      __syncthreads();
-      if (r < rows)
-#pragma unroll 4
-        for (int k = t8; k < n; k += 8) {
-          const float2 ml = __ldcg(p.part_ml + static_cast<long>(first + (k0 + k) * heads) * 16 + r);
-          const float f = ml.x == -INFINITY ? 0.0f : exp2_fast(ml.x - best);
-          weight[k * 16 + r] = f;
-          sum += ml.y * f;
-        }
-      __syncthreads();
-      for (int at = threadIdx.x; at < positions * shares; at += 128) {
-        const int share = at / positions, pos = at - share * positions, row = pos / (D / 4), c4 = pos - row * (D / 4);
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 8
-        for (int k = share; k < n; k += shares) {
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(p.part_o + (static_cast<long>(first + (k0 + k) * heads) * 16 + row) * D) + c4);
-          const float f = weight[k * 16 + row];
-          v = make_float4(v.x + x.x * f, v.y + x.y * f, v.z + x.z * f, v.w + x.w * f);
-        }
-        sums[at] = v;
+      for (int i = 0; i < GO; ++i) {
+        const long slot = static_cast<long>(first_cta + min(k + i * shares, cuts - 1) * heads) * 16 + row;
+        ml[i] = __ldcg(p.part_ml + slot);
+        x[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot * D + col));
       }
-      __syncthreads();
-      if (r < rows)
-        for (int share = 0; share < shares; ++share)
 #pragma unroll
-          for (int i = 0; i < W; i += 4) {
-            const float4 v = sums[share * positions + r * (D / 4) + (c0 + i) / 4];
-            acc[i] += v.x;
-            acc[i + 1] += v.y;
-            acc[i + 2] += v.z;
-            acc[i + 3] += v.w;
-          }
+      for (int i = 0; i < GO; ++i) {
+        if (k + i * shares >= cuts) ml[i].x = -INFINITY;
+        top = fmaxf(top, ml[i].x);
+      }
+      if (top == -INFINITY) continue;
+      const float f = exp2_fast(best - top);
+      v = make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+      sum *= f;
+#pragma unroll
+      for (int i = 0; i < GO; ++i) {
+        if (ml[i].x == -INFINITY) continue;
+        const float e = exp2_fast(ml[i].x - top);
+        v = make_float4(v.x + x[i].x * e, v.y + x[i].y * e, v.z + x[i].z * e, v.w + x[i].w * e);
+        sum += ml[i].y * e;
+      }
+      best = top;
     }
-#pragma unroll
-    for (int o = 4; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    if (shares == 1) {
+      store(row, col, v, best, sum);
+    } else {
+      float* const j = joint + at * 6;
+      j[0] = v.x;
+      j[1] = v.y;
+      j[2] = v.z;
+      j[3] = v.w;
+      j[4] = best;
+      j[5] = sum;
+    }
   }
-  if (r >= rows) return;
-  const int tok = (r0 + r) / p.group, hd = h * p.group + (r0 + r) - tok * p.group;
-  const bool none = best == -INFINITY;  // nothing visible: zeros
-  const float div = none ? 0.0f : 1.0f / sum;
-  T* dst = static_cast<T*>(p.a.out) + (s.start + tok) * p.a.out_token + hd * p.a.out_head + c0;
-#pragma unroll
-  for (int i = 0; i < W; i += 8) {
-    float y[8];
-#pragma unroll
-    for (int k = 0; k < 8; ++k) y[k] = none ? 0.0f : acc[i + k] * div;
-    tj_store_vec(dst + i, y);
+  if (shares == 1) return;
+  __syncthreads();
+  for (int pos = threadIdx.x; pos < positions; pos += R::THREADS) {
+    float best = -INFINITY, sum = 0.0f;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int share = 0; share < shares; ++share) best = fmaxf(best, joint[(share * positions + pos) * 6 + 4]);
+    for (int share = 0; share < shares; ++share) {
+      const float* const j = joint + (share * positions + pos) * 6;
+      if (j[4] == -INFINITY) continue;
+      const float e = exp2_fast(j[4] - best);
+      v = make_float4(v.x + j[0] * e, v.y + j[1] * e, v.z + j[2] * e, v.w + j[3] * e);
+      sum += j[5] * e;
+    }
+    store(pos / (D / 4), (pos - pos / (D / 4) * (D / 4)) * 4, v, best, sum);
   }
-  if (p.a.lse && (threadIdx.x & 7) == 0)
-    p.a.lse[(s.start + tok) * p.a.q_heads + hd] = none ? -INFINITY : (best - P_SHIFT<C> + log2f(sum)) * 0.69314718055994531f;
 }
 
 }  // namespace tjs
