@@ -14,8 +14,8 @@
 // two keys' elements are paired by a byte permutation.  The pieces of a row are permuted by its number
 // so that both ways of reading are free of bank conflicts.
 //
-// An 8-bit cache's codes become f16, bf16 queries too (a row times the power of two that brings its
-// largest element near 2^10: exact but for elements 2^-24 of that): the byte permutations and masks run
+// An 8-bit cache's codes become f16, bf16 queries too (times the power of two that brings the tile's
+// largest element near 2^14: exact but for elements 2^-28 of that): the byte permutations and masks run
 // at half rate and were the bound, and bf16 needs three for a pair of codes where f16 needs 1.5 (keys) and
 // 2 (values).
 //
@@ -46,6 +46,9 @@ TJ_DEV uint32_t word(const uint4& v, int i) { return i == 0 ? v.x : i == 1 ? v.y
 TJ_DEV void copy16(uint32_t dst, const void* src, bool on) {
   const int bytes = on ? 16 : 0;  // 0: zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+TJ_DEV void copy16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
 TJ_DEV void copy4(uint32_t dst, const void* src, bool on) {
   const int bytes = on ? 4 : 0;
@@ -136,32 +139,53 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
     if (lane >= KS || key >= k1) return INT_MIN;
     return table[p.page_shift >= 0 ? key >> p.page_shift : key / page_size];
   };
+  // Where a lane copies to, and reads from, in a block: its first row's piece; further rows are at constant
+  // distances, but for bits that the permutation turns by the row's number, which are constants too.
+  constexpr int PIECES = R::ROW / 16, PER = 32 / PIECES;  // lanes of a row, rows of a warp's instruction
+  const uint32_t copy_at = R::piece(lane / PIECES, lane % PIECES);
+  const uint32_t key_at = R::piece(g, t), value_at0 = R::piece(2 * t, VB == 8 ? g >> 1 : g) + (VB == 8 ? (g & 1) * 8 : 0),
+                 value_at1 = R::piece(2 * t + 1, VB == 8 ? g >> 1 : g) + (VB == 8 ? (g & 1) * 8 : 0);
+  const char* const my_k = kbase + (lane % PIECES) * 16;
+  const long to_v = vbase - kbase;
   auto fetch = [&](int stage, int base, int page) {
-    long off = -1, soff = -1;
+    const char* row = my_k;  // this lane looks it up for others, so the piece is added where it is used
+    long soff = 0;
+    bool on = false;
     if (page >= 0 && page < p.a.cache.pages) {
       const int key = base + lane, slot = p.page_shift >= 0 ? key & (page_size - 1) : key % page_size;
-      off = (page * p.a.cache.page_stride + slot * p.a.cache.slot_stride) * ES;
+      row = kbase + (page * p.a.cache.page_stride + slot * p.a.cache.slot_stride) * ES;
       if (Q8) soff = page * p.a.cache.scale_page + slot * p.a.cache.scale_slot;
+      on = true;
     } else if (page != INT_MIN) {
       tj_report(p.status, TJ_STATUS_BOUNDS, OP_ATTENTION * 16 + SITE_PAGE);
     }
-    if (base < k1) {
-      constexpr int PIECES = R::ROW / 16, PER = 32 / PIECES;  // lanes of a row, rows of a warp's instruction
-      const uint32_t dst = my_ring + stage * R::BLOCK;
-      const int i = lane % PIECES;
+    const unsigned live = __ballot_sync(0xffffffffu, on);
+    const uint32_t dst = my_ring + stage * R::BLOCK;
+    const uint32_t mine = live >> (lane / PIECES);
+    const long add = (lane % PIECES) * 16;
+    constexpr unsigned ALL = KS == 32 ? 0xffffffffu : (1u << KS) - 1;
+    if (live == ALL) {
 #pragma unroll
       for (int j = 0; j < KS / PER; ++j) {
-        const int r = j * PER + lane / PIECES;
-        const long ro = __shfl_sync(0xffffffffu, off, r);
-        const long src = (ro < 0 ? 0 : ro) + i * 16;
-        copy16(dst + R::piece(r, i), kbase + src, ro >= 0);
-        copy16(dst + KS * R::ROW + R::piece(r, i), vbase + src, ro >= 0);
+        const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<long>(row), j * PER + lane / PIECES)) + add;
+        const uint32_t at = dst + (copy_at ^ (((j * PER / 2) & 3) << 5)) + j * PER * R::ROW;
+        copy16(at, src);
+        copy16(at + KS * R::ROW, src + to_v);
       }
-      if (Q8) {
-        const uint32_t s = my_ring + STAGES * R::BLOCK + (stage * KS * 3 + lane) * 4;
-        copy4(s, ksc + (soff < 0 ? 0 : soff), soff >= 0);
-        copy4(s + KS * 4, vsc + (soff < 0 ? 0 : soff), soff >= 0);
+    } else if (base < k1) {
+#pragma unroll
+      for (int j = 0; j < KS / PER; ++j) {
+        const char* src = reinterpret_cast<const char*>(__shfl_sync(0xffffffffu, reinterpret_cast<long>(row), j * PER + lane / PIECES)) + add;
+        const uint32_t at = dst + (copy_at ^ (((j * PER / 2) & 3) << 5)) + j * PER * R::ROW;
+        const bool there = (mine >> (j * PER)) & 1;
+        copy16(at, there ? src : my_k, there);
+        copy16(at + KS * R::ROW, there ? src + to_v : my_k, there);
       }
+    }
+    if (Q8 && base < k1) {
+      const uint32_t s = my_ring + STAGES * R::BLOCK + (stage * KS * 3 + lane) * 4;
+      copy4(s, ksc + soff, on);
+      copy4(s + KS * 4, vsc + soff, on);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -202,31 +226,26 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
     }
   }
 
-  float unscale[2] = {1.0f, 1.0f};  // what the rows' queries were divided by
+  float score_scale = p.scale_log2;
   if constexpr (!std::is_same<T, C>::value) {
+    uint32_t top = 0;  // the largest element of all rows, as bits
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      uint32_t top = 0;
+    for (int c = 0; c < KC * STEPS; ++c)
 #pragma unroll
-      for (int c = 0; c < KC * STEPS; ++c)
+      for (int e = 0; e < 4; ++e) top = max(top, max((qa[c][e] & 0x7fffu) << 16, qa[c][e] & 0x7fff0000u));
+    top = __reduce_max_sync(0xffffffffu, top);
+    // 2^(14 - its exponent), within what f32 holds twice over; 1 for zeros, infinities and NaN
+    const int raise = min(14 - (static_cast<int>(top >> 23) - 127), 100);
+    const bool fine = top >= 0x00800000u && top < 0x7f800000u;
+    const float up = fine ? __int_as_float((127 + raise) << 23) : 1.0f;
+    score_scale *= fine ? __int_as_float((127 - raise) << 23) : 1.0f;
 #pragma unroll
-        for (int e = 0; e < 4; e += 2) top = max(top, max((qa[c][i + e] & 0x7fffu) << 16, qa[c][i + e] & 0x7fff0000u));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^(10 - exponent); none for zeros, infinities and NaN
-      const int exponent = static_cast<int>(top >> 23) - 127;
-      const bool fine = top >= 0x00800000u && top < 0x7f800000u;
-      const float up = fine ? __int_as_float((127 + min(10 - exponent, 127)) << 23) : 1.0f;
-      unscale[i] = fine ? __int_as_float((127 - min(10 - exponent, 126)) << 23) : 1.0f;
-      if (fine && 10 - exponent > 126) unscale[i] = 1.0f / up;
+    for (int c = 0; c < KC * STEPS; ++c)
 #pragma unroll
-      for (int c = 0; c < KC * STEPS; ++c)
-#pragma unroll
-        for (int e = 0; e < 4; e += 2) {
-          uint32_t& w = qa[c][i + e];
-          w = tj_pack_f16x2(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up);
-        }
-    }
+      for (int e = 0; e < 4; ++e) {
+        uint32_t& w = qa[c][e];
+        w = tj_pack_f16x2(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up);
+      }
   }
 
   // keys that all of the tile's rows see need no mask
@@ -250,7 +269,7 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
     const uint32_t kblock = my_ring + stage * R::BLOCK, vblock = kblock + KS * R::ROW;
     float* const scale = reinterpret_cast<float*>(ring + warp * R::WARP + STAGES * R::BLOCK) + stage * KS * 3;
     if constexpr (Q8) {
-      scale[lane] *= p.scale_log2;
+      scale[lane] *= score_scale;
       const float lv = fmaxf(__log2f(scale[KS + lane]), MIN_LOG2_SCALE);
       scale[KS + lane] = lv;
       scale[2 * KS + lane] = exp2_fast(-lv);
@@ -258,49 +277,58 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
     }
     if (++stage == STAGES) stage = 0;
 
+    // the tiles' products are independent chains, so they go side by side
     float sc[NT][4];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
+    for (int j = 0; j < NT; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
 #pragma unroll
-      for (int c = 0; c < KC; ++c) {
-        const uint4 kf = lds16(kblock + R::piece(8 * j + g, c * 4 + t));
-        if constexpr (Q8) {
+    for (int c = 0; c < KC; ++c) {
+      uint4 kf[NT];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint32_t b0, b1;
-            codes4<C, CD>(word(kf, e), b0, b1);
-            mma16816<C>(sc[j], qa[c * 4 + e], b0, b1);
+      for (int j = 0; j < NT; ++j) kf[j] = lds16(kblock + (key_at ^ (c << 6)) + 8 * j * R::ROW);
+#pragma unroll
+      for (int e = 0; e < STEPS; ++e) {
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          uint32_t b0, b1;
+          if constexpr (Q8) {
+            codes4<C, CD>(word(kf[j], e), b0, b1);
+          } else {
+            b0 = word(kf[j], 2 * e);
+            b1 = word(kf[j], 2 * e + 1);
           }
-        } else {
-          mma16816<C>(sc[j], qa[c * 2], kf.x, kf.y);
-          mma16816<C>(sc[j], qa[c * 2 + 1], kf.z, kf.w);
+          mma16816<C>(sc[j], qa[c * STEPS + e], b0, b1);
         }
       }
     }
     // t = scaled score (8-bit cache: + log2 vs); masked keys -inf
-    const bool masked = base < mlo || base + KS > mhi;  // the same for the warp
-    float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
     for (int j = 0; j < NT; ++j) {
-      float2 kfac = make_float2(p.scale_log2, p.scale_log2), lv = make_float2(0.0f, 0.0f);
+      float2 kfac = make_float2(score_scale, score_scale), lv = make_float2(0.0f, 0.0f);
       if constexpr (Q8) {
         kfac = *reinterpret_cast<const float2*>(scale + 8 * j + 2 * t);
         lv = *reinterpret_cast<const float2*>(scale + KS + 8 * j + 2 * t);
       }
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int key = base + 8 * j + 2 * t + e;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          float& x = sc[j][2 * i + e];
-          if (!std::is_same<T, C>::value) x *= unscale[i];
-          x = Q8 ? fmaf(x, e ? kfac.y : kfac.x, e ? lv.y : lv.x) : x * (e ? kfac.y : kfac.x);
-          if (masked && (key < rlo[i] || key >= rhi[i])) x = -INFINITY;
-          mx[i] = fmaxf(mx[i], x);
-        }
+      for (int e = 0; e < 4; ++e) {
+        float& x = sc[j][e];
+        x = Q8 ? fmaf(x, e & 1 ? kfac.y : kfac.x, e & 1 ? lv.y : lv.x) : x * score_scale;
       }
     }
+    if (base < mlo || base + KS > mhi) {  // the same for the warp
+#pragma unroll
+      for (int j = 0; j < NT; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = base + 8 * j + 2 * t + (e & 1);
+          if (key < rlo[e >> 1] || key >= rhi[e >> 1]) sc[j][e] = -INFINITY;
+        }
+    }
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) mx[i] = fmaxf(mx[i], fmaxf(sc[j][2 * i], sc[j][2 * i + 1]));
     bool moved = false;
     float base_m[2], alpha[2];
 #pragma unroll
@@ -340,15 +368,15 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
       const uint32_t pa[4] = {pack2<C>(sc[2 * k16][0], sc[2 * k16][1]), pack2<C>(sc[2 * k16][2], sc[2 * k16][3]),
                               pack2<C>(sc[2 * k16 + 1][0], sc[2 * k16 + 1][1]), pack2<C>(sc[2 * k16 + 1][2], sc[2 * k16 + 1][3])};
       uint32_t va[VW], vb[VW], vc[VW], vd[VW];  // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the step
-      auto value = [&](uint32_t (&v)[VW], int row) {
+      auto value = [&](uint32_t (&v)[VW], uint32_t at) {
         if constexpr (VB == 8) {
-          const uint2 x = lds8(vblock + R::piece(row, g >> 1) + (g & 1) * 8);
+          const uint2 x = lds8(vblock + at);
           v[0] = x.x;
           v[1] = x.y;
         } else {
 #pragma unroll
           for (int c = 0; c < VC; ++c) {
-            const uint4 x = lds16(vblock + R::piece(row, c * 8 + g));
+            const uint4 x = lds16(vblock + at + c * 128);
             v[(4 * c) % VW] = x.x;
             v[(4 * c + 1) % VW] = x.y;
             v[(4 * c + 2) % VW] = x.z;
@@ -356,10 +384,10 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
           }
         }
       };
-      value(va, k16 * 16 + 2 * t);
-      value(vb, k16 * 16 + 2 * t + 1);
-      value(vc, k16 * 16 + 2 * t + 8);
-      value(vd, k16 * 16 + 2 * t + 9);
+      value(va, value_at0 + k16 * 16 * R::ROW);
+      value(vb, value_at1 + k16 * 16 * R::ROW);
+      value(vc, value_at0 + (k16 * 16 + 8) * R::ROW);
+      value(vd, value_at1 + (k16 * 16 + 8) * R::ROW);
 #pragma unroll
       for (int j = 0; j < OT; ++j) {
         uint32_t b0, b1;
@@ -394,7 +422,7 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
   }
   __syncthreads();
   constexpr int NV = VB / ES;           // output columns from one thread's piece of a value, of each of ...
-  constexpr int PER = NV > 16 / ES ? 16 / ES : NV;  // ... PER consecutive ones at a time
+  constexpr int RUN = NV > 16 / ES ? 16 / ES : NV;  // ... RUN consecutive ones at a time
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const int r = g + 8 * i;
@@ -406,7 +434,7 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
     for (int j = 0; j < OT; ++j)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int col = (j / PER) * 8 * PER + (2 * t + e) * PER + j % PER;
+        const int col = (j / RUN) * 8 * RUN + (2 * t + e) * RUN + j % RUN;
         s_o[warp][r][col] = o[j][2 * i + e] * f;
       }
   }
