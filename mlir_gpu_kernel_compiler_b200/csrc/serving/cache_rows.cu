@@ -18,7 +18,10 @@
 // pair (half layout: units u and u + rot / 16) is in one lane's registers, max|x| is a shuffle
 // over the row's lanes, and every access is 16 bytes.  A lane keeps its slot's cosines and sines
 // in registers over the heads of its token: the table is read once per token, not once per row.
-// A warp takes 32 / lanes rows at a time, `batch` of them before it stores.
+// A warp takes 32 / lanes rows at a time and loads four such groups, unconverted, before it turns the first:
+// the kernel is bound by HBM, and so by the reads in flight.
+#include <algorithm>
+
 #include "serving_common.cuh"
 
 static __device__ __align__(16) int tj_serving_words[4];
@@ -31,7 +34,8 @@ struct RowsParams {
   int lanes_log2;  // lanes of a row
   int slots;       // slots of a row: ceil(dim / 16)
   int iters;       // warp iterations over a token's rows
-  int segs;        // warps that share a token
+  Div segs;        // warps that share a token
+  Div page;        // slots of a page
   int op;
 };
 
@@ -44,11 +48,18 @@ TJ_DEV uint4 ld16_row(const void* p) {
                : "memory");
   return v;
 }
-TJ_DEV void load8(const float* p, float* f) {
-  tj_unpack(ld16_row(p), f, p);
-  tj_unpack(ld16_row(p + 4), f + 4, p);
-}
-template <class T> TJ_DEV void load8(const T* p, float* f) { tj_unpack(ld16_row(p), f, p); }
+// a unit of 8 elements as it is read
+template <class T> struct Unit {
+  uint4 v[sizeof(T) / 2];
+  TJ_DEV void load(const T* p) {
+    v[0] = ld16_row(p);
+    if constexpr (sizeof(T) == 4) v[1] = ld16_row(p + 4);
+  }
+  TJ_DEV void get(float* f) const {
+    tj_unpack(v[0], f, (const T*)nullptr);
+    if constexpr (sizeof(T) == 4) tj_unpack(v[1], f + 4, (const T*)nullptr);
+  }
+};
 TJ_DEV void store8(float* p, const float* f) {
   tj_store_vec(p, f);
   tj_store_vec(p + 4, f + 4);
@@ -69,19 +80,18 @@ TJ_DEV uint32_t i8x4(const float* f) {
 
 // ROT: 0 none; 1 half layout, whole units; 2 interleaved, whole units; 3 either, any even rot
 // (pairs that cross units: partners and table entries one by one).
-template <class T, int ROT>
+// CACHE: 0 none, 1 a 16-bit one, 2 i8, 3 e4m3.
+template <class T, int ROT, int CACHE>
 __global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ RowsParams p) {
   const tj_rows& a = p.a;
-  const int lane = threadIdx.x & 31;
-  const long wid = static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-  const long token = wid / p.segs;
-  const int seg = static_cast<int>(wid - token * p.segs);
+  const int lane = threadIdx.x & 31, wid = static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+  const int token = p.segs(wid), seg = wid - token * static_cast<int>(p.segs.d);
   if (token >= a.tokens) return;
   const int dim = static_cast<int>(a.dim), rot = static_cast<int>(a.rot), half = rot >> 1;
   const int lpr = 1 << p.lanes_log2, sub = lane >> p.lanes_log2, per = 32 >> p.lanes_log2, s = lane & (lpr - 1);
   const bool on = s < p.slots;
 
-  // the slot's two units (ua < 0 or ub < 0: none)
+  // the slot's two units
   int ua = 2 * s, ub = 2 * s + 1;
   if (ROT == 1) {
     const int pairs = rot >> 4;
@@ -95,15 +105,37 @@ __global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ RowsP
   }
   const bool has_b = on && ub * 8 < dim;
 
+  const int nq = a.q ? static_cast<int>(a.q_heads) : 0, nk = a.k ? static_cast<int>(a.kv_heads) : 0,
+            nv = a.v ? static_cast<int>(a.kv_heads) : 0;
+  const int rows = nq + nk + nv;
+  const T* const q = static_cast<const T*>(a.q) + token * a.q_token;
+  const T* const k = static_cast<const T*>(a.k) + token * a.k_token;
+  const T* const v = static_cast<const T*>(a.v) + token * a.v_token;
+  auto source = [&](int r) { return r < nq ? q + r * a.q_head : r < nq + nk ? k + (r - nq) * a.k_head : v + (r - nq - nk) * a.v_head; };
+  constexpr int BATCH = sizeof(T) == 4 ? 2 : 4;
+  Unit<T> raw[BATCH][2];
+  const int segs = static_cast<int>(p.segs.d);
+  const int i0 = static_cast<int>(static_cast<unsigned>(seg) * p.iters / segs), i1 = static_cast<int>(static_cast<unsigned>(seg + 1) * p.iters / segs);
+  auto load = [&](int it) {
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      const int r = (it + j) * per + sub;
+      if (it + j < i1 && r < rows && on) {
+        const T* src = source(r);
+        raw[j][0].load(src + ua * 8);
+        if (has_b) raw[j][1].load(src + ub * 8);
+      }
+    }
+  };
+  load(i0);  // in flight while the table's row and the slot are looked up
+
   float cs[8] = {}, sn[8] = {};
   const float* trow = nullptr;
   bool lost = false;  // a position outside the table: the row becomes NaN
-  if (ROT) {
+  if constexpr (ROT != 0) {
     const int pos = a.positions[token];
     lost = pos < 0 || pos >= a.table_rows;
-    if (lost) {
-      if (lane == 0) tj_report(p.status, TJ_STATUS_BOUNDS, p.op * 16 + SITE_POSITION);
-    }
+    if (lost && lane == 0) tj_report(p.status, TJ_STATUS_BOUNDS, p.op * 16 + SITE_POSITION);
     trow = a.table + (lost ? 0 : static_cast<long>(pos) * rot);
     const float sign = a.inverse ? -1.0f : 1.0f;
     if (ROT == 1 && on && ua * 8 < half) {
@@ -132,11 +164,11 @@ __global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ RowsP
     }
   }
   long crow = -1, srow = 0;
-  if (a.slots) {
+  if constexpr (CACHE != 0) {
     const int slot = a.slots[token];
     const long cap = a.cache.pages * a.cache.page_size;
     if (slot >= 0 && slot < cap) {
-      const int page = slot / static_cast<int>(a.cache.page_size), at = slot - page * static_cast<int>(a.cache.page_size);
+      const int page = p.page(slot), at = slot - page * static_cast<int>(p.page.d);
       crow = page * a.cache.page_stride + at * a.cache.slot_stride;
       srow = page * a.cache.scale_page + at * a.cache.scale_slot;
     } else if (slot >= cap && lane == 0) {
@@ -144,59 +176,41 @@ __global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ RowsP
     }
   }
 
-  const int nq = a.q ? static_cast<int>(a.q_heads) : 0, nk = a.k ? static_cast<int>(a.kv_heads) : 0,
-            nv = a.v ? static_cast<int>(a.kv_heads) : 0;
-  const int rows = nq + nk + nv;
-  const int i0 = static_cast<int>(static_cast<long>(seg) * p.iters / p.segs),
-            i1 = static_cast<int>(static_cast<long>(seg + 1) * p.iters / p.segs);
-  constexpr int BATCH = 4;
   for (int it = i0; it < i1; it += BATCH) {
-    float x[BATCH][16];
+    if (it != i0) load(it);
 #pragma unroll
     for (int j = 0; j < BATCH; ++j) {
       const int r = (it + j) * per + sub;
-      if (it + j < i1 && r < rows && on) {
-        const T* src = r < nq          ? static_cast<const T*>(a.q) + token * a.q_token + r * a.q_head
-                       : r < nq + nk ? static_cast<const T*>(a.k) + token * a.k_token + (r - nq) * a.k_head
-                                     : static_cast<const T*>(a.v) + token * a.v_token + (r - nq - nk) * a.v_head;
-        load8(src + ua * 8, x[j]);
-        if (has_b) {
-          load8(src + ub * 8, x[j] + 8);
-        } else {
+      if (it + j >= i1) break;
+      const bool mine = r < rows && on;
+      float x[16];
 #pragma unroll
-          for (int i = 8; i < 16; ++i) x[j][i] = 0.0f;
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[j][i] = 0.0f;
+      for (int i = 0; i < 16; ++i) x[i] = 0.0f;
+      if (mine) {
+        raw[j][0].get(x);
+        if (has_b) raw[j][1].get(x + 8);
       }
-    }
-#pragma unroll
-    for (int j = 0; j < BATCH; ++j) {
-      const int r = (it + j) * per + sub;
-      const bool mine = it + j < i1 && r < rows && on;
-      if (ROT == 1 && mine && r < nq + nk && ua * 8 < half) {
+      if (ROT == 1 && r < nq + nk && ua * 8 < half) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          const float u = x[j][i], v = x[j][i + 8];
-          x[j][i] = __fsub_rn(__fmul_rn(u, cs[i]), __fmul_rn(v, sn[i]));
-          x[j][i + 8] = __fadd_rn(__fmul_rn(v, cs[i]), __fmul_rn(u, sn[i]));
+          const float u = x[i], w = x[i + 8];
+          x[i] = __fsub_rn(__fmul_rn(u, cs[i]), __fmul_rn(w, sn[i]));
+          x[i + 8] = __fadd_rn(__fmul_rn(w, cs[i]), __fmul_rn(u, sn[i]));
         }
       }
-      if (ROT == 2 && mine && r < nq + nk) {
+      if (ROT == 2 && r < nq + nk) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           if ((i < 4 ? ua : ub) * 8 < rot) {
-            const float u = x[j][2 * i], v = x[j][2 * i + 1];
-            x[j][2 * i] = __fsub_rn(__fmul_rn(u, cs[i]), __fmul_rn(v, sn[i]));
-            x[j][2 * i + 1] = __fadd_rn(__fmul_rn(v, cs[i]), __fmul_rn(u, sn[i]));
+            const float u = x[2 * i], w = x[2 * i + 1];
+            x[2 * i] = __fsub_rn(__fmul_rn(u, cs[i]), __fmul_rn(w, sn[i]));
+            x[2 * i + 1] = __fadd_rn(__fmul_rn(w, cs[i]), __fmul_rn(u, sn[i]));
           }
         }
       }
-      if (ROT == 3) {
+      if constexpr (ROT == 3) {
         if (mine && r < nq + nk) {
-          const T* src = r < nq ? static_cast<const T*>(a.q) + token * a.q_token + r * a.q_head
-                                : static_cast<const T*>(a.k) + token * a.k_token + (r - nq) * a.k_head;
+          const T* src = source(r);
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int e = (i < 8 ? ua : ub) * 8 + (i & 7);
@@ -206,67 +220,63 @@ __global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ RowsP
             const int other = a.interleaved ? e ^ 1 : (second ? e - half : e + half);
             float c = trow[pair], sv = trow[half + pair] * (a.inverse ? -1.0f : 1.0f);
             if (lost) c = sv = __int_as_float(0x7fffffff);
-            // re-read: the partner may be in another lane, and x[j] is overwritten in place
+            // read again: the partner may be in another lane, and x is overwritten in place
             const float mate = tj_f32(src[other]), own = tj_f32(src[e]);
-            x[j][i] = second ? __fadd_rn(__fmul_rn(own, c), __fmul_rn(mate, sv))
-                             : __fsub_rn(__fmul_rn(own, c), __fmul_rn(mate, sv));
+            x[i] = second ? __fadd_rn(__fmul_rn(own, c), __fmul_rn(mate, sv)) : __fsub_rn(__fmul_rn(own, c), __fmul_rn(mate, sv));
           }
         }
         __syncwarp();  // every lane has read the row before any lane stores over it (outputs in place)
       }
-      const bool to_cache = a.slots && r >= nq;
-      if (!to_cache) {
+      if (CACHE == 0 || r < nq) {
         if (mine) {
           T* dst = r < nq ? static_cast<T*>(a.q_out) + token * a.qo_token + r * a.qo_head
                           : static_cast<T*>(a.k_out) + token * a.ko_token + (r - nq) * a.ko_head;
-          store8(dst + ua * 8, x[j]);
-          if (has_b) store8(dst + ub * 8, x[j] + 8);
+          store8(dst + ua * 8, x);
+          if (has_b) store8(dst + ub * 8, x + 8);
         }
       }
-      if (!a.slots) continue;
-      const bool key = r < nq + nk;
-      const int h = key ? r - nq : r - nq - nk;
-      void* base = key ? a.cache.k : a.cache.v;
-      const long off = crow + h * a.cache.head_stride;
-      const bool put = mine && to_cache && crow >= 0;
-      if (a.cache.dtype == TJ_BF16 || a.cache.dtype == TJ_F16) {
-        if (put) {
-          if (a.cache.dtype == TJ_BF16) {
-            store8(static_cast<__nv_bfloat16*>(base) + off + ua * 8, x[j]);
-            if (has_b) store8(static_cast<__nv_bfloat16*>(base) + off + ub * 8, x[j] + 8);
-          } else {
-            store8(static_cast<__half*>(base) + off + ua * 8, x[j]);
-            if (has_b) store8(static_cast<__half*>(base) + off + ub * 8, x[j] + 8);
+      if constexpr (CACHE != 0) {
+        const bool key = r < nq + nk, put = mine && r >= nq && crow >= 0;
+        const int h = key ? r - nq : r - nq - nk;
+        void* base = key ? a.cache.k : a.cache.v;
+        const long off = crow + h * a.cache.head_stride;
+        if constexpr (CACHE == 1) {
+          if (put) {
+            if (a.cache.dtype == TJ_BF16) {
+              store8(static_cast<__nv_bfloat16*>(base) + off + ua * 8, x);
+              if (has_b) store8(static_cast<__nv_bfloat16*>(base) + off + ub * 8, x + 8);
+            } else {
+              store8(static_cast<__half*>(base) + off + ua * 8, x);
+              if (has_b) store8(static_cast<__half*>(base) + off + ub * 8, x + 8);
+            }
           }
-        }
-      } else {
-        // max|x| over the row's lanes, as bits: an infinity or a NaN orders above every number
-        uint32_t top = 0;
+        } else {
+          // max|x| over the row's lanes, as bits: an infinity or a NaN orders above every number
+          uint32_t top = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[j][i]) & 0x7fffffffu);
-        for (int o = lpr >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const bool i8 = a.cache.dtype == TJ_I8;
-        float scale = __fdiv_rn(__uint_as_float(top), i8 ? 127.0f : 448.0f);
-        if (put) {
-          // a row with an infinity or a NaN is held as NaN (scale) times zero codes
-          const bool bad = top >= 0x7f800000u;
-          if (bad) scale = __int_as_float(0x7fffffff);
-          const bool zero = bad || scale == 0.0f;
-          float y[16];
+          for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+          for (int o = lpr >> 1; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          float scale = __fdiv_rn(__uint_as_float(top), CACHE == 2 ? 127.0f : 448.0f);
+          if (put) {
+            // a row with an infinity or a NaN is held as NaN (scale) times zero codes
+            const bool bad = top >= 0x7f800000u;
+            if (bad) scale = __int_as_float(0x7fffffff);
+            const bool zero = bad || scale == 0.0f;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) y[i] = zero ? 0.0f : __fdiv_rn(x[j][i], scale);
-          uint8_t* dst = static_cast<uint8_t*>(base) + off;
-          uint2 w0, w1;
-          if (i8) {
-            w0 = make_uint2(i8x4(y), i8x4(y + 4));
-            w1 = make_uint2(i8x4(y + 8), i8x4(y + 12));
-          } else {
-            w0 = make_uint2(e4m3x4(y), e4m3x4(y + 4));
-            w1 = make_uint2(e4m3x4(y + 8), e4m3x4(y + 12));
+            for (int i = 0; i < 16; ++i) x[i] = zero ? 0.0f : __fdiv_rn(x[i], scale);
+            uint8_t* dst = static_cast<uint8_t*>(base) + off;
+            uint2 w0, w1;
+            if (CACHE == 2) {
+              w0 = make_uint2(i8x4(x), i8x4(x + 4));
+              w1 = make_uint2(i8x4(x + 8), i8x4(x + 12));
+            } else {
+              w0 = make_uint2(e4m3x4(x), e4m3x4(x + 4));
+              w1 = make_uint2(e4m3x4(x + 8), e4m3x4(x + 12));
+            }
+            *reinterpret_cast<uint2*>(dst + ua * 8) = w0;
+            if (has_b) *reinterpret_cast<uint2*>(dst + ub * 8) = w1;
+            if (s == 0) (key ? a.cache.k_scale : a.cache.v_scale)[srow + h * a.cache.scale_head] = scale;
           }
-          *reinterpret_cast<uint2*>(dst + ua * 8) = w0;
-          if (has_b) *reinterpret_cast<uint2*>(dst + ub * 8) = w1;
-          if (s == 0) (key ? a.cache.k_scale : a.cache.v_scale)[srow + h * a.cache.scale_head] = scale;
         }
       }
     }
@@ -277,92 +287,109 @@ struct ReadParams {
   tj_kv_cache c;
   const int* slots;
   void* out[2];
-  long rows;  // n * heads
+  int rows;  // n * heads
   int* status;
-  int lanes_log2, slots_per_row, batch;
+  int lanes_log2, slots_per_row, batches;
+  Div heads, page;
 };
 
 // Rows (slot, head) of the keys and of the values back as T: value = code * scale in f32, rounded
-// once.  CD: the cache's dtype.  A slot of -1 reads as zeros.
+// once.  CD: the cache's dtype.  A slot of -1 reads as zeros.  A warp goes through `batches` groups of rows
+// and looks a group's slots up while it reads the one before: the rows' addresses hang on them, and
+// with both in one go there was a second latency with nothing in flight (4000 GB/s).
 template <class T, int CD>
 __global__ void __launch_bounds__(128) read_kernel(const __grid_constant__ ReadParams p) {
   const int lane = threadIdx.x & 31;
   const int lpr = 1 << p.lanes_log2, sub = lane >> p.lanes_log2, per = 32 >> p.lanes_log2, s = lane & (lpr - 1);
-  const int dim = static_cast<int>(p.c.dim), heads = static_cast<int>(p.c.heads);
+  const int dim = static_cast<int>(p.c.dim), heads = static_cast<int>(p.heads.d);
   const bool on = s < p.slots_per_row, has_b = s * 16 + 8 < dim;
   const bool val = blockIdx.y;
-  const char* base = static_cast<const char*>(val ? p.c.v : p.c.k);
-  const float* scales = val ? p.c.v_scale : p.c.k_scale;
-  T* out = static_cast<T*>(p.out[val]);
   constexpr int BATCH = 4, ES = CD == TJ_I8 || CD == TJ_E4M3 ? 1 : 2;
+  const char* base = static_cast<const char*>(val ? p.c.v : p.c.k) + s * 16 * ES;
+  const float* scales = val ? p.c.v_scale : p.c.k_scale;
+  T* out = static_cast<T*>(p.out[val]) + s * 16;
   const bool wide = ES == 2 || (dim % 16 == 0 && (p.c.page_stride | p.c.slot_stride | p.c.head_stride) % 16 == 0);
-  const long first = (static_cast<long>(blockIdx.x) * 4 + (threadIdx.x >> 5)) * p.batch * per + sub;
-  uint4 raw[BATCH][2];
-  float scale[BATCH];
+  const int step = BATCH * per, capacity = static_cast<int>(p.c.pages * p.c.page_size);
+  int first = (static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 5)) * p.batches * step + sub;
+  int slot[BATCH], head[BATCH];
+  auto look_up = [&](int from) {
 #pragma unroll
-  for (int j = 0; j < BATCH; ++j) {
-    const long r = first + static_cast<long>(j) * per;
-    raw[j][0] = raw[j][1] = make_uint4(0, 0, 0, 0);
-    scale[j] = 1.0f;
-    if (j >= p.batch || r >= p.rows) continue;
-    const long n = r / heads;
-    const int h = static_cast<int>(r - n * heads), slot = p.slots[n];
-    if (slot < 0) continue;
-    if (slot >= p.c.pages * p.c.page_size) {
-      if (s == 0) tj_report(p.status, TJ_STATUS_BOUNDS, OP_CACHE_READ * 16 + SITE_SLOT);
-      continue;
-    }
-    const int page = slot / static_cast<int>(p.c.page_size), at = slot - page * static_cast<int>(p.c.page_size);
-    const char* src = base + (page * p.c.page_stride + at * p.c.slot_stride + h * p.c.head_stride + s * 16) * ES;
-    if (on) {
-      if (ES == 2) {
-        raw[j][0] = tj_ld16_stream(src);
-        if (has_b) raw[j][1] = tj_ld16_stream(src + 16);
-      } else if (wide) {
-        raw[j][0] = tj_ld16_stream(src);
-      } else {
-        const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
-        uint2 w2 = make_uint2(0, 0);
-        if (has_b) w2 = __ldg(reinterpret_cast<const uint2*>(src + 8));
-        raw[j][0] = make_uint4(w.x, w.y, w2.x, w2.y);
+    for (int j = 0; j < BATCH; ++j) {
+      const int r = from + j * per;
+      slot[j] = -1;
+      if (r < p.rows) {
+        const int n = p.heads(r);
+        head[j] = r - n * heads;
+        slot[j] = __ldg(p.slots + n);
       }
     }
-    if (ES == 1) scale[j] = scales[page * p.c.scale_page + at * p.c.scale_slot + h * p.c.scale_head];
-  }
+  };
+  look_up(first);
+  for (int b = 0; b < p.batches && first - sub < p.rows; ++b, first += step) {
+    uint4 raw[BATCH][ES];
+    float scale[BATCH];
 #pragma unroll
-  for (int j = 0; j < BATCH; ++j) {
-    const long r = first + static_cast<long>(j) * per;
-    if (j >= p.batch || r >= p.rows || !on) continue;
-    float x[16];
-    if constexpr (CD == TJ_BF16) {
-      tj_unpack(raw[j][0], x, (const __nv_bfloat16*)nullptr);
-      tj_unpack(raw[j][1], x + 8, (const __nv_bfloat16*)nullptr);
-    } else if constexpr (CD == TJ_F16) {
-      tj_unpack(raw[j][0], x, (const __half*)nullptr);
-      tj_unpack(raw[j][1], x + 8, (const __half*)nullptr);
-    } else {
-      const uint32_t w[4] = {raw[j][0].x, raw[j][0].y, raw[j][0].z, raw[j][0].w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if constexpr (CD == TJ_I8) {
-#pragma unroll
-          for (int b = 0; b < 4; ++b) x[4 * i + b] = static_cast<float>(static_cast<int8_t>(w[i] >> (8 * b)));
+    for (int j = 0; j < BATCH; ++j) {
+      raw[j][0] = raw[j][ES - 1] = make_uint4(0, 0, 0, 0);
+      scale[j] = 1.0f;
+      if (slot[j] < 0) continue;
+      if (slot[j] >= capacity) {
+        if (s == 0) tj_report(p.status, TJ_STATUS_BOUNDS, OP_CACHE_READ * 16 + SITE_SLOT);
+        continue;
+      }
+      const int page = p.page(slot[j]), at = slot[j] - page * static_cast<int>(p.page.d);
+      const char* src = base + (page * p.c.page_stride + at * p.c.slot_stride + head[j] * p.c.head_stride) * ES;
+      if (on) {
+        if (ES == 2) {
+          raw[j][0] = tj_ld16_stream(src);
+          if (has_b) raw[j][ES - 1] = tj_ld16_stream(src + 16);
+        } else if (wide) {
+          raw[j][0] = tj_ld16_stream(src);
         } else {
-          __nv_fp8x4_e4m3 q;
-          q.__x = w[i];
-          const float4 f = static_cast<float4>(q);
-          x[4 * i] = f.x;
-          x[4 * i + 1] = f.y;
-          x[4 * i + 2] = f.z;
-          x[4 * i + 3] = f.w;
+          const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
+          uint2 w2 = make_uint2(0, 0);
+          if (has_b) w2 = __ldg(reinterpret_cast<const uint2*>(src + 8));
+          raw[j][0] = make_uint4(w.x, w.y, w2.x, w2.y);
         }
       }
-#pragma unroll
-      for (int i = 0; i < 16; ++i) x[i] *= scale[j];
+      if (ES == 1) scale[j] = __ldg(scales + page * p.c.scale_page + at * p.c.scale_slot + head[j] * p.c.scale_head);
     }
-    T* dst = out + r * dim + s * 16;
-    store8(dst, x);
-    if (has_b) store8(dst + 8, x + 8);
+    if (b + 1 < p.batches) look_up(first + step);
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      const int r = first + j * per;
+      if (r >= p.rows || !on) continue;
+      float x[16];
+      if constexpr (CD == TJ_BF16) {
+        tj_unpack(raw[j][0], x, (const __nv_bfloat16*)nullptr);
+        tj_unpack(raw[j][ES - 1], x + 8, (const __nv_bfloat16*)nullptr);
+      } else if constexpr (CD == TJ_F16) {
+        tj_unpack(raw[j][0], x, (const __half*)nullptr);
+        tj_unpack(raw[j][ES - 1], x + 8, (const __half*)nullptr);
+      } else {
+        const uint32_t w[4] = {raw[j][0].x, raw[j][0].y, raw[j][0].z, raw[j][0].w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if constexpr (CD == TJ_I8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * i + e] = static_cast<float>(static_cast<int8_t>(w[i] >> (8 * e)));
+          } else {
+            __nv_fp8x4_e4m3 q;
+            q.__x = w[i];
+            const float4 f = static_cast<float4>(q);
+            x[4 * i] = f.x;
+            x[4 * i + 1] = f.y;
+            x[4 * i + 2] = f.z;
+            x[4 * i + 3] = f.w;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] *= scale[j];
+      }
+      T* dst = out + static_cast<long>(r) * dim;
+      store8(dst, x);
+      if (has_b) store8(dst + 8, x + 8);
+    }
   }
 }
 
@@ -421,12 +448,23 @@ const char* rows_fault(const tj_rows& a, bool write) {
   return nullptr;
 }
 
-template <class T> void launch_rows(const RowsParams& p, int mode, unsigned grid, cudaStream_t st) {
+template <class T, int ROT> void launch_cache(const RowsParams& p, bool write, unsigned grid, cudaStream_t st) {
+  if (!write) {
+    if constexpr (ROT != 0) rows_kernel<T, ROT, 0><<<grid, 128, 0, st>>>(p);
+  } else if (p.a.cache.dtype == TJ_I8) {
+    rows_kernel<T, ROT, 2><<<grid, 128, 0, st>>>(p);
+  } else if (p.a.cache.dtype == TJ_E4M3) {
+    rows_kernel<T, ROT, 3><<<grid, 128, 0, st>>>(p);
+  } else {
+    rows_kernel<T, ROT, 1><<<grid, 128, 0, st>>>(p);
+  }
+}
+template <class T> void launch_rows(const RowsParams& p, int mode, bool write, unsigned grid, cudaStream_t st) {
   switch (mode) {
-    case 0: rows_kernel<T, 0><<<grid, 128, 0, st>>>(p); break;
-    case 1: rows_kernel<T, 1><<<grid, 128, 0, st>>>(p); break;
-    case 2: rows_kernel<T, 2><<<grid, 128, 0, st>>>(p); break;
-    default: rows_kernel<T, 3><<<grid, 128, 0, st>>>(p); break;
+    case 0: launch_cache<T, 0>(p, write, grid, st); break;
+    case 1: launch_cache<T, 1>(p, write, grid, st); break;
+    case 2: launch_cache<T, 2>(p, write, grid, st); break;
+    default: launch_cache<T, 3>(p, write, grid, st); break;
   }
 }
 
@@ -452,16 +490,18 @@ int run_rows(const char* name, int op, const tj_rows* a, bool write, void* strea
   // four iterations a warp (their loads in flight together); with few tokens one each, so that
   // the rows of a single-token step spread over the multiprocessors
   const bool few = a->tokens * p.iters < 16L * dev.sms;
-  p.segs = few ? p.iters : (p.iters + 3) / 4;
-  const long warps = a->tokens * p.segs, grid = (warps + 3) / 4;
-  if (grid > 0x7fffffffL) return refuse(TJ_ERR_INVALID, name, "too many rows");
+  const int segs = few ? p.iters : (p.iters + 3) / 4;
+  p.segs = Div(static_cast<uint32_t>(segs));
+  p.page = Div(write ? static_cast<uint32_t>(a->cache.page_size) : 1u);
+  const long warps = a->tokens * segs, grid = (warps + 3) / 4;
+  if (warps > 0x7fffff00L) return refuse(TJ_ERR_INVALID, name, "too many rows");
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (a->dtype == TJ_F32)
-    launch_rows<float>(p, mode, static_cast<unsigned>(grid), st);
+    launch_rows<float>(p, mode, write, static_cast<unsigned>(grid), st);
   else if (a->dtype == TJ_F16)
-    launch_rows<__half>(p, mode, static_cast<unsigned>(grid), st);
+    launch_rows<__half>(p, mode, write, static_cast<unsigned>(grid), st);
   else
-    launch_rows<__nv_bfloat16>(p, mode, static_cast<unsigned>(grid), st);
+    launch_rows<__nv_bfloat16>(p, mode, write, static_cast<unsigned>(grid), st);
   return launched(name);
 }
 
@@ -503,15 +543,18 @@ extern "C" int tj_b200_cache_read(const tj_kv_cache* cache, const int32_t* slots
   p.slots = slots;
   p.out[0] = k_out;
   p.out[1] = v_out;
-  p.rows = count * cache->heads;
+  if (count > 0x7fff0000LL / cache->heads) return refuse(TJ_ERR_INVALID, name, "too many rows");
+  p.rows = static_cast<int>(count * cache->heads);
+  p.heads = Div(static_cast<uint32_t>(cache->heads));
+  p.page = Div(static_cast<uint32_t>(cache->page_size));
   p.status = dev.status;
   p.slots_per_row = static_cast<int>((cache->dim + 15) / 16);
   p.lanes_log2 = 0;
   while ((1 << p.lanes_log2) < p.slots_per_row) ++p.lanes_log2;
-  const int per = 32 >> p.lanes_log2;
-  p.batch = p.rows < 32L * per * dev.sms ? 1 : 4;
-  const long grid = (p.rows + 4L * per * p.batch - 1) / (4L * per * p.batch);
-  if (grid > 0x7fffffffL) return refuse(TJ_ERR_INVALID, name, "too many rows");
+  // four groups of rows a batch, and batches until the warps are one wave of 32 an SM
+  const long step = 4L * (32 >> p.lanes_log2), warps_wanted = 32L * dev.sms / 2;
+  p.batches = static_cast<int>(std::max(1L, std::min(16L, (p.rows + step * warps_wanted - 1) / (step * warps_wanted))));
+  const long grid = (p.rows + 4 * step * p.batches - 1) / (4 * step * p.batches);
   const dim3 g(static_cast<unsigned>(grid), 2);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == TJ_F32)

@@ -66,4 +66,16 @@ inline const char* cache_fault(const tj_kv_cache& c) {
   return nullptr;
 }
 
+// n / d for 0 <= n < 2^31 by a multiplication.
+struct Div {
+  uint32_t mul, shift, d;
+  Div() = default;
+  explicit Div(uint32_t by) : d(by) {
+    shift = 0;
+    while ((1ull << shift) < by) ++shift;
+    mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << shift) - by)) / by + 1);
+  }
+  TJ_DEV int operator()(int n) const { return static_cast<int>((__umulhi(mul, static_cast<uint32_t>(n)) + static_cast<uint32_t>(n)) >> shift); }
+};
+
 }  // namespace tjs
