@@ -16,10 +16,12 @@
 //
 // Layout.  A row is cut into slots of two 8-element units; a lane holds one slot, so a rotary
 // pair (half layout: units u and u + rot / 16) is in one lane's registers, max|x| is a shuffle
-// over the row's lanes, and every access is 16 bytes.  A lane keeps its slot's cosines and sines
+// over the row's lanes, and every access is 16 bytes.  Neighbouring lanes hold neighbouring units.  A lane keeps its slot's cosines and sines
 // in registers over the heads of its token: the table is read once per token, not once per row.
-// A warp takes 32 / lanes rows at a time and loads four such groups, unconverted, before it turns the first:
-// the kernel is bound by HBM, and so by the reads in flight.
+// A warp takes 32 / lanes rows at a time and loads four such groups, unconverted, before it looks anything
+// up: the kernel is bound by HBM, and so by the reads in flight.  Measured for 16384 tokens of 40 f16
+// heads of 128 (us): four groups and 24 warps an SM 69, four and 20 72, two and 32 73, one and 32 86; with four
+// more groups in flight while these are stored, which leaves registers for 12 warps, 71.
 #include <algorithm>
 
 #include "serving_common.cuh"
@@ -82,7 +84,7 @@ TJ_DEV uint32_t i8x4(const float* f) {
 // (pairs that cross units: partners and table entries one by one).
 // CACHE: 0 none, 1 a 16-bit one, 2 i8, 3 e4m3.
 template <class T, int ROT, int CACHE>
-__global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ RowsParams p) {
+__global__ void __launch_bounds__(128, ROT == 3 ? 2 : 6) rows_kernel(const __grid_constant__ RowsParams p) {
   const tj_rows& a = p.a;
   const int lane = threadIdx.x & 31, wid = static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 5);
   const int token = p.segs(wid), seg = wid - token * static_cast<int>(p.segs.d);
@@ -92,16 +94,11 @@ __global__ void __launch_bounds__(128) rows_kernel(const __grid_constant__ RowsP
   const bool on = s < p.slots;
 
   // the slot's two units
-  int ua = 2 * s, ub = 2 * s + 1;
+  int ua = s, ub = s + p.slots;
   if (ROT == 1) {
     const int pairs = rot >> 4;
-    if (s < pairs) {
-      ua = s;
-      ub = s + pairs;
-    } else {
-      ua = 2 * pairs + 2 * (s - pairs);
-      ub = ua + 1;
-    }
+    ua = s < pairs ? s : s + pairs;
+    ub = s < pairs ? s + pairs : s + p.slots;
   }
   const bool has_b = on && ub * 8 < dim;
 
@@ -289,106 +286,75 @@ struct ReadParams {
   void* out[2];
   int rows;  // n * heads
   int* status;
-  int lanes_log2, slots_per_row, batches;
+  int lanes_log2;  // lanes of a row: a lane holds 8 elements (64: two rounds of a warp)
+  int group;       // rows of a warp, 32 at the most
   Div heads, page;
 };
 
 // Rows (slot, head) of the keys and of the values back as T: value = code * scale in f32, rounded
-// once.  CD: the cache's dtype.  A slot of -1 reads as zeros.  A warp goes through `batches` groups of rows
-// and looks a group's slots up while it reads the one before: the rows' addresses hang on them, and
-// with both in one go there was a second latency with nothing in flight (4000 GB/s).
+// once.  CD: the cache's dtype.  A slot of -1 reads as zeros.  A lane holds eight elements, so that both
+// its reads and its writes are contiguous with its neighbours'.  Where a row is takes more instructions than
+// converting eight elements, so each lane looks one row of the warp's up and hands its address round.
 template <class T, int CD>
 __global__ void __launch_bounds__(128) read_kernel(const __grid_constant__ ReadParams p) {
-  const int lane = threadIdx.x & 31;
-  const int lpr = 1 << p.lanes_log2, sub = lane >> p.lanes_log2, per = 32 >> p.lanes_log2, s = lane & (lpr - 1);
-  const int dim = static_cast<int>(p.c.dim), heads = static_cast<int>(p.heads.d);
-  const bool on = s < p.slots_per_row, has_b = s * 16 + 8 < dim;
-  const bool val = blockIdx.y;
   constexpr int BATCH = 4, ES = CD == TJ_I8 || CD == TJ_E4M3 ? 1 : 2;
-  const char* base = static_cast<const char*>(val ? p.c.v : p.c.k) + s * 16 * ES;
-  const float* scales = val ? p.c.v_scale : p.c.k_scale;
-  T* out = static_cast<T*>(p.out[val]) + s * 16;
-  const bool wide = ES == 2 || (dim % 16 == 0 && (p.c.page_stride | p.c.slot_stride | p.c.head_stride) % 16 == 0);
-  const int step = BATCH * per, capacity = static_cast<int>(p.c.pages * p.c.page_size);
-  int first = (static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 5)) * p.batches * step + sub;
-  int slot[BATCH], head[BATCH];
-  auto look_up = [&](int from) {
-#pragma unroll
-    for (int j = 0; j < BATCH; ++j) {
-      const int r = from + j * per;
-      slot[j] = -1;
-      if (r < p.rows) {
-        const int n = p.heads(r);
-        head[j] = r - n * heads;
-        slot[j] = __ldg(p.slots + n);
-      }
+  using Raw = typename std::conditional<ES == 1, uint2, uint4>::type;
+  const int lane = threadIdx.x & 31, dim = static_cast<int>(p.c.dim);
+  const int lanes = min(p.lanes_log2, 5), sub = lane >> lanes, per = 32 >> lanes, s0 = lane & ((1 << lanes) - 1);
+  const bool val = blockIdx.y;
+  T* const out = static_cast<T*>(p.out[val]);
+  const int first = (static_cast<int>(blockIdx.x) * 4 + (threadIdx.x >> 5)) * p.group, n = min(p.group, p.rows - first);
+  if (n <= 0) return;
+
+  long address = 0;  // 0: zeros
+  float scale = 1.0f;
+  if (lane < n) {
+    const int token = p.heads(first + lane), head = first + lane - token * static_cast<int>(p.heads.d), slot = __ldg(p.slots + token);
+    if (slot >= static_cast<int>(p.c.pages * p.c.page_size)) {
+      tj_report(p.status, TJ_STATUS_BOUNDS, OP_CACHE_READ * 16 + SITE_SLOT);
+    } else if (slot >= 0) {
+      const int page = p.page(slot), at = slot - page * static_cast<int>(p.page.d);
+      address = reinterpret_cast<long>(val ? p.c.v : p.c.k) + (page * p.c.page_stride + at * p.c.slot_stride + head * p.c.head_stride) * ES;
+      if (ES == 1) scale = __ldg((val ? p.c.v_scale : p.c.k_scale) + page * p.c.scale_page + at * p.c.scale_slot + head * p.c.scale_head);
     }
-  };
-  look_up(first);
-  for (int b = 0; b < p.batches && first - sub < p.rows; ++b, first += step) {
-    uint4 raw[BATCH][ES];
-    float scale[BATCH];
+  }
+  for (int s = s0; s < (1 << p.lanes_log2); s += 32) {
+    const bool on = s * 8 < dim;
+    for (int from = 0; from < n; from += BATCH * per) {
+      Raw raw[BATCH];
+      float factor[BATCH];
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j) {
-      raw[j][0] = raw[j][ES - 1] = make_uint4(0, 0, 0, 0);
-      scale[j] = 1.0f;
-      if (slot[j] < 0) continue;
-      if (slot[j] >= capacity) {
-        if (s == 0) tj_report(p.status, TJ_STATUS_BOUNDS, OP_CACHE_READ * 16 + SITE_SLOT);
-        continue;
+      for (int j = 0; j < BATCH; ++j) {
+        const int r = min(from + j * per + sub, 31);
+        const long src = __shfl_sync(0xffffffffu, address, r);
+        factor[j] = __shfl_sync(0xffffffffu, scale, r);
+        raw[j] = Raw{};
+        if (src && on && from + j * per + sub < n) raw[j] = __ldg(reinterpret_cast<const Raw*>(src + s * 8 * ES));
       }
-      const int page = p.page(slot[j]), at = slot[j] - page * static_cast<int>(p.page.d);
-      const char* src = base + (page * p.c.page_stride + at * p.c.slot_stride + head[j] * p.c.head_stride) * ES;
-      if (on) {
-        if (ES == 2) {
-          raw[j][0] = tj_ld16_stream(src);
-          if (has_b) raw[j][ES - 1] = tj_ld16_stream(src + 16);
-        } else if (wide) {
-          raw[j][0] = tj_ld16_stream(src);
+#pragma unroll
+      for (int j = 0; j < BATCH; ++j) {
+        const int r = from + j * per + sub;
+        if (r >= n || !on) continue;
+        float x[8];
+        if constexpr (CD == TJ_BF16) {
+          tj_unpack(raw[j], x, (const __nv_bfloat16*)nullptr);
+        } else if constexpr (CD == TJ_F16) {
+          tj_unpack(raw[j], x, (const __half*)nullptr);
         } else {
-          const uint2 w = __ldg(reinterpret_cast<const uint2*>(src));
-          uint2 w2 = make_uint2(0, 0);
-          if (has_b) w2 = __ldg(reinterpret_cast<const uint2*>(src + 8));
-          raw[j][0] = make_uint4(w.x, w.y, w2.x, w2.y);
-        }
-      }
-      if (ES == 1) scale[j] = __ldg(scales + page * p.c.scale_page + at * p.c.scale_slot + head[j] * p.c.scale_head);
-    }
-    if (b + 1 < p.batches) look_up(first + step);
+          const uint32_t w[2] = {raw[j].x, raw[j].y};
 #pragma unroll
-    for (int j = 0; j < BATCH; ++j) {
-      const int r = first + j * per;
-      if (r >= p.rows || !on) continue;
-      float x[16];
-      if constexpr (CD == TJ_BF16) {
-        tj_unpack(raw[j][0], x, (const __nv_bfloat16*)nullptr);
-        tj_unpack(raw[j][ES - 1], x + 8, (const __nv_bfloat16*)nullptr);
-      } else if constexpr (CD == TJ_F16) {
-        tj_unpack(raw[j][0], x, (const __half*)nullptr);
-        tj_unpack(raw[j][ES - 1], x + 8, (const __half*)nullptr);
-      } else {
-        const uint32_t w[4] = {raw[j][0].x, raw[j][0].y, raw[j][0].z, raw[j][0].w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          if constexpr (CD == TJ_I8) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * i + e] = static_cast<float>(static_cast<int8_t>(w[i] >> (8 * e)));
-          } else {
-            __nv_fp8x4_e4m3 q;
-            q.__x = w[i];
-            const float4 f = static_cast<float4>(q);
-            x[4 * i] = f.x;
-            x[4 * i + 1] = f.y;
-            x[4 * i + 2] = f.z;
-            x[4 * i + 3] = f.w;
+          for (int i = 0; i < 2; ++i) {
+            uint32_t lo, hi;  // exact in f16
+            codes4<__half, CD>(w[i], lo, hi);
+            const float2 a = __half22float2(reinterpret_cast<const __half2&>(lo)), b = __half22float2(reinterpret_cast<const __half2&>(hi));
+            x[4 * i] = a.x * factor[j];
+            x[4 * i + 1] = a.y * factor[j];
+            x[4 * i + 2] = b.x * factor[j];
+            x[4 * i + 3] = b.y * factor[j];
           }
         }
-#pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] *= scale[j];
+        store8(out + static_cast<long>(first + r) * dim + s * 8, x);
       }
-      T* dst = out + static_cast<long>(r) * dim;
-      store8(dst, x);
-      if (has_b) store8(dst + 8, x + 8);
     }
   }
 }
@@ -487,8 +453,8 @@ int run_rows(const char* name, int op, const tj_rows* a, bool write, void* strea
   while ((1 << p.lanes_log2) < p.slots) ++p.lanes_log2;
   const int per = 32 >> p.lanes_log2;
   p.iters = static_cast<int>((rows + per - 1) / per);
-  // four iterations a warp (their loads in flight together); with few tokens one each, so that
-  // the rows of a single-token step spread over the multiprocessors
+  // four groups a warp; with few tokens one each, so that the rows of a single-token step spread over the
+  // multiprocessors
   const bool few = a->tokens * p.iters < 16L * dev.sms;
   const int segs = few ? p.iters : (p.iters + 3) / 4;
   p.segs = Div(static_cast<uint32_t>(segs));
@@ -548,13 +514,12 @@ extern "C" int tj_b200_cache_read(const tj_kv_cache* cache, const int32_t* slots
   p.heads = Div(static_cast<uint32_t>(cache->heads));
   p.page = Div(static_cast<uint32_t>(cache->page_size));
   p.status = dev.status;
-  p.slots_per_row = static_cast<int>((cache->dim + 15) / 16);
   p.lanes_log2 = 0;
-  while ((1 << p.lanes_log2) < p.slots_per_row) ++p.lanes_log2;
-  // four groups of rows a batch, and batches until the warps are one wave of 32 an SM
-  const long step = 4L * (32 >> p.lanes_log2), warps_wanted = 32L * dev.sms / 2;
-  p.batches = static_cast<int>(std::max(1L, std::min(16L, (p.rows + step * warps_wanted - 1) / (step * warps_wanted))));
-  const long grid = (p.rows + 4 * step * p.batches - 1) / (4 * step * p.batches);
+  while ((8 << p.lanes_log2) < cache->dim) ++p.lanes_log2;
+  // 32 rows a warp; with few rows what a warp has in flight at once, so that they spread
+  const long at_once = 4L * std::max(1, 32 >> p.lanes_log2);
+  p.group = static_cast<int>(p.rows >= 32L * 16 * dev.sms ? 32 : std::min(32L, at_once));
+  const long grid = (p.rows + 4L * p.group - 1) / (4L * p.group);
   const dim3 g(static_cast<unsigned>(grid), 2);
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (dtype == TJ_F32)

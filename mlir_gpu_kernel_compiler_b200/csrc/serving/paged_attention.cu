@@ -1,4 +1,6 @@
 // Host side of the attention over a paged cache: checks, the choice of kernel, the launch.
+#include <algorithm>
+
 #include "paged_attention_rows.cuh"
 #include "paged_attention_tiles.cuh"
 
@@ -32,7 +34,12 @@ const char* attention_fault(const tj_paged_attention& a) {
 Plan plan(const tj_paged_attention& a, const Device& dev) {
   Plan p;
   const long group = a.q_heads / a.cache.heads;
-  p.tiles = a.max_new * group > 16;
+#ifndef TJS_LIMIT
+#define TJS_LIMIT 500000
+#endif
+  const long row_tiles = a.q_starts ? a.tokens * group / 16 + a.batch : a.batch * ((group + 15) / 16);
+  const long reach = a.table_width * a.cache.page_size, keys = a.window > 0 ? std::min<long>(reach, a.window + a.max_new) : reach;
+  p.tiles = a.max_new * group > 16 && row_tiles * a.cache.heads * keys * a.cache.dim / 128 > TJS_LIMIT;
   if (p.tiles) {
     p.rows = TILE_ROWS;
     p.grid = dev.sms;
@@ -42,7 +49,7 @@ Plan plan(const tj_paged_attention& a, const Device& dev) {
     return p;
   }
   p.rows = 16;
-  const long tiles = a.q_starts ? a.tokens * group / 16 + a.batch : a.batch * ((group + 15) / 16);
+  const long tiles = row_tiles;
   // Few row tiles are cut so that all pieces run at once, one CTA an SM (pieces: at most target + tiles).
   // Many uneven ones are cut for three waves of smaller CTAs, which even out what one wave does not.
   const bool q8 = a.cache.dtype == TJ_I8 || a.cache.dtype == TJ_E4M3;

@@ -13,8 +13,6 @@
 // P = 2^(t - m) with m the running maximum of t, and the sum adds P / vs.  So P, rounded to 16 bits
 // for the product with the codes, is at most 1 whatever the scales are.
 #pragma once
-#include <type_traits>
-
 #include "serving_common.cuh"
 
 namespace tjs {
@@ -136,54 +134,6 @@ TJ_DEV float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-
-// Two codes, each in one byte of a 16-bit half of `w` (the low byte for i8, the high one for e4m3;
-// the other byte is anything), as two exact 16-bit floats.
-template <class T, int CD> struct Codes;
-// i8 -> bf16: 0x4300 | low 7 bits is 128 + them; less 128, or 256 where the sign bit is set
-template <> struct Codes<__nv_bfloat16, TJ_I8> {
-  static TJ_DEV uint32_t make(uint32_t w) {
-    const uint32_t x = (w & 0x007f007fu) | 0x43004300u, y = (w & 0x00800080u) | 0x43004300u;
-    const __nv_bfloat162 d = __hsub2(reinterpret_cast<const __nv_bfloat162&>(x), reinterpret_cast<const __nv_bfloat162&>(y));
-    return reinterpret_cast<const uint32_t&>(d);
-  }
-};
-// i8 -> f16: 0x6400 | (code + 128) is 1024 + that
-template <> struct Codes<__half, TJ_I8> {
-  static TJ_DEV uint32_t less(uint32_t x) {
-    const uint32_t y = 0x64806480u;
-    const __half2 d = __hsub2(reinterpret_cast<const __half2&>(x), reinterpret_cast<const __half2&>(y));
-    return reinterpret_cast<const uint32_t&>(d);
-  }
-  static TJ_DEV uint32_t make(uint32_t w) { return less((w & 0x00ff00ffu) ^ 0x64806480u); }
-};
-// e4m3 -> bf16: the code's exponent and mantissa in place, then 2^(127 - 7) for the bias
-template <> struct Codes<__nv_bfloat16, TJ_E4M3> {
-  static TJ_DEV uint32_t make(uint32_t w) {
-    const uint32_t x = (w & 0x80008000u) | ((w & 0x7f007f00u) >> 4), k = 0x7b807b80u;
-    const __nv_bfloat162 d = __hmul2(reinterpret_cast<const __nv_bfloat162&>(x), reinterpret_cast<const __nv_bfloat162&>(k));
-    return reinterpret_cast<const uint32_t&>(d);
-  }
-};
-template <> struct Codes<__half, TJ_E4M3> {  // 2^(15 - 7)
-  static TJ_DEV uint32_t make(uint32_t w) {
-    const uint32_t x = (w & 0x80008000u) | ((w & 0x7f007f00u) >> 1), k = 0x5c005c00u;
-    const __half2 d = __hmul2(reinterpret_cast<const __half2&>(x), reinterpret_cast<const __half2&>(k));
-    return reinterpret_cast<const uint32_t&>(d);
-  }
-};
-
-// The four codes of a word, in order, as two words of 16-bit floats.
-template <class T, int CD> TJ_DEV void codes4(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  if constexpr (CD == TJ_I8 && std::is_same<T, __half>::value) {
-    w ^= 0x80808080u;
-    lo = Codes<T, CD>::less(__byte_perm(w, 0x64646464u, 0x4140));
-    hi = Codes<T, CD>::less(__byte_perm(w, 0x64646464u, 0x4342));
-  } else {
-    lo = Codes<T, CD>::make(__byte_perm(w, 0, CD == TJ_I8 ? 0x4140 : 0x1404));
-    hi = Codes<T, CD>::make(__byte_perm(w, 0, CD == TJ_I8 ? 0x4342 : 0x3424));
-  }
 }
 
 // P is made 2^shift times as large before it is rounded to 16 bits, and so is the sum: f16 has no

@@ -6,6 +6,7 @@
 
 #include <cstdio>
 #include <mutex>
+#include <type_traits>
 
 #include "../../../include/tj_b200.h"
 #include "../kernels/tj_common.cuh"
@@ -64,6 +65,54 @@ inline const char* cache_fault(const tj_kv_cache& c) {
       c.slot_stride * es % unit || c.head_stride * es % unit)
     return "cache rows must start on 16-byte (8-bit caches: 8-byte) boundaries";
   return nullptr;
+}
+
+// Two codes, each in one byte of a 16-bit half of `w` (the low byte for i8, the high one for e4m3;
+// the other byte is anything), as two exact 16-bit floats.
+template <class T, int CD> struct Codes;
+// i8 -> bf16: 0x4300 | low 7 bits is 128 + them; less 128, or 256 where the sign bit is set
+template <> struct Codes<__nv_bfloat16, TJ_I8> {
+  static TJ_DEV uint32_t make(uint32_t w) {
+    const uint32_t x = (w & 0x007f007fu) | 0x43004300u, y = (w & 0x00800080u) | 0x43004300u;
+    const __nv_bfloat162 d = __hsub2(reinterpret_cast<const __nv_bfloat162&>(x), reinterpret_cast<const __nv_bfloat162&>(y));
+    return reinterpret_cast<const uint32_t&>(d);
+  }
+};
+// i8 -> f16: 0x6400 | (code + 128) is 1024 + that
+template <> struct Codes<__half, TJ_I8> {
+  static TJ_DEV uint32_t less(uint32_t x) {
+    const uint32_t y = 0x64806480u;
+    const __half2 d = __hsub2(reinterpret_cast<const __half2&>(x), reinterpret_cast<const __half2&>(y));
+    return reinterpret_cast<const uint32_t&>(d);
+  }
+  static TJ_DEV uint32_t make(uint32_t w) { return less((w & 0x00ff00ffu) ^ 0x64806480u); }
+};
+// e4m3 -> bf16: the code's exponent and mantissa in place, then 2^(127 - 7) for the bias
+template <> struct Codes<__nv_bfloat16, TJ_E4M3> {
+  static TJ_DEV uint32_t make(uint32_t w) {
+    const uint32_t x = (w & 0x80008000u) | ((w & 0x7f007f00u) >> 4), k = 0x7b807b80u;
+    const __nv_bfloat162 d = __hmul2(reinterpret_cast<const __nv_bfloat162&>(x), reinterpret_cast<const __nv_bfloat162&>(k));
+    return reinterpret_cast<const uint32_t&>(d);
+  }
+};
+template <> struct Codes<__half, TJ_E4M3> {  // 2^(15 - 7)
+  static TJ_DEV uint32_t make(uint32_t w) {
+    const uint32_t x = (w & 0x80008000u) | ((w & 0x7f007f00u) >> 1), k = 0x5c005c00u;
+    const __half2 d = __hmul2(reinterpret_cast<const __half2&>(x), reinterpret_cast<const __half2&>(k));
+    return reinterpret_cast<const uint32_t&>(d);
+  }
+};
+
+// The four codes of a word, in order, as two words of 16-bit floats.
+template <class T, int CD> TJ_DEV void codes4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (CD == TJ_I8 && std::is_same<T, __half>::value) {
+    w ^= 0x80808080u;
+    lo = Codes<T, CD>::less(__byte_perm(w, 0x64646464u, 0x4140));
+    hi = Codes<T, CD>::less(__byte_perm(w, 0x64646464u, 0x4342));
+  } else {
+    lo = Codes<T, CD>::make(__byte_perm(w, 0, CD == TJ_I8 ? 0x4140 : 0x1404));
+    hi = Codes<T, CD>::make(__byte_perm(w, 0, CD == TJ_I8 ? 0x4342 : 0x3424));
+  }
 }
 
 // n / d for 0 <= n < 2^31 by a multiplication.
