@@ -34,29 +34,39 @@ const char* attention_fault(const tj_paged_attention& a) {
 Plan plan(const tj_paged_attention& a, const Device& dev) {
   Plan p;
   const long group = a.q_heads / a.cache.heads;
-#ifndef TJS_LIMIT
-#define TJS_LIMIT 500000
-#endif
-  const long row_tiles = a.q_starts ? a.tokens * group / 16 + a.batch : a.batch * ((group + 15) / 16);
-  const long reach = a.table_width * a.cache.page_size, keys = a.window > 0 ? std::min<long>(reach, a.window + a.max_new) : reach;
-  p.tiles = a.max_new * group > 16 && row_tiles * a.cache.heads * keys * a.cache.dim / 128 > TJS_LIMIT;
+  const bool q8 = a.cache.dtype == TJ_I8 || a.cache.dtype == TJ_E4M3;
+  // Sizes if every sequence has max_new tokens over 4096 keys, or a window's, as lengths are known to the
+  // device only: neither tokens of no sequence nor a table's width decide, so they change no bit either.
+  const long new_max = std::min(a.max_new, a.tokens), packed = new_max * group;
+  const double row_tiles = static_cast<double>(a.batch) * static_cast<double>((packed + 15) / 16);
+  // Tokens of one tile of 16 rows take the kernel of few rows.  More do while it passes over less: it reads
+  // the keys once for 16 rows, the other once for 256, but starts, joins and ends in 25 us more (16-bit
+  // caches) or 30 (8-bit ones, whose keys it also converts, at four times the cost).  Few rows against many, us:
+  //   16-bit, dim 128  1 x 16 tokens over 4096 23, 39   1 x 32 44, 46   1 x 64 62, 58   1 x 256 163, 64
+  //                    8 x 16 over 2048 69, 42          16 x 8 over 8192 165, 124      1 x 300 over 300 32, 57
+  //   8-bit, dim 128   1 x 32 over 4096 37, 55          1 x 64 56, 68   1 x 128 84, 68
+  //                    8 x 16 over 2048 57, 57          16 x 8 over 8192 132, 232
+  //   16-bit, dim 64   1 x 32 over 4096 25, 33          1 x 64 40, 42   1 x 128 59, 42
+  const double keys = a.window > 0 ? static_cast<double>(a.window) + new_max : 4096;
+  const double pass = a.cache.heads * keys * static_cast<double>(a.cache.dim + 64) / 192;
+  const double many_tiles = static_cast<double>(a.batch) * static_cast<double>((packed + TILE_ROWS - 1) / TILE_ROWS);
+  p.tiles = packed > 16 && row_tiles * pass > (q8 ? 500e3 + 3.6 * many_tiles * pass : 250e3 + many_tiles * pass);
   if (p.tiles) {
     p.rows = TILE_ROWS;
-    p.grid = dev.sms;
+    p.grid = std::min(dev.sms, MAX_PARTS);
     p.slots = 2 * p.grid;  // a CTA's first and last segment
     p.target = p.min_chunk = 0;
     p.wide = false;
     return p;
   }
   p.rows = 16;
-  const long tiles = row_tiles;
   // Few row tiles are cut so that all pieces run at once, one CTA an SM (pieces: at most target + tiles).
   // Many uneven ones are cut for three waves of smaller CTAs, which even out what one wave does not.
-  const bool q8 = a.cache.dtype == TJ_I8 || a.cache.dtype == TJ_E4M3;
-  const long items = a.cache.heads * tiles;
+  const double items = a.cache.heads * row_tiles;
   p.wide = items <= dev.sms / 2;
-  p.target = static_cast<int>(p.wide ? dev.sms - items : 3L * dev.sms * (q8 ? 3 : 2));
+  p.target = p.wide ? dev.sms - static_cast<int>(items) : 3 * dev.sms * (q8 ? 3 : 2);
   p.min_chunk = 256;
+  const long tiles = a.q_starts ? a.tokens * group / 16 + a.batch : a.batch * ((group + 15) / 16);  // at the most
   p.grid = a.cache.heads * (tiles + 1) + p.target;
   p.slots = p.grid;
   return p;
@@ -83,6 +93,7 @@ template <class T, int CD, int D> cudaError_t launch_dim(const AttnParams& p, co
     constexpr int smem = Tiles<T, CD, D>::SMEM;
     if (const cudaError_t e = allow(attention_tiles<T, CD, D>, smem, tiles_ready, dev)) return e;
     attention_tiles<T, CD, D><<<grid, 512, smem, st>>>(p);
+    join_tiles<T, CD, D><<<dim3(grid, TILE_ROWS / 32), 256, 0, st>>>(p);
   } else {
     return plan.wide ? launch_few<T, CD, D, true>(p, grid, dev, st) : launch_few<T, CD, D, false>(p, grid, dev, st);
   }
@@ -144,6 +155,7 @@ extern "C" int tj_b200_paged_attention(const tj_paged_attention* args, void* str
   for (int i = 0; i < 31; ++i)
     if (a.cache.page_size == (1LL << i)) p.page_shift = i;
   p.target = how.target;
+  p.tile_ctas = static_cast<int>(how.grid);
   p.min_chunk = how.min_chunk;
   p.part_o = static_cast<float*>(a.workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + how.slots * how.rows * a.cache.dim);

@@ -28,6 +28,7 @@ struct AttnParams {
   float* part_o;     // [grid][rows][dim] sums of P V, not yet divided
   float2* part_ml;   // [grid][rows] (maximum, sum)
   int* counters;     // [grid] chunks done, zero between calls
+  int tile_ctas;     // CTAs of the kernel of many rows
 };
 
 // log2 vs is held at this or above: a row of zeros has vs = 0

@@ -25,7 +25,8 @@
 //
 // The work, (tile, block) pairs of all sequences and heads in a row, is cut into as many equal parts as
 // there are SMs (each at least 512 keys): a CTA takes a tile's end, whole tiles and a tile's beginning.
-// Parts of one tile are joined by the CTA whose part comes last, in the tile's order.
+// Parts of one tile are joined, in the tile's order, by a second kernel on all SMs.  (By the CTA that
+// ends last, which then reads a part's 131 KB for each: 64 tokens over 4096 keys took 115 us.)
 //
 // Every wait is bounded (TJ_WAIT_NS): one that runs out raises the CTA's abort flag and the status word.
 #pragma once
@@ -38,7 +39,7 @@
 
 namespace tjs {
 
-constexpr int TILE_ROWS = 256, TILE_KEYS = 64;
+constexpr int TILE_ROWS = 256, TILE_KEYS = 64, MAX_PARTS = 1024;
 
 // The linear order of the work, in keys x group.  A tile weighs its keys, and one block more for what a
 // tile costs by itself.  Positions are cut without 64-bit divisions, which a lone warp takes
@@ -97,6 +98,12 @@ struct Cut {
     return pos < wide ? pos / (share + 1) : rest + (pos - wide) / share;
   }
 };
+// As many parts as CTAs, of 512 keys at the least.
+TJ_DEV Cut cut_work(const AttnParams& p, long total, int ctas) {
+  return Cut(total, min(static_cast<long>(ctas), max(1L, total / (512L * p.group))));
+}
+// blocks that a tile with the key range [lo, hi) goes through
+TJ_DEV int tile_key_blocks(int lo, int hi) { return max(1, (hi + TILE_KEYS - 1) / TILE_KEYS - lo / TILE_KEYS); }
 // How many of a tile's `blocks` key blocks lie before place `a` of its weight: roundings to nearest
 // keep the order, so neighbours that ask with the same place agree, and a = weight gives all.
 TJ_DEV int blocks_before(long a, long weight, int blocks) {
@@ -301,7 +308,6 @@ struct Segment {
   int key0, nb;     // first key and number of blocks of this segment (0: no segment)
   int all;          // blocks of the tile
   int later;        // the tile began in an earlier part
-  long start, weight;
 };
 
 // A CTA's shared memory.
@@ -314,8 +320,8 @@ template <class T, int CD, int D> struct TilesShared {
                             P_READY = S_FULL + 32,             // [2 tiles][2 buffers]
                             PV_DONE = P_READY + 32,            // [2 tiles][2 buffers]
                             SC_FULL = PV_DONE + 32,            // [SCALES], 8-bit caches
-                            DRAIN = SC_FULL + 8 * C::SCALES, SLOT = DRAIN + 16, ABORT = SLOT + 4, LAST = ABORT + 4,
-                            SEGMENT = (LAST + 4 + 15) / 16 * 16, END = SEGMENT + 2 * sizeof(Segment);
+                            DRAIN = SC_FULL + 8 * C::SCALES, SLOT = DRAIN + 16, ABORT = SLOT + 4,
+                            SEGMENT = (ABORT + 4 + 15) / 16 * 16, END = SEGMENT + 2 * sizeof(Segment);
   static_assert(END + 1024 <= C::SMEM, "shared memory");
   uint8_t* base;
   TJ_DEV explicit TilesShared(uint8_t* raw) {
@@ -326,11 +332,9 @@ template <class T, int CD, int D> struct TilesShared {
     return reinterpret_cast<float*>(base + SCALE) + (it % C::SCALES) * C::ARRAYS * TILE_KEYS;
   }
   TJ_DEV volatile int* abort_flag() const { return reinterpret_cast<volatile int*>(base + ABORT); }
-  TJ_DEV volatile int* last() const { return reinterpret_cast<volatile int*>(base + LAST); }
   TJ_DEV volatile uint32_t* tmem_slot() const { return reinterpret_cast<volatile uint32_t*>(base + SLOT); }
   // volatile: read where it is needed, not kept in registers over the blocks
   TJ_DEV volatile Segment& segment(int seg) const { return reinterpret_cast<volatile Segment*>(base + SEGMENT)[seg & 1]; }
-  TJ_DEV int* slots() const { return reinterpret_cast<int*>(base + K); }  // while the parts of a tile are joined
   // Several barriers at once: the polls, each some 140 clocks behind the softmax warps' exponentials, overlap.
   TJ_DEV bool wait3(uint32_t b0, int ph0, uint32_t b1, int ph1, uint32_t b2, int ph2, const AttnParams& p, int site) const {
     const bool x = tjg::mbar_try_wait(at(b0), ph0 & 1), y = tjg::mbar_try_wait(at(b1), ph1 & 1), z = tjg::mbar_try_wait(at(b2), ph2 & 1);
@@ -357,13 +361,11 @@ TJ_DEV void next_segment(const AttnParams& p, long& pos, long to, volatile Segme
     g.rows = min(TILE_ROWS, w.s.n * p.group - g.r0);
     key_range(p, w.s, g.r0 / p.group, (g.r0 + g.rows - 1) / p.group, g.lo, g.hi);
     const int first = g.lo / TILE_KEYS;
-    g.all = max(1, (g.hi + TILE_KEYS - 1) / TILE_KEYS - first);
+    g.all = tile_key_blocks(g.lo, g.hi);
     const int j0 = blocks_before(a0, w.weight, g.all);
     g.nb = blocks_before(a1, w.weight, g.all) - j0;
     g.key0 = (first + j0) * TILE_KEYS;
     g.later = a0 > 0;
-    g.start = w.start;
-    g.weight = w.weight;
   }
   if ((threadIdx.x & 31) == 0) {
     if (g.nb) {
@@ -379,8 +381,6 @@ TJ_DEV void next_segment(const AttnParams& p, long& pos, long to, volatile Segme
       out.key0 = g.key0;
       out.all = g.all;
       out.later = g.later;
-      out.start = g.start;
-      out.weight = g.weight;
     }
     out.nb = g.nb;
   }
@@ -393,69 +393,83 @@ TJ_DEV void row_of(const AttnParams& p, int head, int r, int& tok, int& hd) {
   hd = head * p.group + r - tok * p.group;
 }
 
-// The end of a segment, by every thread of the CTA: false if a wait ran out.  A tile in several parts is
-// joined, in the order of its parts, by the CTA that makes its blocks complete.
-template <class T, int CD, int D>
-TJ_DEV bool end_segment(const AttnParams& p, const TilesShared<T, CD, D>& sh, const Cut& cut, int seg) {
-  using C = Tiles<T, CD, D>;
-  volatile Segment& g = sh.segment(seg);
+// The end of a segment, by every thread of the CTA: false if a wait ran out.
+template <class T, int CD, int D> TJ_DEV bool end_segment(const TilesShared<T, CD, D>& sh) {
   __syncwarp();
-  const int nb = g.nb, all = g.all;
-  const bool whole = nb == all;
-  if (!whole) __threadfence();
   __syncthreads();
   tjg::tc_fence_after();
-  if (*sh.abort_flag()) return false;
-  if (whole) return true;
-  const long start = g.start, weight = g.weight;
-  const int c0 = static_cast<int>(cut.part_of(start)), n = static_cast<int>(cut.part_of(start + weight - 1)) - c0 + 1;
-  if (threadIdx.x == 0) {
-    const int done = atomicAdd(p.counters + c0, nb) + nb;
-    *sh.last() = done == all;
-    if (done == all) p.counters[c0] = 0;  // ready for the next call
-  }
-  // where each part of the tile was left (-1: it had no block); as many as CTAs at the most
-  if (threadIdx.x < n) {
-    const int c = c0 + threadIdx.x;
-    const long b0 = max(0L, cut.begin(c) - start), b1 = min(weight, cut.begin(c + 1) - start);
-    sh.slots()[threadIdx.x] = blocks_before(b0, weight, all) == blocks_before(b1, weight, all) ? -1 : 2 * c + (b0 > 0 ? 0 : 1);
+  return *sh.abort_flag() == 0;
+}
+
+// Joins the tiles that were cut: CTA (c, y) the rows 32 y .. 32 y + 31 of the tile that begins in part c and
+// goes on in part c + 1, if there is one.
+template <class T, int CD, int D> __global__ void __launch_bounds__(256) join_tiles(const __grid_constant__ AttnParams p) {
+  constexpr float SHIFT = Tiles<T, CD, D>::SHIFT;
+  __shared__ int s_slots[MAX_PARTS];
+  __shared__ int s_whole;
+  const long total = total_work(p);
+  if (total == 0) return;
+  const Cut cut = cut_work(p, total, p.tile_ctas);
+  const int c0 = blockIdx.x;
+  if (c0 + 1 >= cut.parts) return;
+  const long from = cut.begin(c0), to = cut.begin(c0 + 1);
+  const TilePart w = find_tile(p, to - 1);
+  if (w.start < from || w.start + w.weight <= to) return;
+  const int r0 = w.tile * TILE_ROWS, rows = min(TILE_ROWS, w.s.n * p.group - r0);
+  if (static_cast<int>(blockIdx.y) * 32 >= rows) return;
+  int lo, hi;
+  key_range(p, w.s, r0 / p.group, (r0 + rows - 1) / p.group, lo, hi);
+  const int all = tile_key_blocks(lo, hi), n = static_cast<int>(cut.part_of(w.start + w.weight - 1)) - c0 + 1;
+  if (threadIdx.x == 0) s_whole = 0;
+  __syncthreads();
+  // where each part was left (-1: it had no block)
+  for (int i = threadIdx.x; i < n; i += 256) {
+    const long b0 = max(0L, cut.begin(c0 + i) - w.start), b1 = min(w.weight, cut.begin(c0 + i + 1) - w.start);
+    const int blocks = blocks_before(b1, w.weight, all) - blocks_before(b0, w.weight, all);
+    s_slots[i] = blocks == 0 ? -1 : 2 * (c0 + i) + (i > 0 ? 0 : 1);
+    if (blocks == all) s_whole = 1;  // it fell to one part after all, which has stored it
   }
   __syncthreads();
-  if (*sh.last()) {
-    __threadfence();
-    const int r0 = g.r0, rows = g.rows, head = g.head, first_token = g.s.start;
-    constexpr int V4 = D / 4;
-    for (int e = threadIdx.x; e < rows * V4; e += 512) {
-      const int r = e / V4, col = (e - r * V4) * 4;
-      float best = -INFINITY, sum = 0.0f;
-      float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-      for (int c = 0; c < n; ++c) {
-        if (sh.slots()[c] < 0) continue;
-        const long slot = static_cast<long>(sh.slots()[c]) * TILE_ROWS + r;
-        const float2 ml = __ldcg(p.part_ml + slot);
-        if (ml.x == -INFINITY) continue;
-        const float next = fmaxf(best, ml.x), f = exp2_fast(best - next), k = exp2_fast(ml.x - next);
-        const float4 v = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot * D + col));
-        acc = make_float4(acc.x * f + v.x * k, acc.y * f + v.y * k, acc.z * f + v.z * k, acc.w * f + v.w * k);
-        sum = sum * f + ml.y * k;
+  if (s_whole) return;
+  constexpr int V4 = D / 4;
+  for (int e = threadIdx.x; e < 32 * V4; e += 256) {
+    const int r = blockIdx.y * 32 + e / V4, col = e % V4 * 4;
+    if (r >= rows) break;
+    float best = -INFINITY, sum = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    constexpr int GO = 4;  // parts whose loads are in flight together
+    for (int i = 0; i < n; i += GO) {
+      float2 ml[GO];
+      float4 v[GO];
+#pragma unroll
+      for (int k = 0; k < GO; ++k) {
+        const int at = i + k < n ? s_slots[i + k] : -1;
+        const long slot = static_cast<long>(max(at, 0)) * TILE_ROWS + r;
+        ml[k] = __ldcg(p.part_ml + slot);
+        v[k] = __ldcg(reinterpret_cast<const float4*>(p.part_o + slot * D + col));
+        if (at < 0) ml[k].x = -INFINITY;
+      }
+#pragma unroll
+      for (int k = 0; k < GO; ++k) {
+        if (ml[k].x == -INFINITY) continue;
+        const float next = fmaxf(best, ml[k].x), f = exp2_fast(best - next), g = exp2_fast(ml[k].x - next);
+        acc = make_float4(acc.x * f + v[k].x * g, acc.y * f + v[k].y * g, acc.z * f + v[k].z * g, acc.w * f + v[k].w * g);
+        sum = sum * f + ml[k].y * g;
         best = next;
       }
-      const bool none = best == -INFINITY;
-      const float inv = none ? 0.0f : 1.0f / sum;
-      int tok, hd;
-      row_of(p, head, r0 + r, tok, hd);
-      T* dst = static_cast<T*>(p.a.out) + (first_token + tok) * p.a.out_token + hd * p.a.out_head + col;
-      uint2 y;
-      y.x = pack2<T>(none ? 0.0f : acc.x * inv, none ? 0.0f : acc.y * inv);
-      y.y = pack2<T>(none ? 0.0f : acc.z * inv, none ? 0.0f : acc.w * inv);
-      *reinterpret_cast<uint2*>(dst) = y;
-      if (p.a.lse && col == 0)
-        p.a.lse[(first_token + tok) * p.a.q_heads + hd] = none ? -INFINITY : (best - C::SHIFT + log2f(sum)) * 0.69314718055994531f;
     }
-    __syncthreads();  // the slots lie where the next keys go
+    const bool none = best == -INFINITY;
+    const float inv = none ? 0.0f : 1.0f / sum;
+    int tok, hd;
+    row_of(p, w.head, r0 + r, tok, hd);
+    tok += w.s.start;
+    uint2 y;
+    y.x = pack2<T>(none ? 0.0f : acc.x * inv, none ? 0.0f : acc.y * inv);
+    y.y = pack2<T>(none ? 0.0f : acc.z * inv, none ? 0.0f : acc.w * inv);
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.a.out) + tok * p.a.out_token + hd * p.a.out_head + col) = y;
+    if (p.a.lse && col == 0)
+      p.a.lse[static_cast<long>(tok) * p.a.q_heads + hd] = none ? -INFINITY : (best - SHIFT + log2f(sum)) * 0.69314718055994531f;
   }
-  return true;
 }
 
 // ---- producers: the queries of a segment, then its keys and values block by block ------------------------------
@@ -826,8 +840,9 @@ __global__ void __launch_bounds__(512, 1) attention_tiles(const __grid_constant_
   const S sh(smem_raw);
   const int warp = threadIdx.x >> 5;
   const long total = total_work(p);
-  const Cut cut(total, min(static_cast<long>(gridDim.x), max(1L, total / (512L * p.group))));
-  if (total == 0 || blockIdx.x >= cut.parts) return;
+  if (total == 0) return;
+  const Cut cut = cut_work(p, total, gridDim.x);
+  if (blockIdx.x >= cut.parts) return;
   long pos = cut.begin(blockIdx.x);
   const long to = cut.begin(blockIdx.x + 1);
 
@@ -870,14 +885,14 @@ __global__ void __launch_bounds__(512, 1) attention_tiles(const __grid_constant_
       if (busy) softmax<T, CD, D>(p, sh, tmem, seg, blocks, tile_blocks);
       blocks += sh.segment(seg).nb;
       if (busy) tile_blocks += sh.segment(seg).nb;
-      if (!end_segment<T, CD, D>(p, sh, cut, seg)) break;
+      if (!end_segment(sh)) break;
     }
   } else if (warp < 12) {
     regs_dec<C::REGS_P>();
     for (int seg = 0; sh.segment(seg).nb; ++seg) {
       produce<T, CD, D>(p, sh, seg, blocks);
       blocks += sh.segment(seg).nb;
-      if (!end_segment<T, CD, D>(p, sh, cut, seg)) break;
+      if (!end_segment(sh)) break;
     }
   } else {
     regs_dec<C::REGS_M>();
@@ -888,7 +903,7 @@ __global__ void __launch_bounds__(512, 1) attention_tiles(const __grid_constant_
       if (warp == 14) next_segment(p, pos, to, sh.segment(seg + 1));
       blocks += sh.segment(seg).nb;
       if (busy) tile_blocks += sh.segment(seg).nb;
-      if (!end_segment<T, CD, D>(p, sh, cut, seg)) break;
+      if (!end_segment(sh)) break;
     }
   }
   __syncthreads();
