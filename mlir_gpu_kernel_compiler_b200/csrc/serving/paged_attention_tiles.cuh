@@ -159,6 +159,10 @@ TJ_DEV void cp_async16(uint32_t dst, const void* src, bool on) {
   const int bytes = on ? 16 : 0;  // 0: zeros
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
+TJ_DEV void cp_async4(uint32_t dst, const void* src, bool on) {
+  const int bytes = on ? 4 : 0;
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 TJ_DEV void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> TJ_DEV void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 // 16 columns of a warp's 32 lanes out of TMEM
@@ -241,12 +245,16 @@ template <class T, int CD, int D> struct Tiles {
   // thread reads these arrays for every block, so one fewer counts.
   static constexpr bool MUL_V = Q8 && BF, EXP_V = Q8 && !BF;
   static constexpr int ARRAYS = MUL_V ? 2 : EXP_V ? 3 : 0;
-  static constexpr int STAGES = D == 128 ? 4 : 8;
+  static constexpr int STAGES = D == 64 ? 8 : Q8 ? 3 : 4;
+  // 8-bit codes and scales wait in shared memory before they are converted, this many blocks of them
+  static constexpr int RAWS = Q8 ? 3 : 0;
+  static constexpr uint32_t RAW_SCALE = 2 * TILE_KEYS * D, RAW_BYTES = RAW_SCALE + 2 * TILE_KEYS * 4;
   // Scale rows outlive their block's operands: a tile's softmax is up to two blocks behind its scores.
   // Block j + SCALES takes over from block j when the scores of block j + 2 are made, which follow its P.
   static constexpr int SCALES = STAGES + 2;
   static constexpr uint32_t Q_BYTES = 128 * D * 2, KV_BYTES = TILE_KEYS * D * 2;
-  static constexpr int SMEM = 1024 + 2 * Q_BYTES + 2 * STAGES * KV_BYTES + SCALES * ARRAYS * TILE_KEYS * 4 + 768;
+  static constexpr int SMEM = 1024 + 2 * Q_BYTES + 2 * STAGES * KV_BYTES + SCALES * ARRAYS * TILE_KEYS * 4 + RAWS * RAW_BYTES + 768;
+  static_assert(SMEM <= 232448, "shared memory");
   // registers of a softmax, producer and other thread; at launch all have 128
   static constexpr int REGS_S = 152, REGS_P = 104, REGS_M = 104;
   static_assert(256 * REGS_S + 128 * REGS_P + 128 * REGS_M <= 512 * 128, "no more than the block was launched with");
@@ -314,7 +322,7 @@ struct Segment {
 template <class T, int CD, int D> struct TilesShared {
   using C = Tiles<T, CD, D>;
   static constexpr uint32_t Q = 0, K = Q + 2 * C::Q_BYTES, V = K + C::STAGES * C::KV_BYTES, SCALE = V + C::STAGES * C::KV_BYTES,
-                            BARS = SCALE + C::SCALES * C::ARRAYS * TILE_KEYS * 4, Q_FULL = BARS, K_FULL = Q_FULL + 8,
+                            RAW = SCALE + C::SCALES * C::ARRAYS * TILE_KEYS * 4, BARS = RAW + C::RAWS * C::RAW_BYTES, Q_FULL = BARS, K_FULL = Q_FULL + 8,
                             V_FULL = K_FULL + 8 * C::STAGES, K_EMPTY = V_FULL + 8 * C::STAGES, V_EMPTY = K_EMPTY + 8 * C::STAGES,
                             S_FULL = V_EMPTY + 8 * C::STAGES,  // [2 tiles][2 buffers]
                             P_READY = S_FULL + 32,             // [2 tiles][2 buffers]
@@ -558,30 +566,36 @@ TJ_DEV void produce(const AttnParams& p, const TilesShared<T, CD, D>& sh, int se
   } else {
     constexpr int LPR = D / 16, PER = 32 / LPR, N = 32 / PER;
     const int piece = lane % LPR;  // 16 codes: two pieces of the 16-bit row
-    uint4 raw[N];
-    float ks, vs;
-    auto load = [&]() {
+    // The codes are copied asynchronously two blocks ahead: each thread those that it will convert itself, so
+    // that only it has to wait for them.  (Loaded one block ahead into registers, a block took 3200 clocks.)
+    const uint32_t raw0 = S::RAW + (warp * N * 32 + lane) * 16, scale0 = S::RAW + C::RAW_SCALE + (row0 + lane) * 4;
+    auto load = [&](int j) {  // of block j, whose place is known; every call commits one group
+      const uint32_t slot = static_cast<uint32_t>(j % C::RAWS) * C::RAW_BYTES;
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         const long ro = __shfl_sync(0xffffffffu, off, i * PER + lane / LPR);
-        raw[i] = make_uint4(0, 0, 0, 0);
-        if (ro >= 0) raw[i] = tj_ld16_stream(base + ro + piece * 16);
+        if (j < nb) cp_async16(sh.at(raw0 + slot + i * 512), base + (ro < 0 ? 0 : ro) + piece * 16, ro >= 0);
       }
-      ks = vs = 0.0f;
-      if (keys && soff >= 0) {  // the keys' producers bring both scales
-        ks = __ldg(p.a.cache.k_scale + soff);
-        vs = __ldg(p.a.cache.v_scale + soff);
+      if (keys && j < nb) {  // the keys' producers bring both scales
+        cp_async4(sh.at(scale0 + slot), p.a.cache.k_scale + (soff < 0 ? 0 : soff), soff >= 0);
+        cp_async4(sh.at(scale0 + slot + TILE_KEYS * 4), p.a.cache.v_scale + (soff < 0 ? 0 : soff), soff >= 0);
       }
+      cp_async_commit();
+      place(j + 1, next_page);
+      next_page = page_of(j + 2);
     };
-    load();
-    place(1, next_page);
-    next_page = page_of(2);
-    cp_async_wait<0>();
-    arrive(S::Q_FULL);
+    load(0);
+    load(1);
     for (int j = 0; j < nb; ++j) {
       const int it = blocks + j, s = it % STAGES;
+      load(j + 2);
+      cp_async_wait<2>();  // block j is there, and the queries
+      if (j == 0) arrive(S::Q_FULL);
       if (!sh.wait(empty + 8 * s, it / STAGES + 1, p, 5)) break;
+      const uint32_t slot = static_cast<uint32_t>(j % C::RAWS) * C::RAW_BYTES;
       if (keys) {
+        const float ks = *reinterpret_cast<const float*>(sh.base + scale0 + slot);
+        const float vs = *reinterpret_cast<const float*>(sh.base + scale0 + slot + TILE_KEYS * 4);
         float* sc = sh.scales(it) + row0 + lane;
         sc[0] = ks * p.scale_log2;
         if constexpr (C::MUL_V) sc[TILE_KEYS] = vs;
@@ -592,12 +606,13 @@ TJ_DEV void produce(const AttnParams& p, const TilesShared<T, CD, D>& sh, int se
         }
         mbar_arrive(sh.at(S::SC_FULL + 8 * (it % C::SCALES)));
       }
+      uint4 raw[N];
+#pragma unroll
+      for (int i = 0; i < N; ++i) raw[i] = *reinterpret_cast<const uint4*>(sh.base + raw0 + slot + i * 512);
       store_rows<T, CD, D>(dst0 + s * C::KV_BYTES, raw, row0);
       announce(it);
-      load();  // the next block's
-      place(j + 2, next_page);
-      next_page = page_of(j + 3);
     }
+    cp_async_wait<0>();
   }
 }
 
