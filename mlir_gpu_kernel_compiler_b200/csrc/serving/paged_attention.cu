@@ -22,6 +22,9 @@ const char* attention_fault(const tj_paged_attention& a) {
   if ((a.cache.dtype == TJ_F16 || a.cache.dtype == TJ_BF16) && a.cache.dtype != a.dtype)
     return "a 16-bit cache must have q's type";
   if (a.cache.dim != 64 && a.cache.dim != 128) return "head dim must be 64 or 128";
+  const int es = element_size(a.cache.dtype);
+  if (a.cache.page_stride * es % 16 || a.cache.slot_stride * es % 16 || a.cache.head_stride * es % 16)
+    return "cache rows must start on 16-byte boundaries";
   if (a.tokens < 0 || a.batch < 0 || a.q_heads <= 0 || a.max_new <= 0 || a.table_width <= 0 || a.window < 0)
     return "bad extent";
   if (a.q_heads % a.cache.heads) return "query heads must be a multiple of the cache's heads";

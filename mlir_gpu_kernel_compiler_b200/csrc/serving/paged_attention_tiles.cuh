@@ -213,28 +213,10 @@ TJ_DEV void store_rows(uint32_t dst, const uint4 (&raw)[N], int row0) {
   }
 }
 
-// 2^x of a pair on the FMA pipes: x = j + f, j its nearest integer (added to the exponent), |f| <= 1/2 and
-// 2^f by a polynomial of degree 4 fitted here (least squares reweighted towards the largest relative error,
-// which is 2.6e-6; its mean is 4e-8).  The units for exponentials make 16 a clock and SM and are as
-// busy as the tensor cores, so some of the pairs take this way.  x <= 127; below -126 it is 2^-126.
-TJ_DEV void exp2_pair(uint64_t x, float& e0, float& e1) {
-  using namespace tja;
-  float x0, x1;
-  f2_unpack(x, x0, x1);
-  x = f2_pack(fmaxf(x0, -126.0f), fmaxf(x1, -126.0f));
-  const uint64_t magic = f2_pack(12582912.0f, 12582912.0f), unmagic = f2_pack(-12582912.0f, -12582912.0f);  // 1.5 * 2^23
-  const uint64_t t = f2_add(x, magic);
-  const uint64_t f = f2_fma(f2_add(t, unmagic), f2_pack(-1.0f, -1.0f), x);
-  auto c = [](float v) { return f2_pack(v, v); };
-  uint64_t y = f2_fma(c(0.009570102207362652f), f, c(0.05591786280274391f));
-  y = f2_fma(y, f, c(0.240247443318367f));
-  y = f2_fma(y, f, c(0.6931217908859253f));
-  y = f2_fma(y, f, c(0.9999992847442627f));
-  float t0, t1, y0, y1;
-  f2_unpack(t, t0, t1);
-  f2_unpack(y, y0, y1);
-  e0 = __int_as_float(__float_as_int(y0) + (__float_as_int(t0) << 23));
-  e1 = __int_as_float(__float_as_int(y1) + (__float_as_int(t1) << 23));
+TJ_DEV uint64_t f2_mul(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
 }
 
 template <class T, int CD, int D> struct Tiles {
@@ -260,46 +242,37 @@ template <class T, int CD, int D> struct Tiles {
   static_assert(256 * REGS_S + 128 * REGS_P + 128 * REGS_M <= 512 * 128, "no more than the block was launched with");
   // TMEM columns: scores of tile t, buffer b at (2 t + b) 64 (P, 32 columns, over them); O_t at 256 + t D
   static constexpr uint32_t TMEM = 512;
-#ifndef TJS_EMU
-#define TJS_EMU 0
-#endif
-  // exponentials of every 16 pairs that go to the FMA pipes: see exp2_pair
-  static constexpr int EMU = TJS_EMU;
   static constexpr float SHIFT = P_SHIFT<T> > 11.0f ? 11.0f : P_SHIFT<T>;  // with RAISE: P < 2^16
   static constexpr float RAISE = P_SHIFT<T> > 0.0f ? 4.0f : 8.0f;
 };
 
 // A row's P = 2^(x c + b) (8-bit caches: x + b) of a block: summed into ll, rounded to 16 bits and
 // written over the scores at tS.
-template <class T, class C, int EMU>
+template <class T, class C>
 TJ_DEV void probabilities(const float (&x)[64], uint64_t c, uint64_t b, const float* sc, uint64_t& ll, uint32_t tS) {
   using namespace tja;
 #pragma unroll
   for (int g = 0; g < 2; ++g) {
     uint32_t pk[16];
+    float4 vs = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
       const int i = g * 32 + 2 * k;
       const uint64_t xx = f2_pack(x[i], x[i + 1]);
       const uint64_t e = C::Q8 ? f2_add(xx, b) : f2_fma(xx, c, b);
       float e0, e1;
-      if (k * EMU % 16 < EMU) {
-        exp2_pair(e, e0, e1);
-      } else {
-        f2_unpack(e, e0, e1);
-        e0 = exp2_fast(e0);
-        e1 = exp2_fast(e1);
-      }
+      f2_unpack(e, e0, e1);
+      e0 = exp2_fast(e0);
+      e1 = exp2_fast(e1);
       if constexpr (C::EXP_V) {
-        const float2 inv = *reinterpret_cast<const float2*>(sc + 2 * TILE_KEYS + i);
-        ll = f2_fma(f2_pack(e0, e1), f2_pack(inv.x, inv.y), ll);
+        if (k % 2 == 0) vs = *reinterpret_cast<const float4*>(sc + 2 * TILE_KEYS + i);  // 1 / vs
+        ll = f2_fma(f2_pack(e0, e1), k % 2 ? f2_pack(vs.z, vs.w) : f2_pack(vs.x, vs.y), ll);
       } else {
         ll = f2_add(ll, f2_pack(e0, e1));
       }
       if constexpr (C::MUL_V) {
-        const float2 vs = *reinterpret_cast<const float2*>(sc + TILE_KEYS + i);
-        e0 *= vs.x;
-        e1 *= vs.y;
+        if (k % 2 == 0) vs = *reinterpret_cast<const float4*>(sc + TILE_KEYS + i);
+        f2_unpack(f2_mul(f2_pack(e0, e1), k % 2 ? f2_pack(vs.z, vs.w) : f2_pack(vs.x, vs.y)), e0, e1);
       }
       pk[k] = pack2<T>(e0, e1);
     }
@@ -740,12 +713,17 @@ TJ_DEV void softmax(const AttnParams& p, const TilesShared<T, CD, D>& sh, uint32
 #pragma unroll
       for (int i = 0; i < 64; i += 4) {
         const float4 k = *reinterpret_cast<const float4*>(sc + i);
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if constexpr (C::EXP_V) v = *reinterpret_cast<const float4*>(sc + TILE_KEYS + i);
-        x[i] = fmaf(x[i], k.x, v.x);
-        x[i + 1] = fmaf(x[i + 1], k.y, v.y);
-        x[i + 2] = fmaf(x[i + 2], k.z, v.z);
-        x[i + 3] = fmaf(x[i + 3], k.w, v.w);
+        uint64_t a = tja::f2_pack(x[i], x[i + 1]), b = tja::f2_pack(x[i + 2], x[i + 3]);
+        if constexpr (C::EXP_V) {
+          const float4 v = *reinterpret_cast<const float4*>(sc + TILE_KEYS + i);
+          a = tja::f2_fma(a, tja::f2_pack(k.x, k.y), tja::f2_pack(v.x, v.y));
+          b = tja::f2_fma(b, tja::f2_pack(k.z, k.w), tja::f2_pack(v.z, v.w));
+        } else {
+          a = f2_mul(a, tja::f2_pack(k.x, k.y));
+          b = f2_mul(b, tja::f2_pack(k.z, k.w));
+        }
+        tja::f2_unpack(a, x[i], x[i + 1]);
+        tja::f2_unpack(b, x[i + 2], x[i + 3]);
       }
     }
     const bool masked = kb < clo || kb + TILE_KEYS > chi;  // the same for the warp
@@ -793,11 +771,7 @@ TJ_DEV void softmax(const AttnParams& p, const TilesShared<T, CD, D>& sh, uint32
     const float base = (m == -INFINITY ? 0.0f : m) - C::SHIFT;
     const uint64_t cc = tja::f2_pack(c, c), nb2 = tja::f2_pack(-base, -base);
     uint64_t ll = tja::f2_pack(l0, l1);
-    // hidden keys have to be exactly 0: a masked block's exponentials are all the unit's
-    if (C::EMU == 0 || masked)
-      probabilities<T, C, 0>(x, cc, nb2, sc, ll, tS);
-    else
-      probabilities<T, C, C::EMU>(x, cc, nb2, sc, ll, tS);
+    probabilities<T, C>(x, cc, nb2, sc, ll, tS);
     tja::f2_unpack(ll, l0, l1);
     tja::tmem_wait_st();
     tc_fence_before();

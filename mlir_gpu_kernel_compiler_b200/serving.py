@@ -16,8 +16,8 @@ tensors' device and return without waiting.  As in ``B200Program``, a wrong type
 ``runtime.RuntimeError_``; a slot, position, page or length out of range is seen by the device alone,
 which skips it and records it: ``check()`` raises for it.
 
-Each operator is one hand-written sm_100a kernel in ``csrc/serving`` behind a C entry point of
-``include/tj_b200.h``.
+Each operator is a C entry point of ``include/tj_b200.h`` over hand-written sm_100a kernels in
+``csrc/serving``.
 """
 from __future__ import annotations
 
@@ -53,7 +53,8 @@ class PagedCache:
 
     ``k`` and ``v``: ``[pages, page_size, kv_heads, head_dim]``, f16 or bf16, or i8 or e4m3 codes with
     scales ``[pages, page_size, kv_heads]`` in f32 (value = code * scale).  Both may be views whose
-    memory is in another order (heads before slots, say), the same for k and v, rows contiguous.
+    memory is in another order (heads before slots, say), the same for k and v, rows contiguous and
+    starting on 16-byte boundaries (8-byte ones do for 8-bit codes that attention does not read).
     Slot ``s`` is place ``s % page_size`` of page ``s // page_size``.
     """
 

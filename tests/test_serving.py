@@ -116,3 +116,13 @@ def test_python_refusals_on_the_host():
         with pytest.raises(ValueError):
             serving.rotary_table(**{"rot_dim": 8, "max_positions": 4, "device": "cpu", **how})
     assert serving.rotary_table(8, 4, device="cpu").shape == (4, 8)
+
+
+@pytest.mark.parametrize("strides", [(2048, 128, 72), (2048, 136, 64), (2056, 128, 64)])
+def test_attention_refuses_cache_rows_that_only_start_on_8_bytes(strides):
+    """The row operators take 8-bit rows at multiples of 8 bytes; attention copies 16 bytes at a time."""
+    lib, size, count = rt.library(), ctypes.c_int64(), ctypes.c_int64()
+    args = ATTENTION.pack(4096, 4096, 0, 4096, 4096, 4096, 4096, 4096, 5, 2, 4, 3, 4, 4, 256, 64, 256, 64, 2, 1, 0, 0.125,
+                          1 << 40, 1 << 30) + _cache(strides=strides)
+    assert lib.tj_b200_paged_attention(args, None) == rt.TJ_ERR_INVALID and b"16-byte" in lib.tj_b200_last_error()
+    assert lib.tj_b200_paged_attention_workspace(args, ctypes.byref(size), ctypes.byref(count)) == rt.TJ_ERR_INVALID
