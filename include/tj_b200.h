@@ -200,15 +200,16 @@ TJ_API int tj_b200_ipc_close(void* dptr, uint64_t offset, int32_t device);
 
 /* ---------------------------------------------------------------------------------------------
  * Serving operators: rotary positions, a paged cache of keys and values, attention over it.
- * No counterpart in the reference (its programs have no state between calls).  They launch one
- * kernel each on `stream` (a cudaStream_t of the current device), allocate nothing and wait for
+ * No counterpart in the reference (its programs have no state between calls).  They launch
+ * one or two kernels on `stream` (a cudaStream_t of the current device), allocate nothing and wait for
  * nothing.  Extents and strides are in elements.  Host-side faults return TJ_ERR_INVALID before
  * anything is launched.  What only the device can see (a slot, position, page or length out of
  * range) is skipped there and recorded in status words, read by tj_b200_serving_status. */
 enum { TJ_F32 = 0, TJ_F16 = 1, TJ_BF16 = 2, TJ_I8 = 3, TJ_E4M3 = 4 };
 
 /* A pool of `pages` pages of `page_size` slots; slot s is place s % page_size of page
- * s / page_size.  k and v share their strides, element 1 apart along the head dim.  dtype f16 or
+ * s / page_size.  k and v share their strides, element 1 apart along the head dim; rows start on 16-byte
+ * boundaries (8-byte ones for 8-bit codes that attention does not read).  dtype f16 or
  * bf16 (no scales), or i8 or e4m3 with one f32 scale for each (slot, head): value = code * scale. */
 typedef struct tj_kv_cache {
   void* k;

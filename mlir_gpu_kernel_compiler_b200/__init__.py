@@ -20,8 +20,9 @@ The package holds: ``plan`` (the plan data model), ``memory`` (arena planner),
 templates and the C++ runtime behind ``include/tj_b200.h``), ``toolchain``
 (nvcc / g++ builds and the cubin cache), ``runtime`` (ctypes binding of the C
 ABI), ``program`` (``B200Program``), ``autotune`` (tcgen05 tile search),
-``distributed`` (row-sharded execution over NCCL) and ``workloads`` (the
-benchmark programs' seeded inputs).
+``distributed`` (row-sharded execution over NCCL), ``serving`` (rotary
+positions, paged cache, attention over it) and ``workloads`` (the benchmark
+programs' seeded inputs).
 """
 from __future__ import annotations
 

@@ -65,9 +65,12 @@ Plan plan(const tj_paged_attention& a, const Device& dev) {
   p.rows = 16;
   // Few row tiles are cut so that all pieces run at once, one CTA an SM (pieces: at most target + tiles).
   // Many uneven ones are cut for three waves of smaller CTAs, which even out what one wave does not.
+  // (One token over 777 keys 9.7 us in this way, 11.1 in the other; three over 100003 in 8 bits 59, 63.)
   const double items = a.cache.heads * row_tiles;
   p.wide = items <= dev.sms / 2;
   p.target = p.wide ? dev.sms - static_cast<int>(items) : 3 * dev.sms * (q8 ? 3 : 2);
+  // Keys of a chunk at least: one token over 4096 keys takes 12.1 us with 256, 12.5 with 128, 14.4 with 512; four
+  // over 2000 keys of 8 bits 13.8, 13.8, 16.1.
   p.min_chunk = 256;
   const long tiles = a.q_starts ? a.tokens * group / 16 + a.batch : a.batch * ((group + 15) / 16);  // at the most
   p.grid = a.cache.heads * (tiles + 1) + p.target;

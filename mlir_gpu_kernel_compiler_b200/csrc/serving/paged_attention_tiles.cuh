@@ -13,15 +13,21 @@
 //              running maximum (moved, and the sums in TMEM rescaled, only when a block exceeds it by
 //              more than 2^RAISE) and sum, and writes P over the scores, 16 bits each.
 //   8-11       producers of the keys (8, 9) and values (10, 11): a warp brings 32 rows of each block.
-//              Pages are looked up one key a lane, rows copied asynchronously (16-bit caches) or
-//              converted to 16 bits on the way (8-bit ones), in the 128-byte-swizzled layout that the
-//              matrix unit reads.  Pages may have any size and the cache any strides, as no copy spans
+//              Pages are looked up one key a lane, rows copied asynchronously in the 128-byte-swizzled
+//              layout that the matrix unit reads; 8-bit codes are copied two blocks ahead and made
+//              16-bit from there.  Pages may have any size and the cache any strides, as no copy spans
 //              two rows.
 //   12, 13     issue the matrix instructions of row tile 0, 1: per block P V, then the scores of the
 //              block after the next over the P that it has read.  (One warp for both was the bound, 2400
 //              clocks a block: a wait for a barrier takes 140 clocks even when it is over, as it queues
 //              behind the softmax warps' exponentials.)
 //   14         looks the next segment up.
+//
+// Measured: 2048 tokens over 16384 bf16 keys, 32 heads of 128 on 8 cached ones, 493 us = 1045 TFLOP/s (64 % of
+// the measured matrix rate) in short runs and 568 us under the board's power limit, where variants that
+// need fewer clocks take as long.  Over i8 codes 820 us: the conversion is made again by every tile of a head,
+// and its instructions and the scales' (two products a score) share the schedulers with the softmax; left
+// out, in a timing build, they give 531.  Eight producer warps of 16 rows each were no help (884 us).
 //
 // The work, (tile, block) pairs of all sequences and heads in a row, is cut into as many equal parts as
 // there are SMs (each at least 512 keys): a CTA takes a tile's end, whole tiles and a tile's beginning.
