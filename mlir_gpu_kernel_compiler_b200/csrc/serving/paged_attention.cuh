@@ -31,8 +31,10 @@ struct AttnParams {
   int tile_ctas;     // CTAs of the kernel of many rows
 };
 
-// log2 vs is held at this or above: a row of zeros has vs = 0
-constexpr float MIN_LOG2_SCALE = -40.0f;
+// log2 vs, held at -80 or above: a row of zeros has vs = 0, and a key whose P = 2^(t - m) underflows f32
+// (2^-126) may be left out of the sum only if it is below 2^-46 of the largest.  Values under 127 * 2^-80 thus come
+// out up to that size.  A NaN (the scale of a row that is not finite) stays one.
+TJ_DEV float log2_scale(float vs) { return vs == vs ? fmaxf(__log2f(vs), -80.0f) : vs; }
 
 struct Seq {
   int start, n, len;  // first new token, new tokens, keys

@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
     float* const scale = reinterpret_cast<float*>(ring + warp * R::WARP + STAGES * R::BLOCK) + stage * KS * 3;
     if constexpr (Q8) {
       scale[lane] *= score_scale;
-      const float lv = fmaxf(__log2f(scale[KS + lane]), MIN_LOG2_SCALE);
+      const float lv = log2_scale(scale[KS + lane]);
       scale[KS + lane] = lv;
       scale[2 * KS + lane] = exp2_fast(-lv);
       __syncwarp();

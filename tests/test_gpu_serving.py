@@ -491,3 +491,23 @@ def test_what_is_refused_before_a_launch():
                       (lambda: serving.paged_attention(x.float(), cache, pages, lens), "dtype")]:
         with pytest.raises(ValueError, match=why):
             call()
+
+
+@pytest.mark.parametrize("new", [1, 300])
+@pytest.mark.parametrize("cache_dtype,dim", [("i8", 128), ("e4m3", 64)])
+def test_very_small_values_beside_zeros(new, cache_dtype, dim):
+    """Value scales around 1e-16, and every third key's scale 0: nothing is held at a larger size."""
+    case = _case([(new, 700), (new, 333), (new, new)], 8, 2, dim, "bf16", cache_dtype, seed=21)
+    scale = case[1].v_scale
+    scale.mul_(1e-15)
+    scale.view(-1, scale.shape[-1])[::3] = 0
+    _agree(case, max_new=new)
+
+
+@pytest.mark.parametrize("new", [1, 300])
+def test_a_value_row_held_as_nan_reaches_the_output(new):
+    case = _case([(new, 700)], 8, 2, 128, "bf16", "i8", seed=22)
+    q, cache, table, lens, starts = case
+    cache.v_scale[table[0, 0].item(), 3] = math.nan
+    out = serving.paged_attention(q, cache, table, lens, starts, max_new=new)
+    assert out.isnan().all()
