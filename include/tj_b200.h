@@ -254,7 +254,8 @@ TJ_API int tj_b200_cache_read(const tj_kv_cache* cache, const int32_t* slots, in
 /* Attention of new tokens over the cache.  Sequence b's new tokens are rows q_starts[b] .. q_starts[b+1]
  * of q (q_starts NULL: one token each, row b); they stand at the end of its kv_lens[b] keys, which lie
  * in pages page_table[b * table_row + i].  causal: a token sees the keys up to its own position;
- * window > 0: the last `window` of those.  A row that sees nothing is 0 (lse: -inf).
+ * window > 0: none before the last `window` up to its own position (without causal, those after it all the
+ * same).  A row that sees nothing is 0 (lse: -inf).
  * counters: int32, zero before the first call and left zero by every call; workspace: anything.
  * Calls that share them must not overlap.  max_new: no sequence has more new tokens. */
 typedef struct tj_paged_attention {

@@ -3,7 +3,8 @@
 //   o[i, h] = sum_j p_ij v_j / sum_j p_ij,   p_ij = exp(scale q_i k_j - max),   j visible to i
 //
 // Token i of a sequence's n new tokens stands at position len - n + i; it sees the keys at
-// positions up to its own (causal) and, with a window w, only the last w of those.  The G query
+// positions up to its own (causal: else those after it too) and, with a window w, none before the last
+// w of its own position and those before it.  The G query
 // heads that share a cached head are packed with the tokens into rows r = i * G + g, so a key or a
 // value is read once for all of them.
 //
@@ -63,24 +64,27 @@ TJ_DEV void key_range(const AttnParams& p, const Seq& s, int t0, int t1, int& lo
 // the same of one row's token
 TJ_DEV void row_range(const AttnParams& p, const Seq& s, int t, int& lo, int& hi) { key_range(p, s, t, t, lo, hi); }
 
-// A CTA's piece of the work: row tile `tile` of sequence `b`, chunk `c` of its keys.
+// A CTA's piece of the work: row tile `tile` of sequence `b`, chunk `c` of its keys, of which `cuts` are launched.
 struct Piece {
-  int b, tile, c, chunk;
+  int b, tile, c, chunk, cuts;
   bool some;
 };
 
 // The work is cut on the device, so that neither lengths nor a plan pass through the host: every
 // warp adds up the sequences' (row tiles x keys), divides by the wanted number of CTAs for the
 // chunk, and finds the piece of unit `unit` among the sequences' counts.  `per_tile` rows are a
-// tile; chunks are multiples of `step` keys.
+// tile; chunks are multiples of `step` keys.  A tile gets as many pieces as the widest of its sequence could
+// need; what key_range then gives of its own keys decides how many of them work.
 TJ_DEV Piece find_piece(const AttnParams& p, int unit, int per_tile, int step) {
   const int lane = threadIdx.x & 31;
   const int batch = static_cast<int>(p.a.batch), per = (batch + 31) / 32;
   const int b0 = min(lane * per, batch), b1 = min(b0 + per, batch);
+  // under a window a tile's keys reach from its first token's window to its last token, or, without the causal
+  // mask, to the sequence's end
   const int tokens_per_tile = (per_tile + p.group - 1) / p.group + 1;
   auto tiles = [&](const Seq& s) { return (s.n * p.group + per_tile - 1) / per_tile; };
   auto span = [&](const Seq& s) {
-    return p.a.window > 0 ? static_cast<int>(min(static_cast<int64_t>(s.len), p.a.window + tokens_per_tile)) : s.len;
+    return p.a.window > 0 ? static_cast<int>(min(static_cast<int64_t>(s.len), p.a.window + (p.a.causal ? tokens_per_tile : s.n))) : s.len;
   };
   long work = 0;
   for (int b = b0; b < b1; ++b) {
@@ -111,7 +115,7 @@ TJ_DEV Piece find_piece(const AttnParams& p, int unit, int per_tile, int step) {
   const unsigned who = __ballot_sync(0xffffffffu, owner);
   g.some = who != 0;
   if (!g.some) return g;
-  int fb = 0, ft = 0, fc = 0;
+  int fb = 0, ft = 0, fc = 0, fn = 1;
   if (owner) {
     int left = unit - before;
     for (int b = b0; b < b1; ++b) {
@@ -121,6 +125,7 @@ TJ_DEV Piece find_piece(const AttnParams& p, int unit, int per_tile, int step) {
         fb = b;
         ft = left / cuts;
         fc = left - ft * cuts;
+        fn = cuts;
         break;
       }
       left -= n;
@@ -130,6 +135,7 @@ TJ_DEV Piece find_piece(const AttnParams& p, int unit, int per_tile, int step) {
   g.b = __shfl_sync(0xffffffffu, fb, src);
   g.tile = __shfl_sync(0xffffffffu, ft, src);
   g.c = __shfl_sync(0xffffffffu, fc, src);
+  g.cuts = __shfl_sync(0xffffffffu, fn, src);
   return g;
 }
 

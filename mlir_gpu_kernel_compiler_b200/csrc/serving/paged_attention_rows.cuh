@@ -118,9 +118,10 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
   const int r0 = w.tile * 16;
   int lo, hi;
   key_range(p, s, r0 / p.group, (r0 + rows - 1) / p.group, lo, hi);
-  const int cuts = max(1, (hi - lo + w.chunk - 1) / w.chunk);
+  // never more chunks than were launched, as each has to arrive at the tile's counter; the last takes what is left
+  const int cuts = min(w.cuts, max(1, (hi - lo + w.chunk - 1) / w.chunk));
   if (w.c >= cuts) return;
-  const int k0 = lo + w.c * w.chunk, k1 = min(hi, k0 + w.chunk);
+  const int k0 = lo + w.c * w.chunk, k1 = w.c + 1 < cuts ? k0 + w.chunk : hi;
   if (threadIdx.x == 0 && w.c == 0 && h == 0 &&
       (p.a.kv_lens[w.b] < 0 || p.a.kv_lens[w.b] > p.a.table_width * p.a.cache.page_size))
     tj_report(p.status, TJ_STATUS_BOUNDS, OP_ATTENTION * 16 + SITE_LENGTH);

@@ -69,7 +69,7 @@ TJ_DEV TileWork tile_work(const AttnParams& p, const Seq& s) {
   if (w.grows)
     span = max(s.len - s.n, 0);
   else if (p.a.window > 0)
-    span = min(span, static_cast<long>(p.a.window) + TILE_ROWS / p.group);
+    span = min(span, static_cast<long>(p.a.window) + (p.a.causal ? TILE_ROWS / p.group : s.n));
   w.base = p.group * (span + TILE_KEYS);
   w.per_head = w.before(w.tiles);
   return w;

@@ -177,8 +177,9 @@ def paged_attention(q, cache: PagedCache, page_table, kv_lens, q_starts=None, *,
     tokens are rows ``q_starts[b]`` to ``q_starts[b + 1]`` of q, the last of its keys (None: one each).
     ``max_new``: the most new tokens of any sequence (default: 1 without q_starts, else all of them).
 
-    A token sees the keys up to its own position (all of them if not ``causal``), of those the last
-    ``window`` if that is positive.  ``scale`` (default head_dim**-0.5) multiplies the scores.  A row that
+    A token sees the keys up to its own position; if not ``causal``, those after it too.  A positive ``window``
+    hides the keys before the last ``window`` up to its own position (its own among them), and, without the
+    causal mask, none of those after it.  ``scale`` (default head_dim**-0.5) multiplies the scores.  A row that
     sees no key is 0; rows of no sequence are not written.  ``return_lse``: also the logarithm of each row's sum
     of exponentials, f32 ``[tokens, q_heads]`` (-inf for a row that sees no key).  Slots that no row of a
     sequence sees may hold anything; visible ones must be finite, as a NaN or an infinity reaches the

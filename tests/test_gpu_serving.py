@@ -511,3 +511,19 @@ def test_a_value_row_held_as_nan_reaches_the_output(new):
     cache.v_scale[table[0, 0].item(), 3] = math.nan
     out = serving.paged_attention(q, cache, table, lens, starts, max_new=new)
     assert out.isnan().all()
+
+
+@pytest.mark.parametrize("cache_dtype", ["bf16", "i8"])
+@pytest.mark.parametrize("hq,hk,dim,new,max_new,window", [(1, 1, 64, 300, 300, 16), (1, 1, 64, 300, 300, 100), (32, 8, 128, 60, 1, 7),
+                                                          (8, 2, 128, 500, 500, 129), (4, 4, 64, 700, 1, 300)])
+def test_windows_without_causal_mask(hq, hk, dim, new, max_new, window, cache_dtype):
+    """Without the causal mask a window hides only what is before it, so a tile's keys go on to the sequence's end.  (max_new
+    chooses the kernel and nothing else: 1 gives the kernel of few rows.)  A cut call after it on the same
+    stream finds its counters at zero."""
+    lens = [(new, 1000), (3, 700), (new, new), (1, 2000)]
+    plain = _case([(1, 9000), (2, 3000)], hq, hk, dim, "bf16", cache_dtype, seed=31)
+    want = [_agree(plain, max_new=2) for _ in range(2)]
+    _agree(_case(lens, hq, hk, dim, "bf16", cache_dtype, seed=30), max_new=max_new, window=window, causal=False)
+    _agree(_case(lens[:1], hq, hk, dim, "bf16", cache_dtype, seed=32), max_new=max_new, window=window, causal=False)
+    for _ in range(3):
+        assert torch.equal(_agree(plain, max_new=2), want[0])
