@@ -154,6 +154,7 @@ extern "C" int tj_b200_paged_attention(const tj_paged_attention* args, void* str
   if (how.grid > 0x7fffffffL) return refuse(TJ_ERR_INVALID, name, "too many rows");
   AttnParams p;
   p.a = a;
+  p.a.window = std::min<int64_t>(a.window, 0x7fffffff);  // no sequence is longer, and the kernels add to it
   p.status = dev.status;
   p.scale_log2 = static_cast<float>(a.scale * 1.4426950408889634);
   p.group = static_cast<int>(a.q_heads / a.cache.heads);

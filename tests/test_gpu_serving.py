@@ -527,3 +527,13 @@ def test_windows_without_causal_mask(hq, hk, dim, new, max_new, window, cache_dt
     _agree(_case(lens[:1], hq, hk, dim, "bf16", cache_dtype, seed=32), max_new=max_new, window=window, causal=False)
     for _ in range(3):
         assert torch.equal(_agree(plain, max_new=2), want[0])
+
+
+@pytest.mark.parametrize("window", [2**31 - 1, 2**31, 2**63 - 1])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("cache_dtype", ["bf16", "i8"])
+def test_windows_as_long_as_integers_go(window, causal, cache_dtype):
+    case = _case([(1, 1), (1, 5000), (1, 130)], 8, 2, 128, "bf16", cache_dtype, seed=33)
+    _agree(case, decode=True, window=window, causal=causal)
+    case = _case([(200, 200), (1, 5000), (90, 3000)], 8, 2, 128, "bf16", cache_dtype, seed=34)
+    _agree(case, max_new=200, window=window, causal=causal)
