@@ -204,7 +204,8 @@ TJ_API int tj_b200_ipc_close(void* dptr, uint64_t offset, int32_t device);
  * one or two kernels on `stream` (a cudaStream_t of the current device), allocate nothing and wait for
  * nothing.  Extents and strides are in elements.  Host-side faults return TJ_ERR_INVALID before
  * anything is launched.  What only the device can see (a slot, position, page or length out of
- * range) is skipped there and recorded in status words, read by tj_b200_serving_status. */
+ * range) is skipped there and recorded in status words, read by tj_b200_serving_status.  A row turned by a
+ * position out of range becomes NaN; q_starts in descending order make an attention call do nothing. */
 enum { TJ_F32 = 0, TJ_F16 = 1, TJ_BF16 = 2, TJ_I8 = 3, TJ_E4M3 = 4 };
 
 /* A pool of `pages` pages of `page_size` slots; slot s is place s % page_size of page
@@ -284,8 +285,8 @@ TJ_API int tj_b200_paged_attention_workspace(const tj_paged_attention* args, int
 
 /* Waits for `stream`, reads the serving operators' status words of the current device and clears
  * them: TJ_OK and *code = 0, or TJ_ERR_DEVICE_STATUS with *code (1 wait timeout, 2 index out of range)
- * and *where = operator * 16 + site (operators 0 rotary, 1 write, 2 read, 3 attention; sites 1 slot,
- * 2 position, 3 page, 4 length, 5 and up a wait). */
+ * and *where = operator * 16 + site (operators 0 rotary, 1 write, 2 read, 3 attention; with code 2 the sites
+ * are 1 slot, 2 position, 3 page, 4 length, 6 q_starts, with code 1 they name the wait). */
 TJ_API int tj_b200_serving_status(int32_t* code, int32_t* where, void* stream);
 
 /* Message of the last failure on this thread ("" if none). */

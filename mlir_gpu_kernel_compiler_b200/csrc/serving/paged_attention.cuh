@@ -55,6 +55,17 @@ TJ_DEV Seq sequence(const AttnParams& p, int b) {
   return s;
 }
 
+// Whether sequence b's token range is turned round.  Where one is, others overlap: rows of the output would have two
+// writers and the work more pieces than were launched, so the whole call does nothing.
+TJ_DEV bool descending(const AttnParams& p, int b) { return p.a.q_starts && p.a.q_starts[b] > p.a.q_starts[b + 1]; }
+// Records what is wrong with sequence b's numbers (its length only if it has new tokens); `sequence` clamps them.
+TJ_DEV void report_sequence(const AttnParams& p, int b) {
+  if (sequence(p, b).n > 0 && (p.a.kv_lens[b] < 0 || p.a.kv_lens[b] > p.a.table_width * p.a.cache.page_size))
+    tj_report(p.status, TJ_STATUS_BOUNDS, OP_ATTENTION * 16 + SITE_LENGTH);
+  if (p.a.q_starts && (p.a.q_starts[b] < 0 || p.a.q_starts[b + 1] > p.a.tokens || descending(p, b)))
+    tj_report(p.status, TJ_STATUS_BOUNDS, OP_ATTENTION * 16 + SITE_STARTS);
+}
+
 // keys that some of the tokens [t0, t1] of a sequence see
 TJ_DEV void key_range(const AttnParams& p, const Seq& s, int t0, int t1, int& lo, int& hi) {
   hi = p.a.causal ? max(0, min(s.len, s.len - s.n + t1 + 1)) : s.len;
@@ -87,15 +98,19 @@ TJ_DEV Piece find_piece(const AttnParams& p, int unit, int per_tile, int step) {
     return p.a.window > 0 ? static_cast<int>(min(static_cast<int64_t>(s.len), p.a.window + (p.a.causal ? tokens_per_tile : s.n))) : s.len;
   };
   long work = 0;
+  bool turned = false;
   for (int b = b0; b < b1; ++b) {
     const Seq s = sequence(p, b);
+    turned |= descending(p, b);
     work += static_cast<long>(tiles(s)) * span(s);
   }
+  Piece g;
+  g.some = false;
+  if (__any_sync(0xffffffffu, turned)) return g;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
   // (in f32, rounded up generously: pieces may only become fewer; 64-bit divisions take hundreds of clocks)
   const long want = static_cast<long>(static_cast<float>(work * p.a.cache.heads) / static_cast<float>(p.target) * 1.000001f) + 1;
-  Piece g;
   g.chunk = static_cast<int>((max(want, static_cast<long>(p.min_chunk)) + step - 1) / step * step);
   auto cuts_of = [&](const Seq& s) {
     const int n = span(s) + g.chunk - 1, q = static_cast<int>(__fdividef(static_cast<float>(n), static_cast<float>(g.chunk)));

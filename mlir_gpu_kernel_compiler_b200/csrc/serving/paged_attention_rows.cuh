@@ -112,6 +112,8 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
   const int heads = static_cast<int>(p.a.cache.heads);
   const int unit = blockIdx.x / heads, h = blockIdx.x - unit * heads;
   const Piece w = find_piece(p, unit, 16, WARPS * KS);
+  if (blockIdx.x == 0)
+    for (int b = threadIdx.x; b < p.a.batch; b += R::THREADS) report_sequence(p, b);
   if (!w.some) return;
   const Seq s = sequence(p, w.b);
   const int rows = min(16, s.n * p.group - w.tile * 16);
@@ -122,9 +124,6 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
   const int cuts = min(w.cuts, max(1, (hi - lo + w.chunk - 1) / w.chunk));
   if (w.c >= cuts) return;
   const int k0 = lo + w.c * w.chunk, k1 = w.c + 1 < cuts ? k0 + w.chunk : hi;
-  if (threadIdx.x == 0 && w.c == 0 && h == 0 &&
-      (p.a.kv_lens[w.b] < 0 || p.a.kv_lens[w.b] > p.a.table_width * p.a.cache.page_size))
-    tj_report(p.status, TJ_STATUS_BOUNDS, OP_ATTENTION * 16 + SITE_LENGTH);
 
   const int* table = p.a.page_table + w.b * p.a.table_row;
   const char* kbase = static_cast<const char*>(p.a.cache.k) + h * p.a.cache.head_stride * ES;

@@ -84,11 +84,13 @@ struct TilePart {
 TJ_DEV long total_work(const AttnParams& p) {
   const int lane = threadIdx.x & 31;
   long mine = 0;
+  bool turned = false;
   for (int b = lane; b < p.a.batch; b += 32) {
     mine += tile_work(p, sequence(p, b)).per_head;
-    if (blockIdx.x == 0 && threadIdx.x < 32 && (p.a.kv_lens[b] < 0 || p.a.kv_lens[b] > p.a.table_width * p.a.cache.page_size))
-      tj_report(p.status, TJ_STATUS_BOUNDS, OP_ATTENTION * 16 + SITE_LENGTH);
+    turned |= descending(p, b);
+    if (blockIdx.x == 0 && threadIdx.x < 32) report_sequence(p, b);
   }
+  if (__any_sync(0xffffffffu, turned)) return 0;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, o);
   return mine * p.a.cache.heads;

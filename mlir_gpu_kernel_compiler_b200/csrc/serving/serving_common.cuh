@@ -19,7 +19,7 @@ namespace tjs {
 constexpr int MAX_DEVICES = 64;
 
 // Where a status word's `where` points: operator * 16 + site.
-enum : int { SITE_SLOT = 1, SITE_POSITION = 2, SITE_PAGE = 3, SITE_LENGTH = 4 };
+enum : int { SITE_SLOT = 1, SITE_POSITION = 2, SITE_PAGE = 3, SITE_LENGTH = 4, SITE_STARTS = 6 };
 enum : int { OP_ROTARY = 0, OP_CACHE_WRITE = 1, OP_CACHE_READ = 2, OP_ATTENTION = 3 };
 
 // cache_rows.cu: the current device's status words and its multiprocessor count.

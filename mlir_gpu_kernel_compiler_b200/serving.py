@@ -174,7 +174,8 @@ def paged_attention(q, cache: PagedCache, page_table, kv_lens, q_starts=None, *,
     ``h * group .. (h + 1) * group`` read cached head ``h``).  A 16-bit cache has q's dtype.
     ``page_table`` int32 ``[batch, width]``: the pages of each sequence in order; ``kv_lens`` ``[batch]``: its
     keys, the new tokens' among them (written before the call); ``q_starts`` ``[batch + 1]``: its new
-    tokens are rows ``q_starts[b]`` to ``q_starts[b + 1]`` of q, the last of its keys (None: one each).
+    tokens are rows ``q_starts[b]`` to ``q_starts[b + 1]`` of q, the last of its keys (None: one each); it
+    does not descend.
     ``max_new``: the most new tokens of any sequence (default: 1 without q_starts, else all of them).
 
     A token sees the keys up to its own position; if not ``causal``, those after it too.  A positive ``window``
@@ -190,12 +191,13 @@ def paged_attention(q, cache: PagedCache, page_table, kv_lens, q_starts=None, *,
 
 
 _OPERATORS = ("rotary", "cache_write", "cache_read", "paged_attention")
-_SITES = {1: "slot", 2: "position", 3: "page", 4: "length"}
+_SITES = {1: "slot", 2: "position", 3: "page", 4: "length", 6: "q_starts"}
 
 
 def check(device="cuda") -> None:
     """Synchronise the current stream and raise if a serving operator met an index out of range since the
-    last check (its row or token was skipped), or a bounded wait of a kernel ran out."""
+    last check (its row or token was skipped; turned by a position out of range, a row became NaN; with
+    ``q_starts`` in descending order attention did nothing), or a bounded wait of a kernel ran out."""
     device = torch.device(device)
     if device.index is None:
         device = torch.device(device.type, torch.cuda.current_device())
@@ -206,6 +208,6 @@ def check(device="cuda") -> None:
         if code.value == 1:
             _native.forget()  # a kernel that gave up may have left its counters as they were
         op, site = _OPERATORS[where.value // 16 % 4], where.value % 16
-        what = f"{_SITES[site]} out of range" if site in _SITES else f"wait timeout (site {site})"
+        what = f"{_SITES[site]} out of range" if code.value == 2 else f"wait timeout (site {site})"
         raise rt.RuntimeError_(rc, f"{op}: {what}")
     rt.check(rc, "tj_b200_serving_status")

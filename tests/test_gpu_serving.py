@@ -537,3 +537,26 @@ def test_windows_as_long_as_integers_go(window, causal, cache_dtype):
     _agree(case, decode=True, window=window, causal=causal)
     case = _case([(200, 200), (1, 5000), (90, 3000)], 8, 2, 128, "bf16", cache_dtype, seed=34)
     _agree(case, max_new=200, window=window, causal=causal)
+
+
+@pytest.mark.parametrize("new,max_new", [(40, 1), (300, 300)])
+@pytest.mark.parametrize("cache_dtype", ["bf16", "i8"])
+def test_token_ranges_out_of_order_or_range(new, max_new, cache_dtype):
+    """Descending q_starts: nothing is written and the fault is recorded; beyond q: the rows that there are, and a
+    record.  A cut call after it on the same stream finds its counters at zero.  (max_new 1: the kernel of few rows.)"""
+    q, cache, table, lens, starts = _case([(new, 3000), (new, 4000), (new, 3500), (new, 2500)], 8, 2, 64, "bf16", cache_dtype, seed=35)
+    good = serving.paged_attention(q, cache, table, lens, starts, max_new=max_new)
+    serving.check()
+    for bad in ([0, 4 * new, 0, 4 * new, 0], [0, new, new, 3 * new, 2 * new], [7, 6, 7, 8, 9]):
+        out = torch.full_like(q, 3.0)
+        serving.paged_attention(q, cache, table, lens, torch.tensor(bad, device="cuda"), max_new=max_new, out=out)
+        with pytest.raises(rt.RuntimeError_, match="paged_attention: q_starts"):
+            serving.check()
+        assert (out == 3.0).all()
+    for _ in range(3):
+        assert torch.equal(serving.paged_attention(q, cache, table, lens, starts, max_new=max_new), good)
+    long = torch.tensor([-3, new, 2 * new, 3 * new, 4 * new + 9], device="cuda")
+    got = serving.paged_attention(q, cache, table, lens, long, max_new=max_new)
+    with pytest.raises(rt.RuntimeError_, match="paged_attention: q_starts"):
+        serving.check()
+    assert torch.equal(got, good)
