@@ -283,6 +283,11 @@ TJ_API int tj_b200_paged_attention(const tj_paged_attention* args, void* stream)
 TJ_API int tj_b200_paged_attention_workspace(const tj_paged_attention* args, int64_t* workspace_bytes,
                                              int64_t* counters_count);
 
+/* 64-bit indices [rows, cols] as contiguous 32-bit ones; what does not fit becomes -(2^31 - 1) or 2^31 - 1, out of
+ * every range that the operators check. */
+TJ_API int tj_b200_narrow_indices(const int64_t* src, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride,
+                                  int32_t* dst, void* stream);
+
 /* Waits for `stream`, reads the serving operators' status words of the current device and clears
  * them: TJ_OK and *code = 0, or TJ_ERR_DEVICE_STATUS with *code (1 wait timeout, 2 index out of range)
  * and *where = operator * 16 + site (operators 0 rotary, 1 write, 2 read, 3 attention; with code 2 the sites

@@ -360,6 +360,15 @@ __global__ void __launch_bounds__(128) read_kernel(const __grid_constant__ ReadP
   }
 }
 
+// 64-bit indices as 32-bit ones.  What does not fit saturates, so that it stays out of every range that the operators
+// check; cut off to its low half it would be another, valid index.
+__global__ void __launch_bounds__(256) narrow_kernel(const int64_t* src, long n, long cols, long row_stride, long col_stride, int32_t* dst) {
+  const long i = static_cast<long>(blockIdx.x) * 256 + threadIdx.x;
+  if (i >= n) return;
+  const long r = i / cols, c = i - r * cols, v = src[r * row_stride + c * col_stride];
+  dst[i] = static_cast<int32_t>(max(-0x7fffffffL, min(0x7fffffffL, v)));
+}
+
 struct Setup {
   std::once_flag once;
   Device dev{};
@@ -529,6 +538,19 @@ extern "C" int tj_b200_cache_read(const tj_kv_cache* cache, const int32_t* slots
     launch_read<__half>(p, g, st);
   else
     launch_read<__nv_bfloat16>(p, g, st);
+  return launched(name);
+}
+
+extern "C" int tj_b200_narrow_indices(const int64_t* src, int64_t rows, int64_t cols, int64_t row_stride, int64_t col_stride, int32_t* dst,
+                                      void* stream) {
+  using namespace tjs;
+  const char* name = "tj_b200_narrow_indices";
+  if (rows < 0 || cols < 0) return refuse(TJ_ERR_INVALID, name, "negative extent");
+  if (rows == 0 || cols == 0) return TJ_OK;
+  if (!src || !dst) return refuse(TJ_ERR_INVALID, name, "NULL pointer");
+  if (rows > 0x7fffffffLL * 256 / cols) return refuse(TJ_ERR_INVALID, name, "too many indices");
+  narrow_kernel<<<static_cast<unsigned>((rows * cols + 255) / 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(src, rows * cols, cols, row_stride,
+                                                                                                               col_stride, dst);
   return launched(name);
 }
 

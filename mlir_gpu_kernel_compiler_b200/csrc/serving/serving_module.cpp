@@ -26,6 +26,7 @@ struct Api {
   decltype(&tj_b200_cache_read) read;
   decltype(&tj_b200_paged_attention) attention;
   decltype(&tj_b200_paged_attention_workspace) attention_workspace;
+  decltype(&tj_b200_narrow_indices) narrow;
   decltype(&tj_b200_last_error) last_error;
 } api;
 PyObject* runtime_error = nullptr;  // runtime.RuntimeError_
@@ -104,13 +105,24 @@ const at::Tensor& tensor(PyObject* o, const char* name, int64_t dim, Types types
   return t;
 }
 
+void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream(); }
+
+// 64-bit indices as 32-bit ones, those that do not fit still out of range
+at::Tensor narrowed(const at::Tensor& t) {
+  const at::Tensor to = at::empty(t.sizes(), t.options().dtype(at::kInt));
+  const bool vector = t.dim() == 1;
+  const c10::cuda::CUDAGuard guard(t.device());
+  launched(api.narrow(t.data_ptr<int64_t>(), vector ? 1 : t.size(0), t.size(t.dim() - 1), vector ? 0 : t.stride(0), t.stride(t.dim() - 1),
+                      to.data_ptr<int32_t>(), stream_of(t.get_device())));
+  return to;
+}
+
 // a vector of 32-bit indices, contiguous
 at::Tensor indices(PyObject* o, const char* name, int device, int64_t size) {
   const at::Tensor& t = tensor(o, name, 1, INDEX, device);
   if (size >= 0 && t.size(0) != size)
     BAD("%s: expected %lld entries, got %lld", name, static_cast<long long>(size), static_cast<long long>(t.size(0)));
-  if (t.scalar_type() == at::kInt && t.is_contiguous()) return t;
-  return t.to(at::kInt).contiguous();
+  return t.scalar_type() == at::kLong ? narrowed(t) : t.contiguous();
 }
 
 bool rows_fit(const at::Tensor& t) {
@@ -182,8 +194,6 @@ PyObject* describe(PyObject* const* a) {
   i.device = dev;
   return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&i), sizeof(i));
 }
-
-void* stream_of(int device) { return c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream(); }
 
 // table and positions into the arguments; the tensors that hold them
 struct Turn {
@@ -388,7 +398,10 @@ PyObject* attention(PyObject* const* a) {
   if ((cache.c.dtype == TJ_F16 || cache.c.dtype == TJ_BF16) && cache.c.dtype != p.dtype)
     BAD("q is %s and the cache %s: a 16-bit cache must have q's dtype", dtype_text(q.scalar_type()), cache.c.dtype == TJ_F16 ? "torch.float16" : "torch.bfloat16");
   at::Tensor table = tensor(a[2], "page_table", 2, INDEX, dev);
-  if (table.scalar_type() != at::kInt || table.stride(1) != 1) table = table.to(at::kInt).contiguous();
+  if (table.scalar_type() == at::kLong)
+    table = narrowed(table);
+  else if (table.stride(1) != 1)
+    table = table.contiguous();
   p.batch = table.size(0);
   p.table_width = table.size(1);
   p.table_row = table.stride(0);
@@ -450,6 +463,7 @@ PyObject* init(PyObject* const* a) {
   get(api.read, "tj_b200_cache_read");
   get(api.attention, "tj_b200_paged_attention");
   get(api.attention_workspace, "tj_b200_paged_attention_workspace");
+  get(api.narrow, "tj_b200_narrow_indices");
   get(api.last_error, "tj_b200_last_error");
   Py_XDECREF(runtime_error);
   runtime_error = Py_NewRef(a[1]);

@@ -26,7 +26,7 @@ EXPORTS = (
     "tj_b200_driver_available", "tj_b200_time_kernels", "tj_b200_linear_f32_noalloc",
     "tj_b200_linear_f32_noalloc_status", "tj_b200_ipc_export", "tj_b200_ipc_open", "tj_b200_ipc_close",
     "tj_b200_set_pdl", "tj_b200_rotary", "tj_b200_cache_write", "tj_b200_cache_read", "tj_b200_paged_attention",
-    "tj_b200_paged_attention_workspace", "tj_b200_serving_status",
+    "tj_b200_paged_attention_workspace", "tj_b200_narrow_indices", "tj_b200_serving_status",
 )
 
 
@@ -114,6 +114,7 @@ def library(path: str | Path | None = None) -> ctypes.CDLL:
         lib.tj_b200_cache_read.argtypes = [ctypes.c_char_p, vp, ctypes.c_int64, vp, vp, i32, vp]
         lib.tj_b200_paged_attention_workspace.argtypes = [ctypes.c_char_p, ctypes.POINTER(ctypes.c_int64),
                                                           ctypes.POINTER(ctypes.c_int64)]
+        lib.tj_b200_narrow_indices.argtypes = [vp, *[ctypes.c_int64] * 4, vp, vp]
         lib.tj_b200_serving_status.argtypes = [ctypes.POINTER(i32), ctypes.POINTER(i32), vp]
         lib.tj_b200_set_pdl.argtypes = [vp, i32]
         lib.tj_b200_set_pdl.restype = ctypes.c_int

@@ -14,7 +14,8 @@ Tensors are ``[tokens, heads, head_dim]``; any strides whose rows are contiguous
 tensors' device and return without waiting.  As in ``B200Program``, a wrong type raises
 ``TypeError``, a wrong shape, dtype or device ``ValueError``, a failed launch
 ``runtime.RuntimeError_``; a slot, position, page or length out of range is seen by the device alone,
-which skips it and records it: ``check()`` raises for it.
+which skips it and records it: ``check()`` raises for it.  Indices are int32; int64 ones are narrowed by a launch
+of their own.
 
 Each operator is a C entry point of ``include/tj_b200.h`` over hand-written sm_100a kernels in
 ``csrc/serving``.

@@ -560,3 +560,43 @@ def test_token_ranges_out_of_order_or_range(new, max_new, cache_dtype):
     with pytest.raises(rt.RuntimeError_, match="paged_attention: q_starts"):
         serving.check()
     assert torch.equal(got, good)
+
+
+@pytest.mark.parametrize("wrap", [2**32, -(2**32), 2**62])
+def test_64_bit_indices_do_not_wrap(wrap):
+    """An index whose low half is valid is out of range all the same: skipped and recorded, negative slots skipped."""
+    cache = serving.PagedCache.empty(4, 16, 2, 64, "bf16")
+    x = _randn(3, 2, 64, dtype=torch.bfloat16)
+    slots = torch.tensor([[7, 0], [5 + wrap, 0], [9, 0]], device="cuda")[:, 0]  # strided too
+    serving.cache_write(cache, x, x, slots)
+    if wrap > 0:
+        with pytest.raises(rt.RuntimeError_, match="cache_write: slot"):
+            serving.check()
+    assert torch.equal(cache.k[0, 7], x[0]) and torch.equal(cache.v[0, 9], x[2]) and (cache.k[0, 5] == 0).all()
+    cache.k[0, 5] = 1.0
+    back = serving.cache_read(cache, slots)[0]
+    if wrap > 0:
+        with pytest.raises(rt.RuntimeError_, match="cache_read: slot"):
+            serving.check()
+    assert torch.equal(back[0], x[0]) and (back[1] == 0).all() and torch.equal(back[2], x[2])
+    turned, _ = serving.rotary(x, None, slots, serving.rotary_table(64, 16))
+    with pytest.raises(rt.RuntimeError_, match="rotary: position"):
+        serving.check()
+    assert turned[0].isfinite().all() and turned[1].isnan().all() and turned[2].isfinite().all()
+    case = _case([(1, 100), (1, 40)], 4, 2, 64, seed=36)
+    q, cache, table, lens, starts = case
+    want = serving.paged_attention(q, cache, table, lens)
+    wide = torch.stack((table.long(), table.long()), 2)[..., 1]
+    assert torch.equal(serving.paged_attention(q, cache, wide, lens.long(), starts.long(), max_new=1), want)
+    for what in ("page", "length", "q_starts"):
+        t, n, s = table.long(), lens.long(), starts.long()
+        if what == "page":
+            t[1, 0] += wrap
+        elif what == "length":
+            n[1] += wrap
+        else:
+            s[2] += wrap
+        got = serving.paged_attention(q, cache, t, n, s, max_new=1)
+        with pytest.raises(rt.RuntimeError_, match=f"paged_attention: {what}"):
+            serving.check()
+        assert (what == "q_starts" and wrap < 0) or torch.equal(got[0], want[0])

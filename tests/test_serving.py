@@ -126,3 +126,11 @@ def test_attention_refuses_cache_rows_that_only_start_on_8_bytes(strides):
                           1 << 40, 1 << 30) + _cache(strides=strides)
     assert lib.tj_b200_paged_attention(args, None) == rt.TJ_ERR_INVALID and b"16-byte" in lib.tj_b200_last_error()
     assert lib.tj_b200_paged_attention_workspace(args, ctypes.byref(size), ctypes.byref(count)) == rt.TJ_ERR_INVALID
+
+
+def test_c_entry_refuses_bad_index_arrays():
+    lib = rt.library()
+    for args, why in [((4096, -1, 4, 4, 1, 4096), b"negative"), ((4096, 4, -1, 4, 1, 4096), b"negative"), ((0, 2, 2, 2, 1, 4096), b"NULL"),
+                      ((4096, 2, 2, 2, 1, 0), b"NULL"), ((4096, 1 << 40, 1 << 20, 2, 1, 4096), b"too many")]:
+        assert lib.tj_b200_narrow_indices(*args, None) == rt.TJ_ERR_INVALID and why in lib.tj_b200_last_error(), why
+    assert lib.tj_b200_narrow_indices(None, 0, 3, 3, 1, None, None) == rt.TJ_OK
