@@ -258,7 +258,8 @@ TJ_API int tj_b200_cache_read(const tj_kv_cache* cache, const int32_t* slots, in
  * window > 0: none before the last `window` up to its own position (without causal, those after it all the
  * same).  A row that sees nothing is 0 (lse: -inf).
  * counters: int32, zero before the first call and left zero by every call; workspace: anything.
- * Calls that share them must not overlap.  max_new: no sequence has more new tokens. */
+ * Calls that share them must not overlap.  max_new: no sequence has more new tokens (above `tokens`: not
+ * known); it helps to choose the kernel and nothing else. */
 typedef struct tj_paged_attention {
   const void* q;  /* [tokens, q_heads, dim], the 16-bit type `dtype` */
   void* out;      /* the same */

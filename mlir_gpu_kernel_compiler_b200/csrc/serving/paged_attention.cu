@@ -39,9 +39,18 @@ Plan plan(const tj_paged_attention& a, const Device& dev) {
   const long group = a.q_heads / a.cache.heads;
   const bool q8 = a.cache.dtype == TJ_I8 || a.cache.dtype == TJ_E4M3;
   // Sizes if every sequence has max_new tokens over 4096 keys, or a window's, as lengths are known to the
-  // device only: neither tokens of no sequence nor a table's width decide, so they change no bit either.
+  // device only: neither tokens of no sequence nor a table's width decide, so they change no bit either.  Where
+  // max_new is not known (above the number of tokens), they are what all tokens can come to, those of no sequence
+  // among them, if each sequence has one and some have the rest: 64 single tokens are 64 row tiles, not 64 x 64
+  // tokens' (over 4096 keys each, 32 heads on 8 of 128: 193 us for the 237 of the other kernel, in 8 bits 143 for
+  // 376; 63 single tokens and a chunk of 512 in 8 bits 323, and 556 if max_new says 512).
+  const bool known = a.max_new <= a.tokens;
   const long new_max = std::min(a.max_new, a.tokens), packed = new_max * group;
-  const double row_tiles = static_cast<double>(a.batch) * static_cast<double>((packed + 15) / 16);
+  const auto tiles_of = [&](long per) {
+    const long all = a.batch * ((packed + per - 1) / per), rest = std::max<long>(a.tokens - a.batch, 0) * group;
+    return static_cast<double>(known ? all : std::min(all, a.batch * ((group + per - 1) / per) + (rest + per - 1) / per));
+  };
+  const double row_tiles = tiles_of(16);
   // Tokens of one tile of 16 rows take the kernel of few rows.  More do while it passes over less: it reads
   // the keys once for 16 rows, the other once for 256, but starts, joins and ends in 25 us more (16-bit
   // caches) or 30 (8-bit ones, whose keys it also converts, at four times the cost).  Few rows against many, us:
@@ -50,9 +59,9 @@ Plan plan(const tj_paged_attention& a, const Device& dev) {
   //   8-bit, dim 128   1 x 32 over 4096 37, 55          1 x 64 56, 68   1 x 128 84, 68
   //                    8 x 16 over 2048 57, 57          16 x 8 over 8192 132, 232
   //   16-bit, dim 64   1 x 32 over 4096 25, 33          1 x 64 40, 42   1 x 128 59, 42
-  const double keys = a.window > 0 ? static_cast<double>(a.window) + new_max : 4096;
+  const double keys = a.window > 0 ? static_cast<double>(a.window) + (known ? new_max : a.tokens / std::max<long>(a.batch, 1)) : 4096;
   const double pass = a.cache.heads * keys * static_cast<double>(a.cache.dim + 64) / 192;
-  const double many_tiles = static_cast<double>(a.batch) * static_cast<double>((packed + TILE_ROWS - 1) / TILE_ROWS);
+  const double many_tiles = tiles_of(TILE_ROWS);
   p.tiles = packed > 16 && row_tiles * pass > (q8 ? 500e3 + 3.6 * many_tiles * pass : 250e3 + many_tiles * pass);
   if (p.tiles) {
     p.rows = TILE_ROWS;

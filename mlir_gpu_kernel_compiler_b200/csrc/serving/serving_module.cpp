@@ -416,7 +416,7 @@ PyObject* attention(PyObject* const* a) {
   } else if (p.tokens != p.batch) {
     BAD("without q_starts there is one token to a sequence: %lld tokens, %lld sequences", static_cast<long long>(p.tokens), static_cast<long long>(p.batch));
   }
-  p.max_new = a[5] != Py_None ? PyLong_AsLongLong(a[5]) : p.q_starts ? std::max<int64_t>(p.tokens, 1) : 1;
+  p.max_new = a[5] != Py_None ? PyLong_AsLongLong(a[5]) : p.q_starts ? INT64_MAX : 1;
   p.window = PyLong_AsLongLong(a[8]);
   p.scale = a[6] != Py_None ? PyFloat_AsDouble(a[6]) : 1.0 / std::sqrt(static_cast<double>(dim));
   p.causal = PyObject_IsTrue(a[7]);

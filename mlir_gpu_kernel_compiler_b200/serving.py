@@ -177,7 +177,8 @@ def paged_attention(q, cache: PagedCache, page_table, kv_lens, q_starts=None, *,
     keys, the new tokens' among them (written before the call); ``q_starts`` ``[batch + 1]``: its new
     tokens are rows ``q_starts[b]`` to ``q_starts[b + 1]`` of q, the last of its keys (None: one each); it
     does not descend.
-    ``max_new``: the most new tokens of any sequence (default: 1 without q_starts, else all of them).
+    ``max_new``: the most new tokens of any sequence (default: 1 without q_starts, else not known).  It helps to
+    choose the kernel and nothing else; with it, rows of no sequence change no bit of the others.
 
     A token sees the keys up to its own position; if not ``causal``, those after it too.  A positive ``window``
     hides the keys before the last ``window`` up to its own position (its own among them), and, without the

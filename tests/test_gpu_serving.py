@@ -600,3 +600,20 @@ def test_64_bit_indices_do_not_wrap(wrap):
         with pytest.raises(rt.RuntimeError_, match=f"paged_attention: {what}"):
             serving.check()
         assert (what == "q_starts" and wrap < 0) or torch.equal(got[0], want[0])
+
+
+@pytest.mark.parametrize("cache_dtype", ["bf16", "i8"])
+def test_single_tokens_without_max_new_take_the_kernel_of_few_rows(cache_dtype):
+    """q_starts alone do not say how many new tokens a sequence has; single tokens are still not planned as if each
+    had all of them, so the bits are those of the call without q_starts.  With max_new given, rows of no sequence
+    change no bit."""
+    q, cache, table, lens, starts = _case([(1, 100 + 61 * i) for i in range(64)], 32, 8, 128, "bf16", cache_dtype, seed=37)
+    want = serving.paged_attention(q, cache, table, lens)
+    assert torch.equal(serving.paged_attention(q, cache, table, lens, starts), want)
+    for new in (1, 33, 64):
+        case = _case([(new, 900), (1, 400)], 32, 8, 128, "bf16", cache_dtype, seed=38)
+        _agree(case)
+        q, cache, table, lens, starts = case
+        want = serving.paged_attention(q, cache, table, lens, starts, max_new=new)
+        padded = serving.paged_attention(torch.cat((q, q[:1].expand(70, -1, -1))), cache, table, lens, starts, max_new=new)
+        assert torch.equal(padded[: new + 1], want)
