@@ -15,10 +15,12 @@
 // two keys' elements are paired by a byte permutation.  The pieces of a row are permuted by its number
 // so that both ways of reading are free of bank conflicts.
 //
-// An 8-bit cache's codes become f16, bf16 queries too (times the power of two that brings the tile's
-// largest element near 2^14: exact but for elements 2^-28 of that): the byte permutations and masks run
+// An 8-bit cache's codes become f16, bf16 queries too (times a power of two that brings the largest element
+// near 2^14; f16 is exact to 2^-28 of that): the byte permutations and masks run
 // at half rate and were the bound, and bf16 needs three for a pair of codes where f16 needs 1.5 (keys) and
-// 2 (values).
+// 2 (values).  The rows of a tile are different tokens and heads.  While their largest elements are within 2^12 of
+// one another they share the power, and no row loses more than 2^-16 - 2^-24 below its own largest, which is under
+// the f32 error of its score; otherwise each has its own, at a multiplication a score.
 //
 // A CTA's warps take blocks of KS keys of its chunk in turn, with a running maximum and sum each; their
 // results are joined at the end, and the chunks of a row tile by the CTA that
@@ -228,24 +230,40 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
   }
 
   float score_scale = p.scale_log2;
+  bool apart = false;  // the same for the warp: the rows' scores are to be multiplied by s_m (free until the end)
   if constexpr (!std::is_same<T, C>::value) {
-    uint32_t top = 0;  // the largest element of all rows, as bits
+    uint32_t top[2] = {0, 0};  // this thread's rows' largest elements, as bits
 #pragma unroll
     for (int c = 0; c < KC * STEPS; ++c)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) top = max(top, max((qa[c][e] & 0x7fffu) << 16, qa[c][e] & 0x7fff0000u));
-    top = __reduce_max_sync(0xffffffffu, top);
-    // 2^(14 - its exponent), within what f32 holds twice over; 1 for zeros, infinities and NaN
-    const int raise = min(14 - (static_cast<int>(top >> 23) - 127), 100);
-    const bool fine = top >= 0x00800000u && top < 0x7f800000u;
-    const float up = fine ? __int_as_float((127 + raise) << 23) : 1.0f;
-    score_scale *= fine ? __int_as_float((127 - raise) << 23) : 1.0f;
+      for (int e = 0; e < 4; ++e) top[e & 1] = max(top[e & 1], max((qa[c][e] & 0x7fffu) << 16, qa[c][e] & 0x7fff0000u));
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+      top[i] = max(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+    }
+    // rows of zeros (or that are not there) go with any power
+    const uint32_t most = __reduce_max_sync(0xffffffffu, max(top[0], top[1]));
+    const uint32_t least = __reduce_min_sync(0xffffffffu, min(top[0] ? top[0] : most, top[1] ? top[1] : most));
+    apart = most >= 0x7f800000u || (most >> 23) > (least >> 23) + 12;
+    float up[2], down = 1.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      // 2^(14 - the exponent), within what f32 holds twice over; 1 for zeros, infinities and NaN
+      const uint32_t x = apart ? top[i] : most;
+      const int raise = x > 0 && x < 0x7f800000u ? min(14 - (static_cast<int>(x >> 23) - 127), 100) : 0;
+      up[i] = __int_as_float((127 + raise) << 23);
+      down = __int_as_float((127 - raise) << 23);
+      if (apart && t == 0) s_m[warp][g + 8 * i] = down;
+    }
+    if (!apart) score_scale *= down;
+    __syncwarp();
 #pragma unroll
     for (int c = 0; c < KC * STEPS; ++c)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         uint32_t& w = qa[c][e];
-        w = tj_pack_f16x2(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up);
+        w = tj_pack_f16x2(__uint_as_float(w << 16) * up[e & 1], __uint_as_float(w & 0xffff0000u) * up[e & 1]);
       }
   }
 
@@ -300,6 +318,15 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
           }
           mma16816<C>(sc[j], qa[c * STEPS + e], b0, b1);
         }
+      }
+    }
+    if constexpr (!std::is_same<T, C>::value) {
+      if (apart) {
+        const float down[2] = {s_m[warp][g], s_m[warp][g + 8]};
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sc[j][e] *= down[e >> 1];
       }
     }
     // t = scaled score (8-bit cache: + log2 vs); masked keys -inf

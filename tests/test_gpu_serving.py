@@ -617,3 +617,25 @@ def test_single_tokens_without_max_new_take_the_kernel_of_few_rows(cache_dtype):
         want = serving.paged_attention(q, cache, table, lens, starts, max_new=new)
         padded = serving.paged_attention(torch.cat((q, q[:1].expand(70, -1, -1))), cache, table, lens, starts, max_new=new)
         assert torch.equal(padded[: new + 1], want)
+
+
+@pytest.mark.parametrize("factor", [2.0**40, 2.0**-60, 2.0**120, math.inf, math.nan])
+@pytest.mark.parametrize("cache_dtype,dim", [("i8", 128), ("e4m3", 64), ("bf16", 128)])
+@pytest.mark.parametrize("max_new", [1, 200])
+def test_a_token_of_another_size_does_not_reach_the_others(factor, cache_dtype, dim, max_new):
+    """Rows of other tokens and heads share a tile: however large, small or broken one token's query is, or one head's, the
+    others' results do not know.  (max_new 1: the kernel of few rows.)"""
+    q, cache, table, lens, starts = _case([(3, 500), (1, 333), (5, 5), (40, 700), (200, 900)], 8, 2, dim, "bf16", cache_dtype, seed=40)
+    q[1] *= factor
+    q[3, 2] *= factor
+    q[12, :, 3] *= factor
+    plain = torch.ones(q.shape[:2], dtype=torch.bool, device="cuda")
+    if factor > 1 or factor != factor:
+        plain[1], plain[3, 2], plain[12] = False, False, False
+    out, lse = serving.paged_attention(q, cache, table, lens, starts, max_new=max_new, return_lse=True)
+    want, want_lse, size = _attend64(q, cache, table, lens, starts)
+    off = (out.double() - want).abs() - (U[q.dtype] * (want.abs() + size) + 2e-5 * size)
+    assert (off[plain] <= 0).all(), off[plain].max().item()
+    assert ((lse.double() - want_lse).abs()[plain] <= 2e-5 * want_lse.abs()[plain].clamp(min=1)).all()
+    if not math.isfinite(factor):
+        assert out[1].isnan().all()
