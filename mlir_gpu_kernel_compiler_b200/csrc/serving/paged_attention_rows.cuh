@@ -113,9 +113,8 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int heads = static_cast<int>(p.a.cache.heads);
   const int unit = blockIdx.x / heads, h = blockIdx.x - unit * heads;
+  if (blockIdx.x == 0) report_sequences(p, threadIdx.x, R::THREADS);
   const Piece w = find_piece(p, unit, 16, WARPS * KS);
-  if (blockIdx.x == 0)
-    for (int b = threadIdx.x; b < p.a.batch; b += R::THREADS) report_sequence(p, b);
   if (!w.some) return;
   const Seq s = sequence(p, w.b);
   const int rows = min(16, s.n * p.group - w.tile * 16);

@@ -22,6 +22,7 @@
 //              clocks a block: a wait for a barrier takes 140 clocks even when it is over, as it queues
 //              behind the softmax warps' exponentials.)
 //   14         looks the next segment up.
+//   15         of the first CTA: records faulty lengths and token ranges.
 //
 // Measured: 2048 tokens over 16384 bf16 keys, 32 heads of 128 on 8 cached ones, 493 us = 1045 TFLOP/s (64 % of
 // the measured matrix rate) in short runs and 568 us under the board's power limit, where variants that
@@ -88,7 +89,6 @@ TJ_DEV long total_work(const AttnParams& p) {
   for (int b = lane; b < p.a.batch; b += 32) {
     mine += tile_work(p, sequence(p, b)).per_head;
     turned |= descending(p, b);
-    if (blockIdx.x == 0 && threadIdx.x < 32) report_sequence(p, b);
   }
   if (__any_sync(0xffffffffu, turned)) return 0;
 #pragma unroll
@@ -837,6 +837,7 @@ __global__ void __launch_bounds__(512, 1) attention_tiles(const __grid_constant_
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const S sh(smem_raw);
   const int warp = threadIdx.x >> 5;
+  if (blockIdx.x == 0 && warp == 15) report_sequences(p, threadIdx.x & 31, 32);  // a warp that has nothing else to do
   const long total = total_work(p);
   if (total == 0) return;
   const Cut cut = cut_work(p, total, gridDim.x);
