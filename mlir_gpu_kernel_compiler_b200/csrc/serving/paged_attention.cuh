@@ -168,6 +168,12 @@ TJ_DEV float exp2_fast(float x) {
 // normal numbers below 2^-14, and a key whose probability is small can have the larger value.
 template <class T> constexpr float P_SHIFT = 0.0f;
 template <> constexpr float P_SHIFT<__half> = 14.0f;
+// So P = 2^(t - base), and a row's base is what the kernels keep in place of its maximum: the maximum less the shift,
+// or the maximum itself where f32's steps at that size (4 at 2^25) make more of the shift than f16 has room for.
+TJ_DEV float base_of(float top, float shift) {
+  const float b = top - shift;
+  return top - b > shift + 1.0f ? top : b;
+}
 
 template <class T> TJ_DEV uint32_t pack2(float lo, float hi);
 template <> TJ_DEV uint32_t pack2<__nv_bfloat16>(float lo, float hi) { return tj_pack_bf16x2(lo, hi); }

@@ -272,167 +272,176 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
   float o[OT][4];
 #pragma unroll
   for (int i = 0; i < OT; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};  // bases and sums
 
-  int stage = 0;
-  for (int base = first; base < k1; base += WARPS * KS) {
-    {
-      const int now = page;
-      page = page_of(ahead + WARPS * KS);
-      fetch(stage == 0 ? STAGES - 1 : stage - 1, ahead, now);
-      ahead += WARPS * KS;
-    }
-    asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
-    __syncwarp();
-    const uint32_t kblock = my_ring + stage * R::BLOCK, vblock = kblock + KS * R::ROW;
-    float* const scale = reinterpret_cast<float*>(ring + warp * R::WARP + STAGES * R::BLOCK) + stage * KS * 3;
-    if constexpr (Q8) {
-      scale[lane] *= score_scale;
-      const float lv = log2_scale(scale[KS + lane]);
-      scale[KS + lane] = lv;
-      scale[2 * KS + lane] = exp2_fast(-lv);
+  // The warp's blocks of keys.  The loop exists twice where rows may have powers of their own: a test inside it costs
+  // tiles of like rows as much as the multiplication (64 single tokens over 4096 keys of 8 bits: 152 us for 136).
+  const auto walk = [&](auto powers) __attribute__((always_inline)) {
+    int stage = 0;
+    for (int base = first; base < k1; base += WARPS * KS) {
+      {
+        const int now = page;
+        page = page_of(ahead + WARPS * KS);
+        fetch(stage == 0 ? STAGES - 1 : stage - 1, ahead, now);
+        ahead += WARPS * KS;
+      }
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
       __syncwarp();
-    }
-    if (++stage == STAGES) stage = 0;
+      const uint32_t kblock = my_ring + stage * R::BLOCK, vblock = kblock + KS * R::ROW;
+      float* const scale = reinterpret_cast<float*>(ring + warp * R::WARP + STAGES * R::BLOCK) + stage * KS * 3;
+      if constexpr (Q8) {
+        scale[lane] *= score_scale;
+        const float lv = log2_scale(scale[KS + lane]);
+        scale[KS + lane] = lv;
+        scale[2 * KS + lane] = exp2_fast(-lv);
+        __syncwarp();
+      }
+      if (++stage == STAGES) stage = 0;
 
-    // the tiles' products are independent chains, so they go side by side
-    float sc[NT][4];
+      // the tiles' products are independent chains, so they go side by side
+      float sc[NT][4];
 #pragma unroll
-    for (int j = 0; j < NT; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
+      for (int j = 0; j < NT; ++j) sc[j][0] = sc[j][1] = sc[j][2] = sc[j][3] = 0.0f;
 #pragma unroll
-    for (int c = 0; c < KC; ++c) {
-      uint4 kf[NT];
+      for (int c = 0; c < KC; ++c) {
+        uint4 kf[NT];
 #pragma unroll
-      for (int j = 0; j < NT; ++j) kf[j] = lds16(kblock + (key_at ^ (c << 6)) + 8 * j * R::ROW);
+        for (int j = 0; j < NT; ++j) kf[j] = lds16(kblock + (key_at ^ (c << 6)) + 8 * j * R::ROW);
 #pragma unroll
-      for (int e = 0; e < STEPS; ++e) {
+        for (int e = 0; e < STEPS; ++e) {
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          uint32_t b0, b1;
-          if constexpr (Q8) {
-            codes4<C, CD>(word(kf[j], e), b0, b1);
-          } else {
-            b0 = word(kf[j], 2 * e);
-            b1 = word(kf[j], 2 * e + 1);
+          for (int j = 0; j < NT; ++j) {
+            uint32_t b0, b1;
+            if constexpr (Q8) {
+              codes4<C, CD>(word(kf[j], e), b0, b1);
+            } else {
+              b0 = word(kf[j], 2 * e);
+              b1 = word(kf[j], 2 * e + 1);
+            }
+            mma16816<C>(sc[j], qa[c * STEPS + e], b0, b1);
           }
-          mma16816<C>(sc[j], qa[c * STEPS + e], b0, b1);
         }
       }
-    }
-    if constexpr (!std::is_same<T, C>::value) {
-      if (apart) {
+      if constexpr (decltype(powers)::value) {
         const float down[2] = {s_m[warp][g], s_m[warp][g + 8]};
 #pragma unroll
         for (int j = 0; j < NT; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) sc[j][e] *= down[e >> 1];
       }
-    }
-    // t = scaled score (8-bit cache: + log2 vs); masked keys -inf
+      // t = scaled score (8-bit cache: + log2 vs); masked keys -inf
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      float2 kfac = make_float2(score_scale, score_scale), lv = make_float2(0.0f, 0.0f);
-      if constexpr (Q8) {
-        kfac = *reinterpret_cast<const float2*>(scale + 8 * j + 2 * t);
-        lv = *reinterpret_cast<const float2*>(scale + KS + 8 * j + 2 * t);
-      }
+      for (int j = 0; j < NT; ++j) {
+        float2 kfac = make_float2(score_scale, score_scale), lv = make_float2(0.0f, 0.0f);
+        if constexpr (Q8) {
+          kfac = *reinterpret_cast<const float2*>(scale + 8 * j + 2 * t);
+          lv = *reinterpret_cast<const float2*>(scale + KS + 8 * j + 2 * t);
+        }
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        float& x = sc[j][e];
-        x = Q8 ? fmaf(x, e & 1 ? kfac.y : kfac.x, e & 1 ? lv.y : lv.x) : x * score_scale;
+        for (int e = 0; e < 4; ++e) {
+          float& x = sc[j][e];
+          x = Q8 ? fmaf(x, e & 1 ? kfac.y : kfac.x, e & 1 ? lv.y : lv.x) : x * score_scale;
+        }
       }
-    }
-    if (base < mlo || base + KS > mhi) {  // the same for the warp
+      if (base < mlo || base + KS > mhi) {  // the same for the warp
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int key = base + 8 * j + 2 * t + (e & 1);
+            if (key < rlo[e >> 1] || key >= rhi[e >> 1]) sc[j][e] = -INFINITY;
+          }
+      }
+      float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int j = 0; j < NT; ++j)
 #pragma unroll
+        for (int i = 0; i < 2; ++i) mx[i] = fmaxf(mx[i], fmaxf(sc[j][2 * i], sc[j][2 * i + 1]));
+      bool moved = false;
+      float from[2], alpha[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
+        mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
+        const float next = fmaxf(m[i], base_of(mx[i], P_SHIFT<C>));
+        moved |= next > m[i];
+        from[i] = next == -INFINITY ? 0.0f : next;
+        alpha[i] = exp2_fast(m[i] - from[i]);
+        m[i] = next;
+      }
+      if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) l[i] *= alpha[i];
+#pragma unroll
+        for (int j = 0; j < OT; ++j) {
+          o[j][0] *= alpha[0];
+          o[j][1] *= alpha[0];
+          o[j][2] *= alpha[1];
+          o[j][3] *= alpha[1];
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < NT; ++j) {
+        float2 inv = make_float2(1.0f, 1.0f);
+        if constexpr (Q8) inv = *reinterpret_cast<const float2*>(scale + 2 * KS + 8 * j + 2 * t);
+#pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int key = base + 8 * j + 2 * t + (e & 1);
-          if (key < rlo[e >> 1] || key >= rhi[e >> 1]) sc[j][e] = -INFINITY;
+          sc[j][e] = exp2_fast(sc[j][e] - from[e >> 1]);
+          l[e >> 1] += Q8 ? sc[j][e] * (e & 1 ? inv.y : inv.x) : sc[j][e];
         }
-    }
-    float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) mx[i] = fmaxf(mx[i], fmaxf(sc[j][2 * i], sc[j][2 * i + 1]));
-    bool moved = false;
-    float base_m[2], alpha[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 1));
-      mx[i] = fmaxf(mx[i], __shfl_xor_sync(0xffffffffu, mx[i], 2));
-      const float next = fmaxf(m[i], mx[i]);
-      moved |= next > m[i];
-      const float from = next == -INFINITY ? 0.0f : next;
-      alpha[i] = exp2_fast(m[i] - from);
-      base_m[i] = from - P_SHIFT<C>;
-      m[i] = next;
-    }
-    if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-      for (int i = 0; i < 2; ++i) l[i] *= alpha[i];
-#pragma unroll
-      for (int j = 0; j < OT; ++j) {
-        o[j][0] *= alpha[0];
-        o[j][1] *= alpha[0];
-        o[j][2] *= alpha[1];
-        o[j][3] *= alpha[1];
       }
-    }
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      float2 inv = make_float2(1.0f, 1.0f);
-      if constexpr (Q8) inv = *reinterpret_cast<const float2*>(scale + 2 * KS + 8 * j + 2 * t);
+      for (int k16 = 0; k16 < KS / 16; ++k16) {
+        const uint32_t pa[4] = {pack2<C>(sc[2 * k16][0], sc[2 * k16][1]), pack2<C>(sc[2 * k16][2], sc[2 * k16][3]),
+                                pack2<C>(sc[2 * k16 + 1][0], sc[2 * k16 + 1][1]), pack2<C>(sc[2 * k16 + 1][2], sc[2 * k16 + 1][3])};
+        uint32_t va[VW], vb[VW], vc[VW], vd[VW];  // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the step
+        auto value = [&](uint32_t (&v)[VW], uint32_t at) {
+          if constexpr (VB == 8) {
+            const uint2 x = lds8(vblock + at);
+            v[0] = x.x;
+            v[1] = x.y;
+          } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        sc[j][e] = exp2_fast(sc[j][e] - base_m[e >> 1]);
-        l[e >> 1] += Q8 ? sc[j][e] * (e & 1 ? inv.y : inv.x) : sc[j][e];
-      }
-    }
-#pragma unroll
-    for (int k16 = 0; k16 < KS / 16; ++k16) {
-      const uint32_t pa[4] = {pack2<C>(sc[2 * k16][0], sc[2 * k16][1]), pack2<C>(sc[2 * k16][2], sc[2 * k16][3]),
-                              pack2<C>(sc[2 * k16 + 1][0], sc[2 * k16 + 1][1]), pack2<C>(sc[2 * k16 + 1][2], sc[2 * k16 + 1][3])};
-      uint32_t va[VW], vb[VW], vc[VW], vd[VW];  // keys 2t, 2t + 1, 2t + 8, 2t + 9 of the step
-      auto value = [&](uint32_t (&v)[VW], uint32_t at) {
-        if constexpr (VB == 8) {
-          const uint2 x = lds8(vblock + at);
-          v[0] = x.x;
-          v[1] = x.y;
-        } else {
-#pragma unroll
-          for (int c = 0; c < VC; ++c) {
-            const uint4 x = lds16(vblock + at + c * 128);
-            v[(4 * c) % VW] = x.x;
-            v[(4 * c + 1) % VW] = x.y;
-            v[(4 * c + 2) % VW] = x.z;
-            v[(4 * c + 3) % VW] = x.w;
+            for (int c = 0; c < VC; ++c) {
+              const uint4 x = lds16(vblock + at + c * 128);
+              v[(4 * c) % VW] = x.x;
+              v[(4 * c + 1) % VW] = x.y;
+              v[(4 * c + 2) % VW] = x.z;
+              v[(4 * c + 3) % VW] = x.w;
+            }
           }
-        }
-      };
-      value(va, value_at0 + k16 * 16 * R::ROW);
-      value(vb, value_at1 + k16 * 16 * R::ROW);
-      value(vc, value_at0 + (k16 * 16 + 8) * R::ROW);
-      value(vd, value_at1 + (k16 * 16 + 8) * R::ROW);
+        };
+        value(va, value_at0 + k16 * 16 * R::ROW);
+        value(vb, value_at1 + k16 * 16 * R::ROW);
+        value(vc, value_at0 + (k16 * 16 + 8) * R::ROW);
+        value(vd, value_at1 + (k16 * 16 + 8) * R::ROW);
 #pragma unroll
-      for (int j = 0; j < OT; ++j) {
-        uint32_t b0, b1;
-        if constexpr (Q8) {
-          // byte j % 4 of both keys' words, into both bytes of a half
-          const int n = j & 3;
-          const uint32_t sel = n | (n << 4) | ((n + 4) << 8) | ((n + 4) << 12);
-          b0 = Codes<C, CD>::make(__byte_perm(va[j >> 2], vb[j >> 2], sel));
-          b1 = Codes<C, CD>::make(__byte_perm(vc[j >> 2], vd[j >> 2], sel));
-        } else {
-          const uint32_t sel = (j & 1) ? 0x7632 : 0x5410;
-          b0 = __byte_perm(va[j >> 1], vb[j >> 1], sel);
-          b1 = __byte_perm(vc[j >> 1], vd[j >> 1], sel);
+        for (int j = 0; j < OT; ++j) {
+          uint32_t b0, b1;
+          if constexpr (Q8) {
+            // byte j % 4 of both keys' words, into both bytes of a half
+            const int n = j & 3;
+            const uint32_t sel = n | (n << 4) | ((n + 4) << 8) | ((n + 4) << 12);
+            b0 = Codes<C, CD>::make(__byte_perm(va[j >> 2], vb[j >> 2], sel));
+            b1 = Codes<C, CD>::make(__byte_perm(vc[j >> 2], vd[j >> 2], sel));
+          } else {
+            const uint32_t sel = (j & 1) ? 0x7632 : 0x5410;
+            b0 = __byte_perm(va[j >> 1], vb[j >> 1], sel);
+            b1 = __byte_perm(vc[j >> 1], vd[j >> 1], sel);
+          }
+          mma16816<C>(o[j], pa, b0, b1);
         }
-        mma16816<C>(o[j], pa, b0, b1);
       }
+      __syncwarp();  // the block's place may be filled again
     }
-    __syncwarp();  // the block's place may be filled again
+  };
+  if constexpr (std::is_same<T, C>::value) {
+    walk(std::false_type());
+  } else {
+    if (apart)
+      walk(std::true_type());
+    else
+      walk(std::false_type());
   }
 
   // join the warps
@@ -478,7 +487,7 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
     if (!none) y = make_uint2(pack2<T>(v.x * div, v.y * div), pack2<T>(v.z * div, v.w * div));
     *reinterpret_cast<uint2*>(static_cast<T*>(p.a.out) + tok * p.a.out_token + hd * p.a.out_head + col) = y;
     if (p.a.lse && col == 0)
-      p.a.lse[static_cast<long>(tok) * p.a.q_heads + hd] = none ? -INFINITY : (best - P_SHIFT<C> + log2f(sum)) * 0.69314718055994531f;
+      p.a.lse[static_cast<long>(tok) * p.a.q_heads + hd] = none ? -INFINITY : (best + log2f(sum)) * 0.69314718055994531f;
   };
   const int positions = rows * (D / 4);
   for (int at = threadIdx.x; at < positions; at += R::THREADS) {

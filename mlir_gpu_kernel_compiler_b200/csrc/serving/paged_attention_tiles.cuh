@@ -394,7 +394,6 @@ template <class T, int CD, int D> TJ_DEV bool end_segment(const TilesShared<T, C
 // Joins the tiles that were cut: CTA (c, y) the rows 32 y .. 32 y + 31 of the tile that begins in part c and
 // goes on in part c + 1, if there is one.
 template <class T, int CD, int D> __global__ void __launch_bounds__(256) join_tiles(const __grid_constant__ AttnParams p) {
-  constexpr float SHIFT = Tiles<T, CD, D>::SHIFT;
   __shared__ int s_slots[MAX_PARTS];
   __shared__ int s_whole;
   const long total = total_work(p);
@@ -458,7 +457,7 @@ template <class T, int CD, int D> __global__ void __launch_bounds__(256) join_ti
     y.y = pack2<T>(none ? 0.0f : acc.z * inv, none ? 0.0f : acc.w * inv);
     *reinterpret_cast<uint2*>(static_cast<T*>(p.a.out) + tok * p.a.out_token + hd * p.a.out_head + col) = y;
     if (p.a.lse && col == 0)
-      p.a.lse[static_cast<long>(tok) * p.a.q_heads + hd] = none ? -INFINITY : (best - SHIFT + log2f(sum)) * 0.69314718055994531f;
+      p.a.lse[static_cast<long>(tok) * p.a.q_heads + hd] = none ? -INFINITY : (best + log2f(sum)) * 0.69314718055994531f;
   }
 }
 
@@ -702,8 +701,14 @@ TJ_DEV void softmax(const AttnParams& p, const TilesShared<T, CD, D>& sh, uint32
   // keys that every row of this warp sees need no mask; from here on relative to the segment's first key
   rlo -= g.key0;
   rhi -= g.key0;
-  const int clo = __reduce_max_sync(0xffffffffu, rlo), chi = __reduce_min_sync(0xffffffffu, rhi);
-  float m = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+  int clo = __reduce_max_sync(0xffffffffu, rlo);
+  const int chi = __reduce_min_sync(0xffffffffu, rhi);
+  float base = -INFINITY, l0 = 0.0f, l1 = 0.0f;
+  // Scores of a 16-bit cache go into P by one fused step from their unscaled form.  Where f32's steps are no longer small
+  // (1/8 at 2^20), the product that was not rounded is as much off the base, which was, and P with it: by more than the
+  // 16-bit types and in the end f32 can hold.  From there on (the same for the warp, clo FAR) products are rounded first.
+  constexpr int FAR = INT_MAX;
+  float c = C::Q8 ? 1.0f : p.scale_log2;
   bool ok = true;
   for (int j = 0; j < nb; ++j) {
     const int it = blocks + j, use = tile_blocks + j, kb = j * TILE_KEYS;
@@ -738,6 +743,10 @@ TJ_DEV void softmax(const AttnParams& p, const TilesShared<T, CD, D>& sh, uint32
     const bool masked = kb < clo || kb + TILE_KEYS > chi;  // the same for the warp
     if (masked) {
       const int a = rlo - kb, b = rhi - kb;
+      if (!C::Q8 && clo == FAR) {
+#pragma unroll
+        for (int i = 0; i < 64; ++i) x[i] *= p.scale_log2;
+      }
 #pragma unroll
       for (int i = 0; i < 64; ++i)
         if (i < a || i >= b) x[i] = -INFINITY;
@@ -752,33 +761,41 @@ TJ_DEV void softmax(const AttnParams& p, const TilesShared<T, CD, D>& sh, uint32
     }
     h0 = tja::fmax3(h0, x[60], x[61]);
     h1 = tja::fmax3(h1, x[62], x[63]);
-    const float c = C::Q8 ? 1.0f : p.scale_log2;
     const float top = tja::fmax3(h0, h1, fmaxf(h2, h3)) * c;
     float alpha = 1.0f;
-    const bool raise = top > m + C::RAISE || (m == -INFINITY && top > m);
+    const bool raise = top - base > C::SHIFT + C::RAISE || (base == -INFINITY && top > base);
     if (raise) {
-      alpha = exp2_fast(m - top);
-      m = top;
+      const float next = base_of(top, C::SHIFT);
+      alpha = exp2_fast(base - next);
+      base = next;
       l0 *= alpha;
       l1 *= alpha;
     }
-    if (j > 0 && __any_sync(0xffffffffu, raise)) {
-      // O at rest.  (A phase is waited for only when the one before it is known to be over: the scores
-      // of block j were made after P V of block j - 2.)
-      ok = sh.wait(S::PV_DONE + 8 * (2 * t + ((use - 1) & 1)), (use - 1) >> 1, p, 14);
-      if (!ok) break;
-      tc_fence_after();
-#pragma unroll 1
-      for (int i = 0; i < D; i += 16) {
-        uint32_t o[16];
-        tmem_ld16(tO + i, o);
+    if (__any_sync(0xffffffffu, raise)) {
+      if (!C::Q8 && clo != FAR && __any_sync(0xffffffffu, fabsf(top) >= 0x1p20f && fabsf(top) < INFINITY)) {
 #pragma unroll
-        for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
-        tja::tmem_st16_wait(tO + i, o);
+        for (int i = 0; i < 64; ++i) x[i] *= c;
+        c = 1.0f;
+        clo = FAR;
+      }
+      if (j > 0) {
+        // O at rest.  (A phase is waited for only when the one before it is known to be over: the scores
+        // of block j were made after P V of block j - 2.)
+        ok = sh.wait(S::PV_DONE + 8 * (2 * t + ((use - 1) & 1)), (use - 1) >> 1, p, 14);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll 1
+        for (int i = 0; i < D; i += 16) {
+          uint32_t o[16];
+          tmem_ld16(tO + i, o);
+#pragma unroll
+          for (int k = 0; k < 16; ++k) o[k] = __float_as_uint(__uint_as_float(o[k]) * alpha);
+          tja::tmem_st16_wait(tO + i, o);
+        }
       }
     }
-    const float base = (m == -INFINITY ? 0.0f : m) - C::SHIFT;
-    const uint64_t cc = tja::f2_pack(c, c), nb2 = tja::f2_pack(-base, -base);
+    const float from = base == -INFINITY ? 0.0f : base;
+    const uint64_t cc = tja::f2_pack(c, c), nb2 = tja::f2_pack(-from, -from);
     uint64_t ll = tja::f2_pack(l0, l1);
     probabilities<T, C>(x, cc, nb2, sc, ll, tS);
     tja::f2_unpack(ll, l0, l1);
@@ -790,8 +807,8 @@ TJ_DEV void softmax(const AttnParams& p, const TilesShared<T, CD, D>& sh, uint32
   if (!ok || !sh.wait(S::PV_DONE + 8 * (2 * t + (last & 1)), last >> 1, p, 13)) return;
   tc_fence_after();
   const float l = l0 + l1;
-  if (l != l && m == -INFINITY) m = 0.0f;  // only NaN scores: the row is NaN, not empty
-  const bool none = m == -INFINITY, mine_to_write = r < g.rows;
+  if (l != l && base == -INFINITY) base = 0.0f;  // only NaN scores: the row is NaN, not empty
+  const bool none = base == -INFINITY, mine_to_write = r < g.rows;
   if (nb == g.all) {
     const float inv = none ? 0.0f : 1.0f / l;
     int tok, hd;
@@ -811,7 +828,7 @@ TJ_DEV void softmax(const AttnParams& p, const TilesShared<T, CD, D>& sh, uint32
       }
     }
     if (p.a.lse && mine_to_write)
-      p.a.lse[static_cast<long>(tok) * p.a.q_heads + hd] = none ? -INFINITY : (m - C::SHIFT + log2f(l)) * 0.69314718055994531f;
+      p.a.lse[static_cast<long>(tok) * p.a.q_heads + hd] = none ? -INFINITY : (base + log2f(l)) * 0.69314718055994531f;
   } else {
     const long slot = (2L * blockIdx.x + (g.later ? 0 : 1)) * TILE_ROWS + r;
     float* dst = p.part_o + slot * D;
@@ -824,7 +841,7 @@ TJ_DEV void softmax(const AttnParams& p, const TilesShared<T, CD, D>& sh, uint32
         for (int k = 0; k < 16; k += 4)
           __stcg(reinterpret_cast<uint4*>(dst + i + k), make_uint4(o[k], o[k + 1], o[k + 2], o[k + 3]));
     }
-    if (mine_to_write) __stcg(p.part_ml + slot, make_float2(m, l));
+    if (mine_to_write) __stcg(p.part_ml + slot, make_float2(base, l));
   }
   tc_fence_before();
 }

@@ -639,3 +639,36 @@ def test_a_token_of_another_size_does_not_reach_the_others(factor, cache_dtype, 
     assert ((lse.double() - want_lse).abs()[plain] <= 2e-5 * want_lse.abs()[plain].clamp(min=1)).all()
     if not math.isfinite(factor):
         assert out[1].isnan().all()
+
+
+def _top_scores64(q, cache, table, lens, starts):
+    """Each row's largest score and its distance to the next, of a causal call in 64 bits."""
+    hq, dim = q.shape[1:]
+    top = torch.full((*q.shape[:2], 2), -math.inf, dtype=torch.float64, device="cuda")
+    for b in range(table.shape[0]):
+        n0, n1, c = int(starts[b]), int(starts[b + 1]), int(lens[b])
+        key = torch.arange(c, device="cuda")
+        k = serving.cache_read(cache, table[b].long()[key // cache.page_size] * cache.page_size + key % cache.page_size, "f32")[0].double()
+        s = torch.einsum("nhd,lhd->nhl", q[n0:n1].double(), k.repeat_interleave(hq // cache.kv_heads, 1)) * dim**-0.5
+        top[n0:n1] = s.masked_fill((key > torch.arange(c - n1 + n0, c, device="cuda")[:, None])[:, None], -math.inf).topk(2, -1).values
+    return top[..., 0], top[..., 0] - top[..., 1]
+
+
+@pytest.mark.parametrize("dtype,cache_dtype,grow,scale", [("bf16", "bf16", 2.0**40, 16.0), ("bf16", "i8", 2.0**40, 16.0), ("bf16", "e4m3", 2.0**30, 16.0),
+                                                          ("f16", "f16", 2.0**13, 4e3), ("f16", "i8", 2.0**13, 4e3), ("bf16", "bf16", 2.0**12, 16.0)])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("max_new", [1, 300])
+def test_scores_past_what_f32_tells_apart(dtype, cache_dtype, grow, scale, dim, max_new):
+    """Scores of 2^18 to 2^46 in every third row.  A score's f32 error is at most 128 2^-24 of its products' sizes, which
+    come to some 11 times the largest score's: 2^-13 of it.  Rows whose largest score is further than twice that and
+    50 above the next have that key's value; in rows with scores under 300 the usual bound holds; all are finite."""
+    q, cache, table, lens, starts = _case([(300, 900), (3, 333), (260, 260)], 4, 2, dim, dtype, cache_dtype, seed=42, scale=scale)
+    q[::3] *= grow
+    out, lse = serving.paged_attention(q, cache, table, lens, starts, max_new=max_new, return_lse=True)
+    want, want_lse, size = _attend64(q, cache, table, lens, starts)
+    top, gap = _top_scores64(q, cache, table, lens, starts)
+    sure = (gap > 50 + 2.0**-12 * top.abs()) | (top.abs() < 300)
+    assert out.isfinite().all() and lse.isfinite().all() and sure[::3].any() and top.max() > 2.0**18
+    off = (out.double() - want).abs() - (U[q.dtype] * (want.abs() + size) + 2e-5 * size + 2.0**-25)
+    assert (off[sure] <= 0).all()
+    assert ((lse.double() - want_lse).abs() <= 2.0**-13 * want_lse.abs().clamp(min=1)).all()
