@@ -419,9 +419,9 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
         for (int j = 0; j < OT; ++j) {
           uint32_t b0, b1;
           if constexpr (Q8) {
-            // byte j % 4 of both keys' words, into both bytes of a half
+            // byte j % 4 of both keys' words: into both bytes of a half (i8), or the two of the low half
             const int n = j & 3;
-            const uint32_t sel = n | (n << 4) | ((n + 4) << 8) | ((n + 4) << 12);
+            const uint32_t sel = CD == TJ_I8 ? n | (n << 4) | ((n + 4) << 8) | ((n + 4) << 12) : n | ((n + 4) << 4);
             b0 = Codes<C, CD>::make(__byte_perm(va[j >> 2], vb[j >> 2], sel));
             b1 = Codes<C, CD>::make(__byte_perm(vc[j >> 2], vd[j >> 2], sel));
           } else {

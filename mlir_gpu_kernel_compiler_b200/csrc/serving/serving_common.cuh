@@ -67,8 +67,8 @@ inline const char* cache_fault(const tj_kv_cache& c) {
   return nullptr;
 }
 
-// Two codes, each in one byte of a 16-bit half of `w` (the low byte for i8, the high one for e4m3;
-// the other byte is anything), as two exact 16-bit floats.
+// Two codes as two exact 16-bit floats.  i8: each in the low byte of a 16-bit half of `w`, the other byte is anything;
+// e4m3: both in the low half of `w`, converted by the instruction for it, NaN among them.
 template <class T, int CD> struct Codes;
 // i8 -> bf16: 0x4300 | low 7 bits is 128 + them; less 128, or 256 where the sign bit is set
 template <> struct Codes<__nv_bfloat16, TJ_I8> {
@@ -87,19 +87,17 @@ template <> struct Codes<__half, TJ_I8> {
   }
   static TJ_DEV uint32_t make(uint32_t w) { return less((w & 0x00ff00ffu) ^ 0x64806480u); }
 };
-// e4m3 -> bf16: the code's exponent and mantissa in place, then 2^(127 - 7) for the bias
-template <> struct Codes<__nv_bfloat16, TJ_E4M3> {
+template <> struct Codes<__half, TJ_E4M3> {
   static TJ_DEV uint32_t make(uint32_t w) {
-    const uint32_t x = (w & 0x80008000u) | ((w & 0x7f007f00u) >> 4), k = 0x7b807b80u;
-    const __nv_bfloat162 d = __hmul2(reinterpret_cast<const __nv_bfloat162&>(x), reinterpret_cast<const __nv_bfloat162&>(k));
+    const __half2_raw d = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w), __NV_E4M3);
     return reinterpret_cast<const uint32_t&>(d);
   }
 };
-template <> struct Codes<__half, TJ_E4M3> {  // 2^(15 - 7)
+template <> struct Codes<__nv_bfloat16, TJ_E4M3> {
   static TJ_DEV uint32_t make(uint32_t w) {
-    const uint32_t x = (w & 0x80008000u) | ((w & 0x7f007f00u) >> 1), k = 0x5c005c00u;
-    const __half2 d = __hmul2(reinterpret_cast<const __half2&>(x), reinterpret_cast<const __half2&>(k));
-    return reinterpret_cast<const uint32_t&>(d);
+    const uint32_t h = Codes<__half, TJ_E4M3>::make(w);
+    const float2 f = __half22float2(reinterpret_cast<const __half2&>(h));
+    return tj_pack_bf16x2(f.x, f.y);
   }
 };
 
@@ -110,8 +108,8 @@ template <class T, int CD> TJ_DEV void codes4(uint32_t w, uint32_t& lo, uint32_t
     lo = Codes<T, CD>::less(__byte_perm(w, 0x64646464u, 0x4140));
     hi = Codes<T, CD>::less(__byte_perm(w, 0x64646464u, 0x4342));
   } else {
-    lo = Codes<T, CD>::make(__byte_perm(w, 0, CD == TJ_I8 ? 0x4140 : 0x1404));
-    hi = Codes<T, CD>::make(__byte_perm(w, 0, CD == TJ_I8 ? 0x4342 : 0x3424));
+    lo = Codes<T, CD>::make(CD == TJ_I8 ? __byte_perm(w, 0, 0x4140) : w);
+    hi = Codes<T, CD>::make(CD == TJ_I8 ? __byte_perm(w, 0, 0x4342) : w >> 16);
   }
 }
 

@@ -672,3 +672,35 @@ def test_scores_past_what_f32_tells_apart(dtype, cache_dtype, grow, scale, dim, 
     off = (out.double() - want).abs() - (U[q.dtype] * (want.abs() + size) + 2e-5 * size + 2.0**-25)
     assert (off[sure] <= 0).all()
     assert ((lse.double() - want_lse).abs() <= 2.0**-13 * want_lse.abs().clamp(min=1)).all()
+
+
+def test_every_code_reads_as_its_value():
+    """All 256 codes of a borrowed 8-bit cache, e4m3's two NaN among them."""
+    codes = torch.arange(256, device="cuda").to(torch.uint8).view(1, 2, 1, 128)
+    for dtype in ("i8", "e4m3"):
+        k = codes.view(DT[dtype])
+        scale = torch.tensor([0.5, 3.0], device="cuda").view(1, 2, 1)
+        cache = serving.PagedCache(k, k.clone(), scale, scale)
+        want = k.float().view(2, 1, 128) * scale.view(2, 1, 1)
+        for kind in ("f32", "f16", "bf16"):
+            for got in serving.cache_read(cache, torch.arange(2, device="cuda"), kind):
+                assert torch.equal(got.isnan(), want.isnan())
+                assert torch.equal(got.nan_to_num(1e4), want.to(DT[kind]).nan_to_num(1e4))
+        assert want.isnan().sum() == (2 if dtype == "e4m3" else 0)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new", [1, 300])
+def test_nan_codes_reach_the_output(new, dim, dtype):
+    q, cache, table, lens, starts = _case([(new, 700), (new, 333)], 8, 2, dim, dtype, "e4m3", seed=41)
+    want = serving.paged_attention(q, cache, table, lens, starts, max_new=new)
+    page, slot = table[0, 2].item(), 5
+    for pool, code in ((cache.k, 0x7F), (cache.v, 0x7F), (cache.k, 0xFF), (cache.v, 0xFF)):
+        held = pool[page, slot, 1, 9].clone()
+        pool.view(torch.uint8)[page, slot, 1, 9] = code
+        out = serving.paged_attention(q, cache, table, lens, starts, max_new=new)
+        pool[page, slot, 1, 9] = held
+        hit = out[:new, 4:] if pool is cache.k else out[:new, 4:, 9]
+        assert hit.isnan().all()
+        assert torch.equal(out[new:], want[new:]) and torch.equal(out[:new, :4], want[:new, :4])
