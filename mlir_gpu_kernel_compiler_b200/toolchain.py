@@ -190,7 +190,8 @@ def build_runtime(force: bool = False, extra_flags: tuple = (), variant: str = "
         out = LIB_PATH if not variant else LIB_PATH.with_name(f"libtj_b200_{variant}.so")
         stamp = out.with_suffix(".hash")
         flags = ["-O2", "-std=c++17", *ARCH_FLAGS, "-lineinfo", "-Xcompiler", "-fPIC,-fvisibility=hidden,-Wall",
-                 "--expt-relaxed-constexpr", *extra_flags, f"-I{INCLUDE}", f"-I{KDIR}"]
+                 "--expt-relaxed-constexpr", *extra_flags]
+        includes = [f"-I{INCLUDE}", f"-I{KDIR}"]  # no part of the key: a built tree may be moved or copied
         units = []
         for src, headers in _runtime_sources():
             h = hashlib.sha256(" ".join(flags).encode() + nvcc_version().encode())
@@ -208,7 +209,7 @@ def build_runtime(force: bool = False, extra_flags: tuple = (), variant: str = "
             if obj.exists() and not force:
                 return
             tmp = obj.with_suffix(f".{os.getpid()}.tmp")
-            r = subprocess.run([nvcc(), "-c", *flags, str(src), "-o", str(tmp)], capture_output=True, text=True)
+            r = subprocess.run([nvcc(), "-c", *flags, *includes, str(src), "-o", str(tmp)], capture_output=True, text=True)
             if r.returncode != 0:
                 raise BuildError(f"runtime build failed ({src.name}):\n{r.stderr[-4000:]}")
             os.replace(tmp, obj)

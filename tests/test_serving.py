@@ -134,3 +134,20 @@ def test_c_entry_refuses_bad_index_arrays():
                       ((4096, 2, 2, 2, 1, 0), b"NULL"), ((4096, 1 << 40, 1 << 20, 2, 1, 4096), b"too many")]:
         assert lib.tj_b200_narrow_indices(*args, None) == rt.TJ_ERR_INVALID and why in lib.tj_b200_last_error(), why
     assert lib.tj_b200_narrow_indices(None, 0, 3, 3, 1, None, None) == rt.TJ_OK
+
+
+def test_a_built_tree_is_not_built_again_where_it_is_copied_to(tmp_path):
+    import shutil
+    import sys
+
+    from mlir_gpu_kernel_compiler_b200 import toolchain
+
+    toolchain.build_runtime(), toolchain.build_serving_module()
+    root = Path(__file__).resolve().parents[1]
+    shutil.copytree(root / "mlir_gpu_kernel_compiler_b200", tmp_path / "mlir_gpu_kernel_compiler_b200", ignore=shutil.ignore_patterns("obj", "*.o"))
+    shutil.copytree(root / "include", tmp_path / "include")
+    code = ("import subprocess\nfrom mlir_gpu_kernel_compiler_b200 import toolchain\nrun = subprocess.run\n"
+            "def no_compiler(cmd, **how):\n    assert '-c' not in cmd and '-shared' not in cmd, cmd\n    return run(cmd, **how)\n"
+            "subprocess.run = no_compiler\nprint(toolchain.build_runtime(), toolchain.build_serving_module())")
+    r = subprocess.run([sys.executable, "-c", code], cwd=tmp_path, capture_output=True, text=True)
+    assert r.returncode == 0 and str(tmp_path) in r.stdout, r.stderr[-2000:]
