@@ -3,6 +3,7 @@
 // arguments from the wrappers in serving.py, which say what they mean; the launches are the C entry
 // points of include/tj_b200.h, taken from the library that runtime.py loads.
 #include <ATen/ATen.h>
+#include <ATen/core/grad_mode.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -132,6 +133,14 @@ bool rows_fit(const at::Tensor& t) {
 // rows that the kernels can read 16 bytes at a time: the tensor itself, or a copy
 at::Tensor rows(const at::Tensor& t) { return t.numel() == 0 || rows_fit(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
 
+// Whether autograd would follow what is made of t.  The entries then return NotImplemented, for the wrappers to put the
+// call into the graph.
+bool followed(const at::Tensor& t) { return t.requires_grad() && at::GradMode::is_enabled(); }
+PyObject* to_the_graph(PyObject* out) {
+  if (out != Py_None) BAD("out: not with inputs that require gradients; call it under torch.no_grad()");
+  return Py_NewRef(Py_NotImplemented);
+}
+
 at::Tensor out_rows(PyObject* o, const char* name, const at::Tensor& like) {
   const at::Tensor& t = tensor(o, name, 3, {like.scalar_type()}, like.get_device());
   if (t.sizes() != like.sizes()) BAD("%s: expected shape %s, got %s", name, shape_text(like).c_str(), shape_text(t).c_str());
@@ -202,6 +211,7 @@ struct Turn {
 Turn turn(tj_rows& r, PyObject* positions, PyObject* table, PyObject* layout, int device) {
   Turn t;
   t.table = tensor(table, "table", 2, {at::kFloat}, device);
+  if (followed(t.table)) BAD("table: no gradient is computed for it");
   const char* how = PyUnicode_Check(layout) ? PyUnicode_AsUTF8(layout) : "";
   r.interleaved = strcmp(how, "interleaved") == 0;
   if (!r.interleaved && strcmp(how, "half")) BAD("layout must be 'half' or 'interleaved', not '%s'", how);
@@ -244,6 +254,7 @@ PyObject* rotary(PyObject* const* a) {
     if (k.size(0) != r.tokens || k.size(2) != r.dim) BAD("k: shape %s does not go with q's %s", shape_text(k).c_str(), shape_text(q).c_str());
     r.kv_heads = k.size(1);
   }
+  if (followed(q) || (keys && followed(k))) return to_the_graph(a[6]);
   if (a[6] == Py_None) {
     q2 = at::empty(q.sizes(), q.options());
     if (keys) k2 = at::empty(k.sizes(), k.options());
@@ -301,6 +312,7 @@ PyObject* write(PyObject* const* a) {
     if (a[1] != Py_None) {
       const at::Tensor& q = tensor(a[1], "q", 3, {k.scalar_type()}, dev);
       if (q.size(0) != r.tokens || q.size(2) != r.dim) BAD("q: shape %s does not go with k's %s", shape_text(q).c_str(), shape_text(k).c_str());
+      if (followed(q)) return to_the_graph(a[8]);
       q2 = a[8] == Py_None ? at::empty(q.sizes(), q.options()) : out_rows(a[8], "out", q);
       qr = rows(q);
       if (q.numel()) {
@@ -423,6 +435,7 @@ PyObject* attention(PyObject* const* a) {
   if (PyErr_Occurred()) return nullptr;
   if (p.max_new < 1 || p.window < 0) BAD("max_new must be positive and window not negative");
   if (!(p.scale > 0.0) || !std::isfinite(p.scale)) BAD("scale must be positive");
+  if (followed(q)) return to_the_graph(a[10]);
   const at::Tensor out = a[10] == Py_None ? at::empty(q.sizes(), q.options()) : out_rows(a[10], "out", q);
   at::Tensor lse;
   if (PyObject_IsTrue(a[9])) {

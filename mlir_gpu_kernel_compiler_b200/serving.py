@@ -17,6 +17,10 @@ tensors' device and return without waiting.  As in ``B200Program``, a wrong type
 which skips it and records it: ``check()`` raises for it.  Indices are int32; int64 ones are narrowed by a launch
 of their own.
 
+Gradients: ``rotary`` has one, its inverse, and so has the turned ``q`` of ``rotary_cache_write``.  Attention has none:
+its result raises in the backward pass.  A cache keeps values, not what they came from, so nothing flows back
+through it.
+
 Each operator is a C entry point of ``include/tj_b200.h`` over hand-written sm_100a kernels in
 ``csrc/serving``.
 """
@@ -131,15 +135,43 @@ def _described(cache) -> bytes:
     return cache._native
 
 
+class _Rotary(torch.autograd.Function):
+    """Turning is linear, and turning back is its transpose (whatever the table's magnitude)."""
+
+    @staticmethod
+    def forward(ctx, q, k, positions, table, layout, inverse):
+        ctx.save_for_backward(positions, table)
+        ctx.how = layout, inverse, k is None
+        return _native.rotary(q, k, positions, table, layout, inverse, None)
+
+    @staticmethod
+    def backward(ctx, q_grad, k_grad):
+        layout, inverse, alone = ctx.how
+        q_grad, k_grad = rotary(q_grad, None if alone else k_grad, *ctx.saved_tensors, layout=layout, inverse=not inverse)
+        return q_grad, k_grad, None, None, None, None
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, *args):
+        return _native.attention(args[0], q, *args[1:])
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise NotImplementedError("paged_attention has no gradient: call it under torch.no_grad()")
+
+
 def rotary(q, k, positions, table, *, layout: str = "half", inverse: bool = False, out=None):
     """Rotary positions on ``q`` and ``k`` (``k`` may be None): ``(q', k')``.
 
     ``[tokens, heads, head_dim]`` in f32, f16 or bf16, head_dim a multiple of 8 up to 512; the first
     ``table.shape[1]`` elements of a row are turned, the rest passed on.  ``layout``: pairs
-    ``(i, i + rot / 2)`` ("half") or ``(2 i, 2 i + 1)`` ("interleaved").  ``inverse`` turns back, which is
-    also the gradient's pass.  ``out``: ``(q', k')`` to write, which may be q and k themselves.
+    ``(i, i + rot / 2)`` ("half") or ``(2 i, 2 i + 1)`` ("interleaved").  ``inverse`` turns by the opposite angles, which
+    undoes the turn (times the square of a table's magnitude) and is also the gradient's pass; autograd follows
+    the call.  ``out``: ``(q', k')`` to write, which may be q and k themselves (not under autograd).
     """
-    return _native.rotary(q, k, positions, table, layout, inverse, out)
+    got = _native.rotary(q, k, positions, table, layout, inverse, out)
+    return _Rotary.apply(q, k, positions, table, layout, inverse) if got is NotImplemented else got
 
 
 def cache_write(cache: PagedCache, k, v, slots) -> None:
@@ -159,7 +191,11 @@ def rotary_cache_write(cache: PagedCache, q, k, v, slots, positions, table, *, l
     """
     if table is None or positions is None:
         raise TypeError("rotary_cache_write needs positions and a table")
-    return _native.write(_described(cache), q, k, v, slots, positions, table, layout, out)
+    got = _native.write(_described(cache), q, k, v, slots, positions, table, layout, out)
+    if got is NotImplemented:  # q's turn goes into autograd's graph
+        _native.write(_described(cache), None, k, v, slots, positions, table, layout, None)
+        got = rotary(q, None, positions, table, layout=layout)[0]
+    return got
 
 
 def cache_read(cache: PagedCache, slots, dtype: str = "bf16") -> tuple[torch.Tensor, torch.Tensor]:
@@ -188,8 +224,9 @@ def paged_attention(q, cache: PagedCache, page_table, kv_lens, q_starts=None, *,
     sequence sees may hold anything; visible ones must be finite, as a NaN or an infinity reaches the
     sequence's other rows too.
     """
-    return _native.attention(_described(cache), q, page_table, kv_lens, q_starts, max_new, scale, causal, window,
-                             return_lse, out)
+    how = page_table, kv_lens, q_starts, max_new, scale, causal, window, return_lse, out
+    got = _native.attention(_described(cache), q, *how)
+    return _Attention.apply(q, _described(cache), *how) if got is NotImplemented else got
 
 
 _OPERATORS = ("rotary", "cache_write", "cache_read", "paged_attention")

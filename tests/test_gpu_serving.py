@@ -704,3 +704,60 @@ def test_nan_codes_reach_the_output(new, dim, dtype):
         hit = out[:new, 4:] if pool is cache.k else out[:new, 4:, 9]
         assert hit.isnan().all()
         assert torch.equal(out[new:], want[new:]) and torch.equal(out[:new, :4], want[:new, :4])
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_autograd_follows_rotary(layout, dtype):
+    """d/dx <w, rotary(x)> through torch's graph, of q and of k, against 64-bit autograd; a table's magnitude, a second
+    derivative (the map is linear: the gradient with respect to w turns back), an expanded gradient."""
+    table = serving.rotary_table(24, 64, magnitude=1.25)
+    pos = torch.tensor([0, 5, 63], device="cuda")
+    x = [_randn(3, h, 32, dtype=DT[dtype], seed=4 + h).requires_grad_() for h in (4, 2)]
+    w = [_randn(3, h, 32, dtype=DT[dtype], seed=14 + h).requires_grad_() for h in (4, 2)]
+    got = serving.rotary(*x, pos, table, layout=layout)
+    with torch.no_grad():
+        plain = serving.rotary(*x, pos, table, layout=layout)
+    assert all(torch.equal(a, b) and a.requires_grad and not b.requires_grad for a, b in zip(got, plain))
+    grads = torch.autograd.grad(got, x, w, create_graph=True)
+    u = 2.0**-22 if dtype == "f32" else U[DT[dtype]]
+    for a, g, s in zip(x, grads, w):
+        a64 = a.detach().double().requires_grad_()
+        (_turn64(a64, pos, table, layout) * s.detach().double()).sum().backward()
+        assert g.dtype == a.dtype and ((g.double() - a64.grad).abs() <= _rot_tol(a64.grad, u) * 1.6).all()
+    again = torch.autograd.grad(grads, w, [a.detach() for a in x])
+    assert all(torch.equal(a, b) for a, b in zip(again, plain))
+    alone = serving.rotary(x[0], None, pos, table, layout=layout)
+    assert alone[1] is None
+    alone[0].sum().backward()
+    ones = serving.rotary(torch.ones_like(x[0]).detach(), None, pos, table, layout=layout, inverse=True)[0]
+    assert torch.equal(x[0].grad, ones) and x[1].grad is None
+    cache = serving.PagedCache.empty(2, 4, 2, 32, "bf16")
+    x[0].grad = None
+    turned = serving.rotary_cache_write(cache, x[0], x[1], x[1], torch.arange(3, device="cuda"), pos, table, layout=layout)
+    assert torch.equal(turned, plain[0])
+    turned.sum().backward()
+    assert torch.equal(x[0].grad, ones) and torch.equal(cache.v[0, :3], x[1].to(torch.bfloat16))
+
+
+def test_what_has_no_gradient_says_so():
+    """A result that would lose its gradient without a word is refused, at the latest in the backward pass."""
+    q, cache, table, lens, starts = _case([(1, 100), (1, 40)], 4, 2, 64, seed=43)
+    want = serving.paged_attention(q, cache, table, lens, return_lse=True)
+    q.requires_grad_()
+    got = serving.paged_attention(q, cache, table, lens, return_lse=True)
+    assert all(torch.equal(a, b) and a.requires_grad for a, b in zip(got, want))
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        got[0].sum().backward()
+    with pytest.raises(NotImplementedError, match="no gradient"):
+        serving.paged_attention(q, cache, table, lens).sum().backward()
+    turns, pos = serving.rotary_table(64, 8), torch.zeros(2, dtype=torch.int32, device="cuda")
+    for call in (lambda: serving.paged_attention(q, cache, table, lens, out=torch.empty_like(q)),
+                 lambda: serving.rotary(q, None, pos, turns, out=(torch.empty_like(q), None)),
+                 lambda: serving.rotary_cache_write(cache, q, q[:, :2], q[:, :2], pos - 1, pos, turns, out=torch.empty_like(q))):
+        with pytest.raises(ValueError, match="require gradients"):
+            call()
+        with torch.no_grad():
+            call()
+    with pytest.raises(ValueError, match="table: no gradient"):
+        serving.rotary(q, None, pos, turns.clone().requires_grad_())
