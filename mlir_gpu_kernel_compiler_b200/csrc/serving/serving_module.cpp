@@ -152,14 +152,20 @@ void head_dim(int64_t dim) {
   if (dim % 8 || dim <= 0 || dim > 512) BAD("head dim %lld is not a multiple of 8 from 8 to 512", static_cast<long long>(dim));
 }
 
-// What PagedCache keeps of its tensors.
+// What PagedCache keeps of its tensors, which it holds and which cannot be replaced.
 struct CacheInfo {
   tj_kv_cache c;
   int64_t device;
+  c10::TensorImpl* tensors[4];  // k, v, their scales or NULL
 };
 const CacheInfo& cache_info(PyObject* o) {
   if (!PyBytes_Check(o) || PyBytes_GET_SIZE(o) != sizeof(CacheInfo)) fail(PyExc_TypeError, "cache: not a PagedCache's description");
-  return *reinterpret_cast<const CacheInfo*>(PyBytes_AS_STRING(o));
+  const CacheInfo& i = *reinterpret_cast<const CacheInfo*>(PyBytes_AS_STRING(o));
+  // a tensor may have been given other memory since (t.data = ..., module.to()), and the old may be someone else's
+  const void* held[4] = {i.c.k, i.c.v, i.c.k_scale, i.c.v_scale};
+  for (int n = 0; n < 4; ++n)
+    if (i.tensors[n] && i.tensors[n]->data() != held[n]) BAD("cache: its tensors have other memory than when the PagedCache was made");
+  return i;
 }
 
 PyObject* describe(PyObject* const* a) {
@@ -201,6 +207,7 @@ PyObject* describe(PyObject* const* a) {
   i.c.head_stride = k.stride(2);
   i.c.dtype = code_of(k.scalar_type());
   i.device = dev;
+  for (int n = 0; n < 4; ++n) i.tensors[n] = a[n] == Py_None ? nullptr : THPVariable_Unpack(a[n]).unsafeGetTensorImpl();
   return PyBytes_FromStringAndSize(reinterpret_cast<const char*>(&i), sizeof(i));
 }
 

@@ -54,7 +54,7 @@ _native = _load()
 
 
 class PagedCache:
-    """A pool of pages of keys and values; borrows its tensors.
+    """A pool of pages of keys and values; borrows its tensors, which cannot be replaced.
 
     ``k`` and ``v``: ``[pages, page_size, kv_heads, head_dim]``, f16 or bf16, or i8 or e4m3 codes with
     scales ``[pages, page_size, kv_heads]`` in f32 (value = code * scale).  Both may be views whose
@@ -63,12 +63,16 @@ class PagedCache:
     Slot ``s`` is place ``s % page_size`` of page ``s // page_size``.
     """
 
-    __slots__ = ("k", "v", "k_scale", "v_scale", "_native")
+    __slots__ = ("_tensors", "_native")
 
     def __init__(self, k, v, k_scale=None, v_scale=None):
         self._native = _native.describe(k, v, k_scale, v_scale)
-        self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
+        self._tensors = k, v, k_scale, v_scale
 
+    k = property(lambda self: self._tensors[0])
+    v = property(lambda self: self._tensors[1])
+    k_scale = property(lambda self: self._tensors[2])
+    v_scale = property(lambda self: self._tensors[3])
     device = property(lambda self: self.k.device)
     dtype = property(lambda self: self.k.dtype)
     pages = property(lambda self: self.k.shape[0])

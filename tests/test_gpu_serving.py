@@ -761,3 +761,20 @@ def test_what_has_no_gradient_says_so():
             call()
     with pytest.raises(ValueError, match="table: no gradient"):
         serving.rotary(q, None, pos, turns.clone().requires_grad_())
+
+
+@pytest.mark.parametrize("name", ["k", "v", "k_scale", "v_scale"])
+def test_a_cache_whose_memory_was_exchanged_is_refused(name):
+    cache = serving.PagedCache.empty(4, 16, 2, 64, "i8")
+    rows, slots = _randn(2, 2, 64), torch.arange(2, device="cuda")
+    serving.cache_write(cache, rows, rows, slots)
+    held = getattr(cache, name)
+    kept = held.data
+    held.data = held.clone()
+    q, page, lens = _randn(1, 2, 64, dtype=torch.bfloat16), torch.zeros(1, 1, dtype=torch.int32, device="cuda"), torch.ones(1, dtype=torch.int32, device="cuda")
+    for call in (lambda: serving.cache_write(cache, rows, rows, slots), lambda: serving.cache_read(cache, slots),
+                 lambda: serving.paged_attention(q, cache, page, lens)):
+        with pytest.raises(ValueError, match="other memory"):
+            call()
+    held.data = kept
+    serving.cache_write(cache, rows, rows, slots)

@@ -151,3 +151,11 @@ def test_a_built_tree_is_not_built_again_where_it_is_copied_to(tmp_path):
             "subprocess.run = no_compiler\nprint(toolchain.build_runtime(), toolchain.build_serving_module())")
     r = subprocess.run([sys.executable, "-c", code], cwd=tmp_path, capture_output=True, text=True)
     assert r.returncode == 0 and str(tmp_path) in r.stdout, r.stderr[-2000:]
+
+
+@pytest.mark.parametrize("name", ["k", "v", "k_scale", "v_scale"])
+def test_a_caches_tensors_cannot_be_replaced(name):
+    """The operators go by the memory that the cache was made with."""
+    cache = object.__new__(serving.PagedCache)
+    with pytest.raises(AttributeError):
+        setattr(cache, name, torch.zeros(1))
