@@ -141,10 +141,17 @@ PyObject* to_the_graph(PyObject* out) {
   return Py_NewRef(Py_NotImplemented);
 }
 
+// Torch counts a tensor's changes, by which autograd knows that a value it has kept is no longer there.
+void changed(c10::TensorImpl* t) {
+  if (t && !t->is_inference()) t->bump_version();
+}
+
 at::Tensor out_rows(PyObject* o, const char* name, const at::Tensor& like) {
   const at::Tensor& t = tensor(o, name, 3, {like.scalar_type()}, like.get_device());
   if (t.sizes() != like.sizes()) BAD("%s: expected shape %s, got %s", name, shape_text(like).c_str(), shape_text(t).c_str());
   if (t.numel() && !rows_fit(t)) BAD("%s: rows must be contiguous and start on 16-byte boundaries", name);
+  if (followed(t)) BAD("%s: requires gradients; call it under torch.no_grad()", name);
+  changed(t.unsafeGetTensorImpl());
   return t;
 }
 
@@ -334,6 +341,10 @@ PyObject* write(PyObject* const* a) {
     }
   }
   if (r.tokens) {
+    for (c10::TensorImpl* t : cache.tensors) {
+      if (t && t->requires_grad() && at::GradMode::is_enabled()) BAD("cache: requires gradients; write it under torch.no_grad()");
+      changed(t);
+    }
     const at::Tensor kr = rows(k), vr = rows(v);
     r.k = kr.data_ptr();
     r.v = vr.data_ptr();

@@ -778,3 +778,31 @@ def test_a_cache_whose_memory_was_exchanged_is_refused(name):
             call()
     held.data = kept
     serving.cache_write(cache, rows, rows, slots)
+
+
+def test_changes_in_place_are_counted():
+    """What autograd has kept for a backward pass and an operator then changes is noticed there."""
+    q, cache, table, lens, starts = _case([(1, 100), (1, 40)], 4, 2, 64, "bf16", "i8", seed=44)
+    half = serving.PagedCache.empty(4, 16, 2, 64, "bf16")
+    turns, pos, slots = serving.rotary_table(64, 8), torch.zeros(2, dtype=torch.int32, device="cuda"), torch.arange(2, device="cuda")
+    rows, out, out2 = _randn(2, 2, 64, dtype=torch.bfloat16), torch.zeros_like(q), torch.zeros_like(q)
+    for kept, call in ((half.k, lambda: serving.cache_write(half, rows, rows, slots)), (half.v, lambda: serving.cache_write(half, rows, rows, slots)),
+                       (cache.k_scale, lambda: serving.cache_write(cache, rows, rows, slots)), (cache.v_scale, lambda: serving.cache_write(cache, rows, rows, slots)),
+                       (half.k, lambda: serving.rotary_cache_write(half, None, rows, rows, slots, pos, turns)),
+                       (out, lambda: serving.paged_attention(q, cache, table, lens, out=out)), (out, lambda: serving.rotary(q, None, pos, turns, out=(out, None))),
+                       (out2, lambda: serving.rotary_cache_write(cache, q, rows, rows, slots, pos, turns, out=out2))):
+        before = kept._version
+        y = (torch.ones_like(kept, requires_grad=True) * kept).sum()
+        call()
+        assert kept._version == before + 1
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.backward()
+    leaf = serving.PagedCache(half.k.clone().requires_grad_(), half.v.clone())
+    with pytest.raises(ValueError, match="requires gradients"):
+        serving.cache_write(leaf, rows, rows, slots)
+    with torch.no_grad():
+        serving.cache_write(leaf, rows, rows, slots)
+    with torch.inference_mode():
+        made = serving.PagedCache.empty(4, 16, 2, 64, "bf16")
+    serving.cache_write(made, rows, rows, slots)
+    assert torch.equal(made.k[0, :2], rows) and torch.equal(leaf.v[0, :2], rows)
