@@ -806,3 +806,12 @@ def test_changes_in_place_are_counted():
         made = serving.PagedCache.empty(4, 16, 2, 64, "bf16")
     serving.cache_write(made, rows, rows, slots)
     assert torch.equal(made.k[0, :2], rows) and torch.equal(leaf.v[0, :2], rows)
+
+
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+def test_more_heads_than_16_bits_count(layout):
+    """140000 heads of one token: as the same rows of 140 tokens."""
+    table, x = serving.rotary_table(264, 16), _randn(1, 140000, 264, dtype=torch.bfloat16)
+    got, _ = serving.rotary(x, None, torch.tensor([7], device="cuda"), table, layout=layout)
+    want, _ = serving.rotary(x.view(140, 1000, 264), None, torch.full((140,), 7, device="cuda"), table, layout=layout)
+    assert torch.equal(got.view(-1), want.view(-1))
