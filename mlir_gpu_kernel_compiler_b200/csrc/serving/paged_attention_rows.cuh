@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
   auto page_of = [&](int base) {
     const int key = base + lane;
     if (lane >= KS || key >= k1) return INT_MIN;
-    return table[p.page_shift >= 0 ? key >> p.page_shift : key / page_size];
+    return max(-1, table[p.page_shift >= 0 ? key >> p.page_shift : key / page_size]);  // INT_MIN is no key's page
   };
   // Where a lane copies to, and reads from, in a block: its first row's piece; further rows are at constant
   // distances, but for bits that the permutation turns by the row's number, which are constants too.

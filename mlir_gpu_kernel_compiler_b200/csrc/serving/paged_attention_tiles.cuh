@@ -493,7 +493,7 @@ TJ_DEV void produce(const AttnParams& p, const TilesShared<T, CD, D>& sh, int se
   auto page_of = [&](int j) {
     const int key = key0 + j * TILE_KEYS + lane;
     if (j >= nb || key < lo || key >= hi) return INT_MIN;
-    return table[p.page_shift >= 0 ? key >> p.page_shift : key / page_size];
+    return max(-1, table[p.page_shift >= 0 ? key >> p.page_shift : key / page_size]);  // INT_MIN is no key's page
   };
   long off, soff;
   auto place = [&](int j, int page) {

@@ -815,3 +815,17 @@ def test_more_heads_than_16_bits_count(layout):
     got, _ = serving.rotary(x, None, torch.tensor([7], device="cuda"), table, layout=layout)
     want, _ = serving.rotary(x.view(140, 1000, 264), None, torch.full((140,), 7, device="cuda"), table, layout=layout)
     assert torch.equal(got.view(-1), want.view(-1))
+
+
+@pytest.mark.parametrize("new,max_new", [(1, 1), (300, 300)])
+@pytest.mark.parametrize("cache_dtype", ["bf16", "i8"])
+@pytest.mark.parametrize("page", [-1, -(2**31), 2**31 - 1])
+def test_every_page_out_of_range_is_recorded(page, cache_dtype, new, max_new):
+    q, cache, table, lens, starts = _case([(new, 900), (new, 500)], 8, 2, 64, "bf16", cache_dtype, seed=45)
+    want = serving.paged_attention(q, cache, table, lens, starts, max_new=max_new)
+    serving.check()
+    table[1, 3] = page
+    got = serving.paged_attention(q, cache, table, lens, starts, max_new=max_new)
+    with pytest.raises(rt.RuntimeError_, match="paged_attention: page"):
+        serving.check()
+    assert torch.equal(got[:new], want[:new]) and got.isfinite().all()
