@@ -115,7 +115,8 @@ TJ_DEV Piece find_piece(const AttnParams& p, int unit, int per_tile, int step) {
   for (int o = 16; o > 0; o >>= 1) work += __shfl_xor_sync(0xffffffffu, work, o);
   // (in f32, rounded up generously: pieces may only become fewer; 64-bit divisions take hundreds of clocks)
   const long want = static_cast<long>(static_cast<float>(work * p.a.cache.heads) / static_cast<float>(p.target) * 1.000001f) + 1;
-  g.chunk = static_cast<int>((max(want, static_cast<long>(p.min_chunk)) + step - 1) / step * step);
+  // (a chunk of 2^30 keys is any sequence's whole: with max_new far too small `want` may pass 32 bits)
+  g.chunk = static_cast<int>((min(max(want, static_cast<long>(p.min_chunk)), 1L << 30) + step - 1) / step * step);
   auto cuts_of = [&](const Seq& s) {
     const int n = span(s) + g.chunk - 1, q = static_cast<int>(__fdividef(static_cast<float>(n), static_cast<float>(g.chunk)));
     return max(1, q + (n - q * g.chunk >= g.chunk) - (n - q * g.chunk < 0));  // the estimate is off by one at the most
