@@ -151,13 +151,22 @@ class PagedDecoder:
         """New tokens of some sequences, ``{sequence: tokens}``: the logits after each one's last, f32 [len(new), vocab]."""
         c, size = self.config, self.config.page_size
         tokens, slots, positions, starts = [], [], [], [0]
+        need = 0   # everything that can be refused is, before a page or a length changes
+        for s, ts in new.items():
+            if not ts:
+                raise ValueError(f"sequence {s}: no new token")
+            have = self.lengths.get(s, 0) + len(ts)
+            if have > c.positions:
+                raise ValueError(f"sequence {s}: more than {c.positions} positions")
+            need += -(-have // size) - len(self.pages.get(s, ()))
+        n = sum(len(ts) for ts in new.values())
+        if not 0 < n <= c.rows:
+            raise ValueError(f"{n} new tokens, at least 1 and at most {c.rows}")
+        if need > len(self.free):
+            raise RuntimeError("no free page")
         for s, ts in new.items():
             have, pages = self.lengths.get(s, 0), self.pages.setdefault(s, [])
-            if have + len(ts) > c.positions:
-                raise ValueError(f"sequence {s}: more than {c.positions} positions")
             while len(pages) * size < have + len(ts):
-                if not self.free:
-                    raise RuntimeError("no free page")
                 pages.append(self.free.pop())
             at = range(have, have + len(ts))
             tokens += ts
@@ -165,9 +174,6 @@ class PagedDecoder:
             slots += [pages[i // size] * size + i % size for i in at]
             starts.append(len(tokens))
             self.lengths[s] = have + len(ts)
-        n = len(tokens)
-        if n > c.rows:
-            raise ValueError(f"{n} new tokens, at most {c.rows}")
         pad = c.rows - n   # rows of no sequence: their slot is -1, attention does not reach them
         width = max(len(self.pages[s]) for s in new)
 

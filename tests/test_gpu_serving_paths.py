@@ -116,3 +116,20 @@ def test_a_wait_of_the_attention_kernel_that_runs_out_is_reported():
     lines = [x for x in r.stdout.splitlines() if x.startswith("RESULT")]
     assert len(lines) == 2 and all("paged_attention: wait timeout" in x for x in lines), r.stdout
     assert "AFTER True" in r.stdout
+
+
+@pytest.mark.gpu
+def test_a_refused_step_changes_nothing():
+    model = PagedDecoder(Config(pages=6, positions=90))
+    tokens = list(range(60))
+    model.step({0: tokens[:20]})
+    state = list(model.free), {s: list(p) for s, p in model.pages.items()}, dict(model.lengths)
+    for new, why, what in (({1: [1] * 65}, ValueError, "at most 64"), ({0: [1] * 50, 1: [2] * 20}, ValueError, "at most 64"), ({0: [1] * 71}, ValueError, "positions"),
+                           ({1: [1] * 60, 0: [2] * 4, 2: []}, ValueError, "no new token"), ({}, ValueError, "at least 1"), ({1: [1] * 33, 2: [2] * 17}, RuntimeError, "no free page")):
+        with pytest.raises(why, match=what):
+            model.step(new)
+        assert state == (list(model.free), model.pages, model.lengths)
+    got = model.step({0: tokens[20:60]})[0]
+    want = model.dense_logits(tokens)[-1]
+    assert (got - want).norm() <= 2e-2 * want.norm()
+    serving.check()
