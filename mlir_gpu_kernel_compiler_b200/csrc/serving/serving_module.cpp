@@ -50,6 +50,19 @@ void fail(PyObject* type, const char* fmt, ...) {
 }
 #define BAD(...) fail(PyExc_ValueError, __VA_ARGS__)
 
+// Arguments whose conversion Python refuses (its exception is set already: `type` is NULL, `code` 0)
+bool truth(PyObject* o) {
+  const int t = PyObject_IsTrue(o);
+  if (t < 0) throw Fault{nullptr, "", 0};
+  return t;
+}
+const char* text(PyObject* o) {
+  if (!PyUnicode_Check(o)) return "";
+  const char* s = PyUnicode_AsUTF8(o);
+  if (!s) throw Fault{nullptr, "", 0};
+  return s;
+}
+
 void launched(int rc) {
   if (rc != TJ_OK) throw Fault{nullptr, api.last_error(), rc};
 }
@@ -226,7 +239,7 @@ Turn turn(tj_rows& r, PyObject* positions, PyObject* table, PyObject* layout, in
   Turn t;
   t.table = tensor(table, "table", 2, {at::kFloat}, device);
   if (followed(t.table)) BAD("table: no gradient is computed for it");
-  const char* how = PyUnicode_Check(layout) ? PyUnicode_AsUTF8(layout) : "";
+  const char* how = text(layout);
   r.interleaved = strcmp(how, "interleaved") == 0;
   if (!r.interleaved && strcmp(how, "half")) BAD("layout must be 'half' or 'interleaved', not '%s'", how);
   r.rot = t.table.size(1);
@@ -260,7 +273,7 @@ PyObject* rotary(PyObject* const* a) {
   head_dim(r.dim);
   r.dtype = code_of(q.scalar_type());
   const Turn held = turn(r, a[2], a[3], a[4], dev);
-  r.inverse = PyObject_IsTrue(a[5]);
+  r.inverse = truth(a[5]);
   const bool keys = a[1] != Py_None;
   at::Tensor k, q2, k2;
   if (keys) {
@@ -363,7 +376,7 @@ PyObject* write(PyObject* const* a) {
 PyObject* read(PyObject* const* a) {
   const CacheInfo& cache = cache_info(a[0]);
   const int dev = static_cast<int>(cache.device);
-  const char* how = PyUnicode_Check(a[2]) ? PyUnicode_AsUTF8(a[2]) : "";
+  const char* how = text(a[2]);
   at::ScalarType kind;
   if (!strcmp(how, "bf16"))
     kind = at::kBFloat16;
@@ -449,14 +462,14 @@ PyObject* attention(PyObject* const* a) {
   p.max_new = a[5] != Py_None ? PyLong_AsLongLong(a[5]) : p.q_starts ? INT64_MAX : 1;
   p.window = PyLong_AsLongLong(a[8]);
   p.scale = a[6] != Py_None ? PyFloat_AsDouble(a[6]) : 1.0 / std::sqrt(static_cast<double>(dim));
-  p.causal = PyObject_IsTrue(a[7]);
+  p.causal = truth(a[7]);
   if (PyErr_Occurred()) return nullptr;
   if (p.max_new < 1 || p.window < 0) BAD("max_new must be positive and window not negative");
   if (!(p.scale > 0.0) || !std::isfinite(p.scale)) BAD("scale must be positive");
   if (followed(q)) return to_the_graph(a[10]);
   const at::Tensor out = a[10] == Py_None ? at::empty(q.sizes(), q.options()) : out_rows(a[10], "out", q);
   at::Tensor lse;
-  if (PyObject_IsTrue(a[9])) {
+  if (truth(a[9])) {
     lse = at::empty({p.tokens, p.q_heads}, q.options().dtype(at::kFloat));
     p.lse = lse.data_ptr<float>();
   }
@@ -514,7 +527,7 @@ template <PyObject* (*F)(PyObject* const*), int N> PyObject* entry(PyObject*, Py
   } catch (const Fault& f) {
     if (f.type) {
       PyErr_SetString(f.type, f.what.c_str());
-    } else {
+    } else if (f.code != 0) {
       PyObject* e = PyObject_CallFunction(runtime_error, "is", f.code, f.what.c_str());
       if (e) {
         PyErr_SetObject(runtime_error, e);

@@ -829,3 +829,27 @@ def test_every_page_out_of_range_is_recorded(page, cache_dtype, new, max_new):
     with pytest.raises(rt.RuntimeError_, match="paged_attention: page"):
         serving.check()
     assert torch.equal(got[:new], want[:new]) and got.isfinite().all()
+
+
+def test_arguments_that_do_not_convert():
+    """Python's own errors come through (text that is no text in UTF-8 ended the process)."""
+    cache, x = serving.PagedCache.empty(4, 16, 2, 64), _randn(2, 2, 64, dtype=torch.bfloat16)
+    slots, table = torch.zeros(2, dtype=torch.int32, device="cuda"), serving.rotary_table(64, 8)
+
+    class Neither:
+        def __bool__(self):
+            raise ArithmeticError("neither")
+
+    for call in (lambda: serving.rotary(x, None, slots, table, inverse=Neither()), lambda: serving.paged_attention(x, cache, slots[:, None], slots, causal=Neither()),
+                 lambda: serving.paged_attention(x, cache, slots[:, None], slots, return_lse=Neither())):
+        with pytest.raises(ArithmeticError, match="neither"):
+            call()
+    for call in (lambda: serving.rotary(x, None, slots, table, layout="\ud800"), lambda: serving.cache_read(cache, slots, "\ud800")):
+        with pytest.raises(UnicodeEncodeError):
+            call()
+    for call in (lambda: serving.paged_attention(x, cache, slots[:, None], slots, max_new="x"), lambda: serving.paged_attention(x, cache, slots[:, None], slots, window=1.5),
+                 lambda: serving.paged_attention(x, cache, slots[:, None], slots, scale="x")):
+        with pytest.raises(TypeError):
+            call()
+    with pytest.raises(OverflowError):
+        serving.paged_attention(x, cache, slots[:, None], slots, window=2**63)
