@@ -35,8 +35,8 @@ struct RowsParams {
   int* status;
   int lanes_log2;  // lanes of a row
   int slots;       // slots of a row: ceil(dim / 16)
+  int iters;       // warp iterations over a token's rows; times the number of warps that share it below 2^32
   Div segs;        // warps that share a token
-  int each, more;  // each has so many iterations over the token's rows, the first `more` one more
   Div page;        // slots of a page
   int op;
 };
@@ -111,7 +111,8 @@ __global__ void __launch_bounds__(128, ROT == 3 ? 2 : 6) rows_kernel(const __gri
   auto source = [&](int r) { return r < nq ? q + r * a.q_head : r < nq + nk ? k + (r - nq) * a.k_head : v + (r - nq - nk) * a.v_head; };
   constexpr int BATCH = sizeof(T) == 4 ? 2 : 4;
   Unit<T> raw[BATCH][2];
-  const int i0 = seg * p.each + min(seg, p.more), i1 = i0 + p.each + (seg < p.more);
+  const int segs = static_cast<int>(p.segs.d);
+  const int i0 = static_cast<int>(static_cast<unsigned>(seg) * p.iters / segs), i1 = static_cast<int>(static_cast<unsigned>(seg + 1) * p.iters / segs);
   auto load = [&](int it) {
 #pragma unroll
     for (int j = 0; j < BATCH; ++j) {
@@ -461,14 +462,13 @@ int run_rows(const char* name, int op, const tj_rows* a, bool write, void* strea
   p.lanes_log2 = 0;
   while ((1 << p.lanes_log2) < p.slots) ++p.lanes_log2;
   if (rows > 0x40000000L) return refuse(TJ_ERR_INVALID, name, "too many rows");
-  const int per = 32 >> p.lanes_log2, iters = static_cast<int>((rows + per - 1) / per);
+  const int per = 32 >> p.lanes_log2;
+  p.iters = static_cast<int>((rows + per - 1) / per);
   // four groups a warp; with few tokens one each, so that the rows of a single-token step spread over the
   // multiprocessors
-  const bool few = a->tokens * iters < 16L * dev.sms;
-  const int segs = few ? iters : (iters + 3) / 4;
+  const bool few = a->tokens * p.iters < 16L * dev.sms;
+  const int segs = static_cast<int>(std::min<long>(few ? p.iters : (p.iters + 3) / 4, 0xffffffffL / p.iters));
   p.segs = Div(static_cast<uint32_t>(segs));
-  p.each = iters / segs;
-  p.more = iters % segs;
   p.page = Div(write ? static_cast<uint32_t>(a->cache.page_size) : 1u);
   const long warps = a->tokens * segs, grid = (warps + 3) / 4;
   if (warps > 0x7fffff00L) return refuse(TJ_ERR_INVALID, name, "too many rows");
