@@ -136,10 +136,10 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
   // Lane i looks key base + i of a block up: its page a block ahead, then the byte offset of its row and
   // its place among the scales (-1: not there).
   const int page_size = static_cast<int>(p.a.cache.page_size);
-  auto page_of = [&](int base) {
+  auto page_of = [&](int base) {  // (nothing may be done to the page here: the look-up would be waited for)
     const int key = base + lane;
-    if (lane >= KS || key >= k1) return INT_MIN;
-    return max(-1, table[p.page_shift >= 0 ? key >> p.page_shift : key / page_size]);  // INT_MIN is no key's page
+    if (lane >= KS || key >= k1) return 0;
+    return table[p.page_shift >= 0 ? key >> p.page_shift : key / page_size];
   };
   // Where a lane copies to, and reads from, in a block: its first row's piece; further rows are at constant
   // distances, but for bits that the permutation turns by the row's number, which are constants too.
@@ -152,13 +152,14 @@ __global__ void __launch_bounds__(Rows<T, CD, D, WIDE>::THREADS, Rows<T, CD, D, 
   auto fetch = [&](int stage, int base, int page) {
     const char* row = my_k;  // this lane looks it up for others, so the piece is added where it is used
     long soff = 0;
+    const bool here = lane < KS && base + lane < k1;
     bool on = false;
-    if (page >= 0 && page < p.a.cache.pages) {
+    if (here && page >= 0 && page < p.a.cache.pages) {
       const int key = base + lane, slot = p.page_shift >= 0 ? key & (page_size - 1) : key % page_size;
       row = kbase + (page * p.a.cache.page_stride + slot * p.a.cache.slot_stride) * ES;
       if (Q8) soff = page * p.a.cache.scale_page + slot * p.a.cache.scale_slot;
       on = true;
-    } else if (page != INT_MIN) {
+    } else if (here) {
       tj_report(p.status, TJ_STATUS_BOUNDS, OP_ATTENTION * 16 + SITE_PAGE);
     }
     const unsigned live = __ballot_sync(0xffffffffu, on);

@@ -490,20 +490,24 @@ TJ_DEV void produce(const AttnParams& p, const TilesShared<T, CD, D>& sh, int se
   // This lane's key of block j: its page (looked up a block before it is used), then the byte offset
   // of its row and its place among the scales (-1: not there).
   const int page_size = static_cast<int>(p.a.cache.page_size);
-  auto page_of = [&](int j) {
+  int next_page;
+  bool next_there;  // a look-up's key is one of the tile's (what is looked up is not touched before it is used)
+  auto look_up = [&](int j) {
     const int key = key0 + j * TILE_KEYS + lane;
-    if (j >= nb || key < lo || key >= hi) return INT_MIN;
-    return max(-1, table[p.page_shift >= 0 ? key >> p.page_shift : key / page_size]);  // INT_MIN is no key's page
+    next_there = j < nb && key >= lo && key < hi;
+    if (next_there) next_page = table[p.page_shift >= 0 ? key >> p.page_shift : key / page_size];
   };
   long off, soff;
-  auto place = [&](int j, int page) {
+  auto place = [&](int j) {  // what was looked up last, for block j
     off = soff = -1;
+    if (!next_there) return;
+    const int page = next_page;
     if (page >= 0 && page < p.a.cache.pages) {
       const int key = key0 + j * TILE_KEYS + lane;
       const int slot = p.page_shift >= 0 ? key & (page_size - 1) : key % page_size;
       off = (page * p.a.cache.page_stride + slot * p.a.cache.slot_stride) * ES;
       if (C::Q8) soff = page * p.a.cache.scale_page + slot * p.a.cache.scale_slot + head * p.a.cache.scale_head;
-    } else if (page != INT_MIN) {
+    } else {
       tj_report(p.status, TJ_STATUS_BOUNDS, OP_ATTENTION * 16 + SITE_PAGE);
     }
   };
@@ -518,8 +522,9 @@ TJ_DEV void produce(const AttnParams& p, const TilesShared<T, CD, D>& sh, int se
 #endif
     arrive(full + 8 * (it % STAGES));
   };
-  place(0, page_of(0));
-  int next_page = page_of(1);
+  look_up(0);
+  place(0);
+  look_up(1);
   if constexpr (!C::Q8) {
     constexpr int LPR = D / 8, PER = 32 / LPR;  // lanes of a row, rows of a warp's instruction
     const int piece = lane % LPR;
@@ -539,8 +544,8 @@ TJ_DEV void produce(const AttnParams& p, const TilesShared<T, CD, D>& sh, int se
         arrive(S::Q_FULL);
       else
         announce(it - 1);
-      place(j + 1, next_page);
-      next_page = page_of(j + 2);
+      place(j + 1);
+      look_up(j + 2);
     }
     cp_async_wait<0>();
     if (!*sh.abort_flag()) announce(blocks + nb - 1);
@@ -562,8 +567,8 @@ TJ_DEV void produce(const AttnParams& p, const TilesShared<T, CD, D>& sh, int se
         cp_async4(sh.at(scale0 + slot + TILE_KEYS * 4), p.a.cache.v_scale + (soff < 0 ? 0 : soff), soff >= 0);
       }
       cp_async_commit();
-      place(j + 1, next_page);
-      next_page = page_of(j + 2);
+      place(j + 1);
+      look_up(j + 2);
     };
     load(0);
     load(1);
