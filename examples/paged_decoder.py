@@ -39,6 +39,10 @@ class Config:
     cache: str = "bf16"
 
 
+# chunks of 512 tokens, which attention takes with its kernel of many rows
+LONG_CHUNKS = dict(width=512, q_heads=8, kv_heads=2, head_dim=128, hidden=1024, rows=512, pages=128)
+
+
 class _Plan:
     """A plan of row normalisations and GEMMs in tensorjit's JSON form."""
 

@@ -133,3 +133,33 @@ def test_a_refused_step_changes_nothing():
     want = model.dense_logits(tokens)[-1]
     assert (got - want).norm() <= 2e-2 * want.norm()
     serving.check()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("cache,tol", [("bf16", 2e-2), ("i8", 3e-2), ("e4m3", 1e-1)])
+def test_decoder_in_long_chunks_reaches_the_kernel_of_many_rows(cache, tol):
+    """The same bounds as for short chunks; which kernel a chunk gets is told by the workspace that it asks for."""
+    import ctypes
+    import struct
+
+    from paged_decoder import LONG_CHUNKS
+
+    model = PagedDecoder(Config(cache=cache, **LONG_CHUNKS))
+    c = model.config
+    size, count, pool = ctypes.c_int64(), ctypes.c_int64(), model.caches[0]
+    args = struct.pack("=21qd2q", 16, 16, 0, 16, 16, 16, 0, 0, c.rows, 1, c.q_heads, c.rows, 64, 64, c.q_heads * 128, 128, c.q_heads * 128, 128, 2, 1, 0,
+                       0.1, 0, 0) + pool._native[:15 * 8]
+    assert rt.library().tj_b200_paged_attention_workspace(args, ctypes.byref(size), ctypes.byref(count)) == rt.TJ_OK
+    sms = torch.cuda.get_device_properties(0).multi_processor_count
+    assert size.value == 2 * sms * 256 * (128 * 4 + 8)  # two parts of 256 rows a multiprocessor
+    gen = torch.Generator().manual_seed(4)
+    tokens = {s: torch.randint(0, 512, (n,), generator=gen).tolist() for s, n in ((0, 1013), (1, 140))}
+    want = {s: model.dense_logits(t) for s, t in tokens.items()}
+    at = dict.fromkeys(tokens, 0)
+    for new in ({0: 512}, {0: 372, 1: 140}, {0: 128}, {0: 1}):
+        got = model.step({s: tokens[s][at[s]:at[s] + n] for s, n in new.items()})
+        for i, (s, n) in enumerate(new.items()):
+            at[s] += n
+            assert (got[i] - want[s][at[s] - 1]).norm() <= tol * want[s][at[s] - 1].norm(), (s, at[s])
+    serving.check()
+    assert at == {s: len(t) for s, t in tokens.items()}
