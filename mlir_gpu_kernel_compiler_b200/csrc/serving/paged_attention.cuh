@@ -12,7 +12,8 @@
 // codes are exact in bf16 and f16, so they enter the matrix products as they are; ks multiplies the
 // score's column, and vs enters the exponent:  t = log2e * scale * ks * (q . code) + log2 vs,
 // P = 2^(t - m) with m the running maximum of t, and the sum adds P / vs.  So P, rounded to 16 bits
-// for the product with the codes, is at most 1 whatever the scales are.
+// for the product with the codes, is at most 1 whatever the scales are.  (The kernel of many rows does so for f16
+// queries only: bf16 has f32's range, and P is multiplied by vs.)
 #pragma once
 #include "serving_common.cuh"
 
@@ -32,9 +33,10 @@ struct AttnParams {
   int tile_ctas;     // CTAs of the kernel of many rows
 };
 
-// log2 vs, held at -80 or above: a row of zeros has vs = 0, and a key whose P = 2^(t - m) underflows f32
-// (2^-126) may be left out of the sum only if it is below 2^-46 of the largest.  Values under 127 * 2^-80 thus come
-// out up to that size.  A NaN (the scale of a row that is not finite) stays one.
+// log2 vs, held at -80 or above: a row of zeros has vs = 0, and a key whose P = 2^(t - m), or whose part of the sum as m
+// moves, underflows f32 (2^-126) has to weigh little.  Beside a key with the value scale v it may be lost below 2^-46 v of
+// that key's weight: below f32's rounding up to v = 2^20 (values of 1e8), which is the limit that callers are told.
+// Values under 127 * 2^-80 thus come out up to that size.  A NaN (the scale of a row that is not finite) stays one.
 TJ_DEV float log2_scale(float vs) { return vs == vs ? fmaxf(__log2f(vs), -80.0f) : vs; }
 
 struct Seq {

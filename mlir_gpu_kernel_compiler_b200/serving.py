@@ -226,7 +226,11 @@ def paged_attention(q, cache: PagedCache, page_table, kv_lens, q_starts=None, *,
     sees no key is 0; rows of no sequence are not written.  ``return_lse``: also the logarithm of each row's sum
     of exponentials, f32 ``[tokens, q_heads]`` (-inf for a row that sees no key).  Slots that no row of a
     sequence sees may hold anything; visible ones must be finite, as a NaN or an infinity reaches the
-    sequence's other rows too.
+    sequence's other rows too.  Value scales of an 8-bit cache up to 2**20 (values of 1e8) are exact to f32 beside any
+    others; beside larger ones the weights of keys with much smaller values may be lost.
+
+    A call needs a workspace (a partial result of 16 or 256 rows for each CTA, some MB to some hundred for thousands of
+    sequences), which is kept for each stream.
     """
     how = page_table, kv_lens, q_starts, max_new, scale, causal, window, return_lse, out
     got = _native.attention(_described(cache), q, *how)

@@ -853,3 +853,18 @@ def test_arguments_that_do_not_convert():
             call()
     with pytest.raises(OverflowError):
         serving.paged_attention(x, cache, slots[:, None], slots, window=2**63)
+
+
+@pytest.mark.parametrize("new", [1, 300])
+@pytest.mark.parametrize("dtype,top", [("bf16", 1e8), ("f16", 4e3)])
+@pytest.mark.parametrize("cache_dtype", ["i8", "e4m3"])
+def test_values_of_very_different_size_at_equal_scores(new, dtype, top, cache_dtype):
+    """Every third key's values are as large as is promised (scales of 2^20; f16 results end at 65504), the others' small or
+    zero, and all weigh the same."""
+    case = _case([(new, 700), (new, 2000), (new, new)], 8, 2, 128, dtype, cache_dtype, seed=46)
+    q, cache, table, lens, starts = case
+    for b, c in enumerate(lens.tolist()):
+        key = torch.arange(c, device="cuda")
+        v = _randn(c, 2, 128, seed=47 + b) * torch.tensor([top / 4, 0.0, 1e-3], device="cuda")[key % 3][:, None, None]
+        serving.cache_write(cache, _randn(c, 2, 128, seed=50 + b, scale=1e-6), v, table[b].long()[key // 16] * 16 + key % 16)
+    _agree(case, max_new=new)
