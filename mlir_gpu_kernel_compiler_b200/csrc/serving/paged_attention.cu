@@ -54,11 +54,16 @@ Plan plan(const tj_paged_attention& a, const Device& dev) {
   // Tokens of one tile of 16 rows take the kernel of few rows.  More do while it passes over less: it reads
   // the keys once for 16 rows, the other once for 256, but starts, joins and ends in 25 us more (16-bit
   // caches) or 30 (8-bit ones, whose keys it also converts, at four times the cost).  Few rows against many, us:
-  //   16-bit, dim 128  1 x 16 tokens over 4096 23, 39   1 x 32 44, 46   1 x 64 62, 58   1 x 256 163, 64
-  //                    8 x 16 over 2048 69, 42          16 x 8 over 8192 165, 124      1 x 300 over 300 32, 57
-  //   8-bit, dim 128   1 x 32 over 4096 37, 55          1 x 64 56, 68   1 x 128 84, 68
-  //                    8 x 16 over 2048 57, 57          16 x 8 over 8192 132, 232
-  //   16-bit, dim 64   1 x 32 over 4096 25, 33          1 x 64 40, 42   1 x 128 59, 42
+  //   16-bit, dim 128  1 x 16 tokens over 4096 22, 36   1 x 32 42, 44   1 x 64 61, 56   1 x 256 161, 62
+  //                    8 x 16 over 2048 68, 40          16 x 8 over 8192 163, 121
+  //   i8, dim 128      1 x 32 over 4096 38, 49          1 x 64 57, 64   1 x 128 86, 64
+  //                    8 x 16 over 2048 58, 48          16 x 8 over 8192 135, 190
+  //   e4m3, dim 128    1 x 32 over 4096 34, 48          1 x 64 52, 62   1 x 128 78, 63
+  //                    8 x 16 over 2048 54, 46          16 x 8 over 8192 118, 175
+  //   16-bit, dim 64   1 x 32 over 4096 25, 31          1 x 64 39, 39   1 x 128 59, 40
+  // Contexts that are not near 4096 keys are taken for that all the same, and get the slower kernel at both ends:
+  //   16-bit, dim 128  1 x 300 over 300 32, 56 (many)   1 x 32 over 32768 254, 71 (few)
+  //   i8, dim 128      1 x 300 over 300 31, 63 (many)   1 x 64 over 32768 238, 112 (few)
   const double keys = a.window > 0 ? static_cast<double>(a.window) + (known ? new_max : a.tokens / std::max<long>(a.batch, 1)) : 4096;
   const double pass = a.cache.heads * keys * static_cast<double>(a.cache.dim + 64) / 192;
   const double many_tiles = tiles_of(TILE_ROWS);
@@ -74,7 +79,7 @@ Plan plan(const tj_paged_attention& a, const Device& dev) {
   p.rows = 16;
   // Few row tiles are cut so that all pieces run at once, one CTA an SM (pieces: at most target + tiles).
   // Many uneven ones are cut for three waves of smaller CTAs, which even out what one wave does not.
-  // (One token over 777 keys 9.7 us in this way, 11.1 in the other; three over 100003 in 8 bits 59, 63.)
+  // (One token over 777 keys 10.5 us in this way, 11.1 in the other; three over 100003 in i8 56, 87, in e4m3 49, 83.)
   const double items = a.cache.heads * row_tiles;
   p.wide = items <= dev.sms / 2;
   p.target = p.wide ? dev.sms - static_cast<int>(items) : 3 * dev.sms * (q8 ? 3 : 2);

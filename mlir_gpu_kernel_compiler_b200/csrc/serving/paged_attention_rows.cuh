@@ -4,9 +4,9 @@
 // of its bytes at the most, far below the tensor cores' rate; so it is HBM, and the kernel has to keep
 // enough reads in flight.  Each warp has a ring of its own in shared memory (8 warps of 24 KB an SM, or
 // 12 of 16 KB for 8-bit caches, whose codes take more instructions) that asynchronous copies fill one or
-// more blocks ahead, so the main loop has no barrier.  64 single tokens over up to 8192 keys take 228 us, 96 % of
+// more blocks ahead, so the main loop has no barrier.  64 single tokens over up to 8192 keys take 231 us, 94 % of
 // the rate of a copy (with the loads straight into registers, where a block's are in flight only until
-// it is used, 387 us).  Three over up to 100003 keys of 8 bits take 53 us, 59 %.
+// it is used, 387 us).  Three over up to 100003 keys of i8 take 56 us, 57 %, of e4m3 49 us, 64 %.
 //
 // The order of the head dimension inside a product is free as long as both operands agree, so 16
 // bytes of a key serve a thread as its fragments of two (16-bit) or four (8-bit) steps, read with one
@@ -15,12 +15,13 @@
 // two keys' elements are paired by a byte permutation.  The pieces of a row are permuted by its number
 // so that both ways of reading are free of bank conflicts.
 //
-// An 8-bit cache's codes become f16, bf16 queries too (times a power of two that brings the largest element
-// near 2^14; f16 is exact to 2^-28 of that): the byte permutations and masks run
-// at half rate and were the bound, and bf16 needs three for a pair of codes where f16 needs 1.5 (keys) and
-// 2 (values).  The rows of a tile are different tokens and heads.  While their largest elements are within 2^12 of
-// one another they share the power, and no row loses more than 2^-16 - 2^-24 below its own largest, which is under
-// the f32 error of its score; otherwise each has its own, at a multiplication a score.
+// An 8-bit cache's codes become f16, bf16 queries too, times a power of two that brings the largest element
+// near 2^14: byte permutations and masks run at half rate, and of i8 codes bf16 needs three for a pair where f16
+// needs 1.5 (keys) and 2 (values); e4m3 has an instruction to f16.  The rows of a tile are different tokens and
+// heads.  While their largest elements are within 2^12 of one another they share the power: f16's step of 2^-24 then
+// leaves no element off by more than 2^-27 of its row's largest, less than f32 does in the score.  Otherwise each has
+// its own, at a multiplication a score.  (That loop beside the other costs three single tokens over 100003 i8
+// keys 56 us for 54: warps wait for instructions, 0.5 an issue.)
 //
 // A CTA's warps take blocks of KS keys of its chunk in turn, with a running maximum and sum each; their
 // results are joined at the end, and the chunks of a row tile by the CTA that

@@ -24,11 +24,11 @@
 //   14         looks the next segment up.
 //   15         of the first CTA: records faulty lengths and token ranges.
 //
-// Measured: 2048 tokens over 16384 bf16 keys, 32 heads of 128 on 8 cached ones, 493 us = 1045 TFLOP/s (64 % of
-// the measured matrix rate) in short runs and 568 us under the board's power limit, where variants that
-// need fewer clocks take as long.  Over i8 codes 820 us: the conversion is made again by every tile of a head,
-// and its instructions and the scales' (two products a score) share the schedulers with the softmax; left
-// out, in a timing build, they give 531.  Eight producer warps of 16 rows each were no help (884 us).
+// Measured: 2048 tokens over 16384 bf16 keys, 32 heads of 128 on 8 cached ones, 486 us = 1060 TFLOP/s (65 % of
+// the measured matrix rate) in short runs and 554 to 566 us under the board's power limit, where variants that
+// need fewer clocks take as long.  Over i8 codes 835 us, over e4m3 761: the conversion is made again by every tile of a
+// head, and its instructions and the scales' (two products a score) share the schedulers with the softmax; left
+// out, in a timing build, they give 531.  Eight producer warps of 16 rows each were no help (884 us for 820).
 //
 // The work, (tile, block) pairs of all sequences and heads in a row, is cut into as many equal parts as
 // there are SMs (each at least 512 keys): a CTA takes a tile's end, whole tiles and a tile's beginning.

@@ -113,7 +113,8 @@ template <class T, int CD> TJ_DEV void codes4(uint32_t w, uint32_t& lo, uint32_t
   }
 }
 
-// n / d for 0 <= n < 2^31 by a multiplication.
+// n / d for 0 <= n < 2^31 by a multiplication and a shift (Granlund and Montgomery 1994, "Division by invariant
+// integers using multiplication").
 struct Div {
   uint32_t mul, shift, d;
   Div() = default;
