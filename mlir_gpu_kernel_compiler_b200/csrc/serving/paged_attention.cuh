@@ -168,7 +168,8 @@ TJ_DEV float exp2_fast(float x) {
 }
 
 // P is made 2^shift times as large before it is rounded to 16 bits, and so is the sum: f16 has no
-// normal numbers below 2^-14, and a key whose probability is small can have the larger value.
+// normal numbers below 2^-14, and a key whose probability is small can have the larger value.  What is left of the
+// type's end: a key's part is off by at most 2^-39 of its value (2^-25 of 2^14), however small its probability.
 template <class T> constexpr float P_SHIFT = 0.0f;
 template <> constexpr float P_SHIFT<__half> = 14.0f;
 // So P = 2^(t - base), and a row's base is what the kernels keep in place of its maximum: the maximum less the shift,

@@ -868,3 +868,18 @@ def test_values_of_very_different_size_at_equal_scores(new, dtype, top, cache_dt
         v = _randn(c, 2, 128, seed=47 + b) * torch.tensor([top / 4, 0.0, 1e-3], device="cuda")[key % 3][:, None, None]
         serving.cache_write(cache, _randn(c, 2, 128, seed=50 + b, scale=1e-6), v, table[b].long()[key // 16] * 16 + key % 16)
     _agree(case, max_new=new)
+
+
+@pytest.mark.parametrize("dtype,cache_dtype", FORMS)
+@pytest.mark.parametrize("new", [1, 260])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_sharp_scores(dtype, cache_dtype, new, dim):
+    """Scores 2 q k: probabilities down to e^-100, and elements that only improbable keys have (codes of 0).  Besides the usual
+    bound, each of 400 keys is off by at most 2^-39 of its value where P is f16, and the scores' f32 error, for
+    scores of some 100, is 128 2^-24 of the sum of their products' sizes, 2 * 128."""
+    q, cache, table, lens, starts = _case([(new, 400), (1, 333), (min(new, 77), 77)], 6, 2, dim, dtype, cache_dtype, seed=60)
+    out = serving.paged_attention(q, cache, table, lens, starts, max_new=new, scale=2.0)
+    want, _, size = _attend64(q, cache, table, lens, starts, scale=2.0)
+    tail = 400 * 2.0**-39 * 6 if dtype == "f16" or cache_dtype in TOP else 0.0
+    off = (out.double() - want).abs() - (U[q.dtype] * (want.abs() + size) + 128 * 2.0**-24 * 256 * size + tail + (2.0**-25 if dtype == "f16" else 0))
+    assert (off <= 0).all(), off.max().item()
